@@ -1,0 +1,54 @@
+// Kernels of the gated feed-forward block that is trained in 8 bits (mx_train.hip) and what they are given.
+#pragma once
+#include "mx_common.h"
+
+namespace mx {
+
+// where a block's scale byte goes: [rows][blocks], or one of the layouts that the products read (mx_common.h)
+enum { kScalePlain = 0, kScaleNativeA = 1, kScaleNativeB = 2 };
+
+// quantisation of one matrix along its rows (q, s) and, transposed, along its columns (qt, st); either pair may be null
+struct BothTensor {
+  const void* x;
+  int64_t x_ld;                      // elements
+  uint8_t *q, *s, *qt, *st;
+  int64_t q_ld, s_ld, qt_ld, st_ld;  // bytes; s_ld, st_ld of plain scales
+  int32_t rows, K, x_dtype;
+  int32_t s_kind, st_kind;           // kScale*
+  // filled in by the launcher
+  int32_t first, tiles_k, vec;
+};
+constexpr int kBothMax = 3;
+struct BothArgs {
+  BothTensor t[kBothMax];
+  int32_t n, scale_mode;
+};
+// up to kBothMax matrices, all quantised to `fmt` (MX_E4M3, MX_E5M2): one launch per run of equal x_dtype
+int launch_quantize_both(const BothTensor* list, int n, int fmt, int scale_mode, hipStream_t stream);
+
+// [g|u] (bf16 [rows, 2 F]) -> silu(g) * u, as bf16 or quantised, and optionally [g|u] quantised to E4M3
+struct GateUpArgs {
+  const uint16_t* gu;
+  int64_t gu_ld;
+  void* h;                           // bf16 (h_fmt MX_BF16) or codes
+  uint8_t* hs;
+  uint8_t *c, *cs;                   // checkpoint; may be null
+  int64_t h_ld, hs_ld, c_ld, cs_ld;  // elements of h; bytes
+  int64_t rows;
+  int32_t F, h_fmt, scale_mode;
+};
+int launch_gate_up(const GateUpArgs& a, hipStream_t stream);
+
+// dh and the checkpoint [g|u] -> d[g|u] quantised along rows and columns, silu(g) * u along columns (all E4M3)
+struct SiluBackwardArgs {
+  const uint16_t* dh;                // bf16
+  const uint8_t *gu, *gus;
+  uint8_t *d, *ds, *dt, *dts, *at, *ats;
+  int64_t dh_ld, gu_ld, gus_ld, d_ld, ds_ld, dt_ld, dts_ld, at_ld, ats_ld;
+  int32_t rows, F, scale_mode;
+  int32_t ds_kind, dts_kind, ats_kind;   // kScale*; other than plain only with F % 64 == 0
+  int32_t tiles_k, vec;                  // filled in by the launcher
+};
+int launch_silu_backward(const SiluBackwardArgs& a, hipStream_t stream);
+
+}  // namespace mx

@@ -88,6 +88,18 @@ SYMBOLS = {
                                     ctypes.c_int64, ctypes.c_void_p]),
     "mx_quantize": (ctypes.c_int, [_P(MxTensor)] * 3 + [ctypes.c_int32, ctypes.c_void_p]),
     "mx_silu_mul_quantize": (ctypes.c_int, [_P(MxTensor)] * 3 + [ctypes.c_int32, ctypes.c_void_p]),
+    "mx_quantize_both": (ctypes.c_int, [_P(MxTensor)] * 5 + [ctypes.c_int32, ctypes.c_void_p]),
+    "mx_gated_gemm_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64] * 3 + [_P(MxGemmOpts)]),
+    "mx_gated_gemm": (ctypes.c_int, [_P(MxTensor)] * 8 + [ctypes.c_int32, _P(MxGemmOpts), ctypes.c_void_p, ctypes.c_int64,
+                                                         ctypes.c_void_p]),
+    "mx_silu_mul_backward_quantize": (ctypes.c_int, [_P(MxTensor)] * 9 + [ctypes.c_int32, ctypes.c_void_p]),
+    "mx_ffn_saved_bytes": (ctypes.c_int64, [ctypes.c_int64] * 4),
+    "mx_ffn_forward_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64] * 4),
+    "mx_ffn_backward_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64] * 4),
+    "mx_ffn_forward": (ctypes.c_int, [_P(MxTensor)] * 4 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                                          ctypes.c_int64, ctypes.c_void_p]),
+    "mx_ffn_backward": (ctypes.c_int, [_P(MxTensor), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]
+                        + [_P(MxTensor)] * 3 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
     "mx_probe_mfma_rate": (ctypes.c_int, [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
                                           ctypes.c_void_p, ctypes.c_void_p]),
     "mx_probe_rcp": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define MXGEMM_VERSION 105
+#define MXGEMM_VERSION 106
 
 /* Exported symbols (the library is built with hidden default visibility). */
 #if defined(__GNUC__)
@@ -331,6 +331,69 @@ MX_API int mx_moe_forward(const mx_tensor* X, const mx_tensor* Xs, const mx_tens
                    const mx_tensor* W2, const mx_tensor* W2s, const float* topk_weights, const void* topk_ids,
                    int32_t ids64, int32_t topk, mx_tensor* out, int32_t scale_mode, const mx_gemm_opts* opts,
                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * MX quantisation of a matrix along both of its axes, in one pass over it: what a product needs of it whose sum runs along its
+ * rows, and one whose sum runs along its columns (a weight's gradient sums over tokens).  No reference counterpart: the
+ * reference's block_quantize (test/kernels/kernel_utils.py:38-80) takes the last axis only.
+ *   x       [rows, K] MX_F32 | MX_BF16 | MX_F16, rows contiguous
+ *   xq      [rows, Kpad], scale [rows, Kpad/32]: as mx_quantize (Kpad = K rounded up to 32)
+ *   xt      [K, Rpad], scale_t [K, Rpad/32]: the same of the transposed matrix, Rpad = rows rounded up to 32, the tail zero
+ * xq and xt are both MX_E4M3 or both MX_E5M2; rows of xq start at multiples of 8 bytes, rows of xt at multiples of 16.
+ */
+MX_API int mx_quantize_both(const mx_tensor* x, mx_tensor* xq, mx_tensor* scale, mx_tensor* xt, mx_tensor* scale_t,
+                     int32_t scale_mode, void* stream);
+
+/*
+ * Both projections of a gated feed-forward block, the activation and the product:
+ *   [G|U] = bf16((A * As) @ (W * Ws).T),  out = silu(G) * U
+ * the gate_up GEMM of samples/MoE.py:197-288 followed by silu_and_mul_kernel (test/kernels/fused_moe.py:85-108), dense.
+ *   A [M,K], W [2F,K] (gate rows first; K contiguous), element formats, scales and layouts as in mx_gemm (Ws is
+ *   [2F,K/32]; opts->a_scale_layout / b_scale_layout are As's / Ws's); F % 32 == 0
+ *   out [M,F] MX_BF16 (out_scale NULL), or MX_E4M3 / MX_E5M2 with out_scale [M,F/32], as mx_silu_mul_quantize leaves it
+ *   gate_up [M,2F] MX_E4M3 with gate_up_scale [M,2F/32], optional (both NULL): [G|U] quantised, which is what
+ *   mx_silu_mul_backward_quantize takes (8.25 bits an element from the forward to the backward pass)
+ * Workspace: mx_gated_gemm_workspace_bytes().
+ */
+MX_API int64_t mx_gated_gemm_workspace_bytes(int64_t M, int64_t F, int64_t K, const mx_gemm_opts* opts);
+MX_API int mx_gated_gemm(const mx_tensor* A, const mx_tensor* A_scale, const mx_tensor* W, const mx_tensor* W_scale,
+                  mx_tensor* out, mx_tensor* out_scale, mx_tensor* gate_up, mx_tensor* gate_up_scale, int32_t scale_mode,
+                  const mx_gemm_opts* opts, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Backward pass of silu(g) * u from an 8-bit checkpoint of [g|u]: with s = 1 / (1 + exp(-g))
+ *   du = dh * g * s,  dg = dh * u * s * (1 + g * (1 - s)),  a = g * s * u
+ *   dh [rows,F] MX_BF16; gate_up [rows,2F] MX_E4M3 with gate_up_scale [rows,2F/32]; F % 32 == 0
+ *   d  [rows,2F], d_scale:  [dg|du] quantised along the rows, for dx = d @ w1
+ *   dt [2F,Rpad], dt_scale: its transposed form quantised along the tokens, for dw1 = d.T @ x
+ *   at [F,Rpad],  at_scale: the activation, recomputed and quantised along the tokens, for dw2 = dy.T @ a
+ * all MX_E4M3, layouts as in mx_quantize_both.
+ */
+MX_API int mx_silu_mul_backward_quantize(const mx_tensor* dh, const mx_tensor* gate_up, const mx_tensor* gate_up_scale,
+                                  mx_tensor* d, mx_tensor* d_scale, mx_tensor* dt, mx_tensor* dt_scale, mx_tensor* at,
+                                  mx_tensor* at_scale, int32_t scale_mode, void* stream);
+
+/*
+ * A gated feed-forward block and its backward pass, every product block-scaled (MXFP8 E4M3).  Q_r, Q_c: quantised along the
+ * rows, along the columns (the gradients of weights sum over tokens, those of inputs over features):
+ *   forward   [G|U] = bf16(Q_r(x) Q_r(w1)^T);  y = Q_r(silu(G) * U) Q_r(w2)^T
+ *   backward  dh = bf16(Q_r(dy) Q_c(w2));  d[G|U] and a as mx_silu_mul_backward_quantize, from Q_r([G|U])
+ *             dx = Q_r(d) Q_c(w1);  dw1 = Q_c(d)^T Q_c(x);  dw2 = Q_c(dy)^T Q_c(a)
+ *   x [T,H], w1 [2F,H] (gate rows first), w2 [H_out,F], dy [T,H_out]: MX_F32, MX_BF16 or MX_F16; y, dx, dw1, dw2 MX_F32 or
+ *   MX_BF16; rows contiguous; H, F and H_out multiples of 32
+ * `saved` (mx_ffn_saved_bytes(), NULL where no backward pass will follow) is what the forward pass leaves for the backward
+ * pass: Q_c(x), Q_r([G|U]), Q_c(w1), Q_c(w2).  The backward pass reads it only, and neither x nor the weights.  Of dx,
+ * dw1 and dw2 those that are not wanted may be NULL.  A T of zero is a valid forward pass and no valid backward pass.
+ * saved and workspace are aligned to 256 bytes.
+ */
+MX_API int64_t mx_ffn_saved_bytes(int64_t T, int64_t H, int64_t F, int64_t H_out);
+MX_API int64_t mx_ffn_forward_workspace_bytes(int64_t T, int64_t H, int64_t F, int64_t H_out);
+MX_API int64_t mx_ffn_backward_workspace_bytes(int64_t T, int64_t H, int64_t F, int64_t H_out);
+MX_API int mx_ffn_forward(const mx_tensor* x, const mx_tensor* w1, const mx_tensor* w2, mx_tensor* y, int32_t scale_mode,
+                   void* saved, int64_t saved_bytes, void* workspace, int64_t workspace_bytes, void* stream);
+MX_API int mx_ffn_backward(const mx_tensor* dy, const void* saved, int64_t saved_bytes, int64_t H, int64_t F, mx_tensor* dx,
+                    mx_tensor* dw1, mx_tensor* dw2, int32_t scale_mode, void* workspace, int64_t workspace_bytes,
+                    void* stream);
 
 /*
  * Re-lays a scale tensor into an MFMA-ready native layout consumed by the MFMA kernels
