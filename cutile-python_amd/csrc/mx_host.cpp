@@ -10,6 +10,8 @@
 // Scratch comes from the caching allocator on every call and goes back to it when the call returns: blocks are reused
 // in stream order, so calls from several threads and streams, and graph captures, need no rule of their own.
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/Context.h>
@@ -18,6 +20,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 
@@ -39,6 +42,16 @@ struct Lib {
   MX_FN(mx_silu_mul_quantize);
   MX_FN(mx_moe_forward);
   MX_FN(mx_moe_forward_workspace_bytes);
+  MX_FN(mx_last_error);
+  MX_FN(mx_quantize_both);
+  MX_FN(mx_gated_gemm);
+  MX_FN(mx_gated_gemm_workspace_bytes);
+  MX_FN(mx_silu_mul_backward_quantize);
+  MX_FN(mx_ffn_saved_bytes);
+  MX_FN(mx_ffn_forward);
+  MX_FN(mx_ffn_forward_workspace_bytes);
+  MX_FN(mx_ffn_backward);
+  MX_FN(mx_ffn_backward_workspace_bytes);
 } lib;
 #undef MX_FN
 PyObject* packed_type = nullptr;   // ops.PackedScales
@@ -410,6 +423,298 @@ PyObject* py_moe(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return rc_or(rc, out);
 }
 
+// ---- the feed-forward block that is trained in 8 bits -----------------------------------------------------------------------------
+int float_code(at::ScalarType t) { return t == at::kFloat ? MX_F32 : t == at::kBFloat16 ? MX_BF16 : t == at::kHalf ? MX_F16 : -1; }
+inline int64_t up32(int64_t n) { return (n + 31) / 32 * 32; }
+
+// a tensor of two or more dimensions as [rows, last axis] with contiguous rows; false: it is no such matrix without a copy
+bool matrix(const at::Tensor& t, int dtype, mx_tensor* d) {
+  const int nd = (int)t.dim();
+  if (nd < 1 || dtype < 0) return false;
+  const int64_t cols = t.size(-1);
+  if (cols == 0 || t.numel() == 0) return false;
+  int64_t ld = cols;
+  if (nd == 2 && t.stride(1) == 1 && t.stride(0) >= 0) ld = t.stride(0);
+  else if (!t.is_contiguous()) return false;
+  *d = mx_tensor{t.data_ptr(), dtype, 2, {t.numel() / cols, cols, 0, 0}, {ld, 1, 0, 0}, -1, 0};
+  return true;
+}
+// room for elements and scales of a [rows, cols] matrix, cols a multiple of 32
+struct Codes {
+  at::Tensor q, s;
+  mx_tensor dq, ds;
+  Codes() = default;
+  Codes(int64_t rows, int64_t cols, int fmt, const at::Device& dev)
+      : q(device_empty({rows, cols}, fmt == MX_E5M2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn, dev)),
+        s(device_empty({rows, cols / 32}, at::kFloat8_e8m0fnu, dev)), dq(desc(q, fmt)), ds(desc(s, MX_E8M0)) {}
+};
+int format_of(PyObject* o) {   // an 8-bit format given as dtype or name
+  if (THPDtype_Check(o)) {
+    const auto t = ((THPDtype*)o)->scalar_type;
+    return t == at::kFloat8_e4m3fn ? MX_E4M3 : t == at::kFloat8_e5m2 ? MX_E5M2 : -1;
+  }
+  if (!PyUnicode_Check(o)) return -1;
+  return PyUnicode_CompareWithASCIIString(o, "e4m3") == 0 ? MX_E4M3 : PyUnicode_CompareWithASCIIString(o, "e5m2") == 0 ? MX_E5M2 : -1;
+}
+PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
+  PyObject* res = PyTuple_New((Py_ssize_t)ts.size());
+  if (!res) return nullptr;
+  Py_ssize_t i = 0;
+  for (const auto& t : ts) {
+    PyObject* o = THPVariable_Wrap(t);
+    if (!o) { Py_DECREF(res); return nullptr; }
+    PyTuple_SET_ITEM(res, i++, o);
+  }
+  return res;
+}
+
+// quantize_both(x, dtype | str, mode) -> (x_q, scale, xt_q, scale_t), error code, or None
+PyObject* py_quantize_both(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 3) { PyErr_SetString(PyExc_TypeError, "quantize_both takes 3 arguments"); return nullptr; }
+  if (!THPVariable_Check(a[0])) Py_RETURN_NONE;
+  const at::Tensor& x = THPVariable_Unpack(a[0]);
+  const int fmt = format_of(a[1]);
+  mx_tensor dx;
+  if (fmt < 0 || !on_current_device(x) || !matrix(x, float_code(x.scalar_type()), &dx) || dx.shape[1] < 32) Py_RETURN_NONE;
+  const at::Device dev = x.device();
+  const int64_t rows = dx.shape[0], K = dx.shape[1];
+  Codes r(rows, up32(K), fmt, dev), t(K, up32(rows), fmt, dev);
+  const int mode = (int)PyLong_AsLong(a[2]);
+  int rc;
+  {
+    NoGil nogil;
+    rc = lib.p_mx_quantize_both(&dx, &r.dq, &r.ds, &t.dq, &t.ds, mode, stream_of(dev));
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  if (x.dim() != 2) {
+    auto shape = x.sizes().vec();
+    shape.back() = up32(K);
+    r.q = r.q.view(shape);
+    shape.back() = up32(K) / 32;
+    r.s = r.s.view(shape);
+  }
+  return tuple_of({r.q, r.s, t.q, t.s});
+}
+
+// gated(A, A_scale, W, W_scale, a_format, w_format, out_dtype, mode, checkpoint, kernel) -> result or tuple, error code, or None
+PyObject* py_gated(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10) { PyErr_SetString(PyExc_TypeError, "gated takes 10 arguments"); return nullptr; }
+  if (!THPVariable_Check(a[0]) || !THPVariable_Check(a[2])) Py_RETURN_NONE;
+  const at::Tensor &A = THPVariable_Unpack(a[0]), &W = THPVariable_Unpack(a[2]);
+  if (A.dim() != 2 || W.dim() != 2 || !on_current_device(A) || W.device() != A.device()) Py_RETURN_NONE;
+  const int fa = elem_format(A, a[4]), fw = elem_format(W, a[5]);
+  if (fa < 0 || fw < 0 || A.stride(1) != 1 || W.stride(1) != 1) Py_RETURN_NONE;
+  const at::Device dev = A.device();
+  const mx_tensor dA = desc(A, fa, fa == MX_E2M1 ? 1 : -1), dW = desc(W, fw, fw == MX_E2M1 ? 1 : -1);
+  const int64_t M = dA.shape[0], K = dA.shape[1], N = dW.shape[0], F = N / 2;
+  if (M == 0 || K == 0 || dW.shape[1] != K || N == 0 || N % 64 != 0) Py_RETURN_NONE;
+  mx_tensor dAs, dWs;
+  mx_gemm_opts o = {sizeof(mx_gemm_opts), 0, 0, 0, (int32_t)PyLong_AsLong(a[9]), 32, 0, 0};
+  if (!scale_desc(a[1], M, K, false, dev, &dAs, &o.a_scale_layout) || !scale_desc(a[3], N, K, true, dev, &dWs, &o.b_scale_layout)) Py_RETURN_NONE;
+  const bool bf16 = THPDtype_Check(a[6]) && ((THPDtype*)a[6])->scalar_type == at::kBFloat16;
+  const int fo = bf16 ? MX_BF16 : format_of(a[6]);
+  const int mode = (int)PyLong_AsLong(a[7]), keep = PyObject_IsTrue(a[8]);
+  if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  if (fo < 0) Py_RETURN_NONE;
+  Codes h, c;
+  if (bf16) {
+    h.q = device_empty({M, F}, at::kBFloat16, dev);
+    h.dq = desc(h.q, MX_BF16);
+  } else {
+    h = Codes(M, F, fo, dev);
+  }
+  if (keep) c = Codes(M, N, MX_E4M3, dev);
+  const int64_t need = lib.p_mx_gated_gemm_workspace_bytes(M, F, K, &o);
+  at::Tensor ws;
+  if (need > 0) ws = device_empty({need}, at::kByte, dev);
+  int rc;
+  {
+    NoGil nogil;
+    rc = lib.p_mx_gated_gemm(&dA, &dAs, &dW, &dWs, &h.dq, bf16 ? nullptr : &h.ds, keep ? &c.dq : nullptr, keep ? &c.ds : nullptr, mode, &o,
+                             need > 0 ? ws.data_ptr() : nullptr, need, stream_of(dev));
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  if (bf16) return keep ? tuple_of({h.q, c.q, c.s}) : THPVariable_Wrap(h.q);
+  return keep ? tuple_of({h.q, h.s, c.q, c.s}) : tuple_of({h.q, h.s});
+}
+
+// silu_backward(dh, gate_up_q, gate_up_scale, mode) -> (d, its scales, dt, .., at, ..), error code, or None
+PyObject* py_silu_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4) { PyErr_SetString(PyExc_TypeError, "silu_backward takes 4 arguments"); return nullptr; }
+  for (int i = 0; i < 3; ++i)
+    if (!THPVariable_Check(a[i])) Py_RETURN_NONE;
+  const at::Tensor &dh = THPVariable_Unpack(a[0]), &gu = THPVariable_Unpack(a[1]), &gus = THPVariable_Unpack(a[2]);
+  const at::Device dev = dh.device();
+  if (!on_current_device(dh) || gu.device() != dev || gus.device() != dev || dh.dim() != 2 || gu.dim() != 2 || gus.dim() != 2) Py_RETURN_NONE;
+  mx_tensor dd, dg, ds;
+  if (dh.scalar_type() != at::kBFloat16 || gu.scalar_type() != at::kFloat8_e4m3fn || !is_e8m0(gus) || !matrix(dh, MX_BF16, &dd) ||
+      !matrix(gu, MX_E4M3, &dg) || !matrix(gus, MX_E8M0, &ds))
+    Py_RETURN_NONE;
+  const int64_t M = dd.shape[0], F = dd.shape[1];
+  if (F % 32 != 0 || dg.shape[0] != M || dg.shape[1] != 2 * F || ds.shape[0] != M || ds.shape[1] != F / 16 || (uintptr_t)dg.ptr % 8 != 0 ||
+      (M > 1 && dg.stride[0] % 8 != 0))
+    Py_RETURN_NONE;
+  Codes d(M, 2 * F, MX_E4M3, dev), t(2 * F, up32(M), MX_E4M3, dev), act(F, up32(M), MX_E4M3, dev);
+  const int mode = (int)PyLong_AsLong(a[3]);
+  int rc;
+  {
+    NoGil nogil;
+    rc = lib.p_mx_silu_mul_backward_quantize(&dd, &dg, &ds, &d.dq, &d.ds, &t.dq, &t.ds, &act.dq, &act.ds, mode, stream_of(dev));
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  return tuple_of({d.q, d.s, t.q, t.s, act.q, act.s});
+}
+
+struct Refused { int rc; };   // by the library, before anything was enqueued
+struct FfnSizes { int64_t T, H, F, Ho; };
+// the block's operands as matrices; false: not for the native path
+bool ffn_operands(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, mx_tensor* dx, mx_tensor* d1, mx_tensor* d2, FfnSizes* s) {
+  if (!on_current_device(x) || w1.device() != x.device() || w2.device() != x.device() || x.dim() < 2 || w1.dim() != 2 || w2.dim() != 2 ||
+      out_code(x.scalar_type()) < 0 || out_code(w1.scalar_type()) < 0 || out_code(w2.scalar_type()) < 0)
+    return false;
+  if (!matrix(x, out_code(x.scalar_type()), dx) || !matrix(w1, out_code(w1.scalar_type()), d1) || !matrix(w2, out_code(w2.scalar_type()), d2)) return false;
+  *s = {dx->shape[0], dx->shape[1], d1->shape[0] / 2, d2->shape[0]};
+  return d1->shape[0] % 2 == 0 && d1->shape[1] == s->H && d2->shape[1] == s->F && s->H % 32 == 0 && s->F % 32 == 0 && s->Ho % 32 == 0;
+}
+// y, and where `saved` is given what the backward pass needs
+at::Tensor ffn_forward(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, int mode, at::Tensor* saved) {
+  mx_tensor dx, d1, d2;
+  FfnSizes s;
+  if (!ffn_operands(x, w1, w2, &dx, &d1, &d2, &s)) throw Refused{0};
+  const at::Device dev = x.device();
+  auto shape = x.sizes().vec();
+  shape.back() = s.Ho;
+  at::Tensor y = device_empty(shape, x.scalar_type(), dev);
+  mx_tensor dy{y.data_ptr(), out_code(y.scalar_type()), 2, {s.T, s.Ho, 0, 0}, {s.Ho, 1, 0, 0}, -1, 0};
+  const int64_t kept = saved ? lib.p_mx_ffn_saved_bytes(s.T, s.H, s.F, s.Ho) : 0, need = lib.p_mx_ffn_forward_workspace_bytes(s.T, s.H, s.F, s.Ho);
+  if (saved) *saved = device_empty({kept}, at::kByte, dev);
+  at::Tensor ws = device_empty({need}, at::kByte, dev);
+  const int rc = lib.p_mx_ffn_forward(&dx, &d1, &d2, &dy, mode, saved ? saved->data_ptr() : nullptr, kept, ws.data_ptr(), need, stream_of(dev));
+  if (rc != MX_OK) throw Refused{rc};
+  return y;
+}
+// dx, dw1, dw2 (undefined where not asked for) from dy [T, Ho]
+std::vector<at::Tensor> ffn_backward(const at::Tensor& dy, const at::Tensor& saved, const FfnSizes& s, const at::ScalarType (&types)[3], const bool (&want)[3],
+                                     int mode) {
+  const at::Device dev = dy.device();
+  mx_tensor d{};
+  if (!matrix(dy, float_code(dy.scalar_type()), &d)) throw Refused{0};
+  const int64_t rows[3] = {s.T, 2 * s.F, s.Ho}, cols[3] = {s.H, s.H, s.F};
+  std::vector<at::Tensor> out(3);
+  mx_tensor od[3];
+  for (int i = 0; i < 3; ++i)
+    if (want[i]) {
+      out[i] = device_empty({rows[i], cols[i]}, types[i], dev);
+      od[i] = desc(out[i], out_code(types[i]));
+    }
+  const int64_t need = lib.p_mx_ffn_backward_workspace_bytes(s.T, s.H, s.F, s.Ho);
+  at::Tensor ws = device_empty({need}, at::kByte, dev);
+  const int rc = lib.p_mx_ffn_backward(&d, saved.data_ptr(), saved.numel(), s.H, s.F, want[0] ? &od[0] : nullptr, want[1] ? &od[1] : nullptr,
+                                       want[2] ? &od[2] : nullptr, mode, ws.data_ptr(), need, stream_of(dev));
+  if (rc != MX_OK) throw Refused{rc};
+  return out;
+}
+
+struct FeedForward : torch::autograd::Function<FeedForward> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, int64_t mode) {
+    at::Tensor saved;
+    at::Tensor y = ffn_forward(x, w1, w2, (int)mode, &saved);
+    ctx->save_for_backward({saved});
+    ctx->saved_data["x"] = x.sizes().vec();
+    ctx->saved_data["sizes"] = std::vector<int64_t>{x.numel() / x.size(-1), x.size(-1), w2.size(1), w2.size(0), mode, (int64_t)x.scalar_type(),
+                                                    (int64_t)w1.scalar_type(), (int64_t)w2.scalar_type()};
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const bool again = at::GradMode::is_enabled();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto v = ctx->saved_data["sizes"].toIntVector();
+    const at::ScalarType types[3] = {(at::ScalarType)v[5], (at::ScalarType)v[6], (at::ScalarType)v[7]};
+    const bool want[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)};
+    at::Tensor dy = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({v[0], v[3]});
+    if (dy.stride(1) != 1 || dy.stride(0) < 0) dy = dy.contiguous();
+    std::vector<at::Tensor> r;
+    try {
+      r = ffn_backward(dy, ctx->get_saved_variables()[0], {v[0], v[1], v[2], v[3]}, types, want, (int)v[4]);
+    } catch (const Refused& e) {
+      TORCH_CHECK(false, "gated_feed_forward, backward pass: ", e.rc ? lib.p_mx_last_error() : "unexpected gradient");
+    }
+    const auto shape = ctx->saved_data["x"].toIntVector();
+    if (want[0] && shape.size() != 2) r[0] = r[0].view(shape);
+    if (again)   // asked for a graph of the gradients: there is none
+      r = torch::autograd::DelayedError("gated_feed_forward: its gradients cannot be differentiated", 3)(std::move(r));
+    r.emplace_back();
+    return r;
+  }
+};
+
+// feed_forward(x, w1, w2, mode, form) -> result, error code, or None.  form 0: y without a backward pass; 1: (y, state for
+// feed_forward_backward); 2: y that autograd differentiates, not under graph capture
+PyObject* py_feed_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 5) { PyErr_SetString(PyExc_TypeError, "feed_forward takes 5 arguments"); return nullptr; }
+  for (int i = 0; i < 3; ++i)
+    if (!THPVariable_Check(a[i])) Py_RETURN_NONE;
+  const at::Tensor &x = THPVariable_Unpack(a[0]), &w1 = THPVariable_Unpack(a[1]), &w2 = THPVariable_Unpack(a[2]);
+  mx_tensor dx, d1, d2;
+  FfnSizes s;
+  if (!ffn_operands(x, w1, w2, &dx, &d1, &d2, &s)) Py_RETURN_NONE;
+  const int mode = (int)PyLong_AsLong(a[3]), form = (int)PyLong_AsLong(a[4]);
+  if (form == 2 && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) Py_RETURN_NONE;
+  at::Tensor y, saved;
+  int rc = MX_OK;
+  {
+    NoGil nogil;
+    try {
+      if (form == 2) {
+        y = FeedForward::apply(x, w1, w2, (int64_t)mode);
+      } else {
+        at::AutoDispatchBelowADInplaceOrView below;
+        y = ffn_forward(x, w1, w2, mode, form == 1 ? &saved : nullptr);
+      }
+    } catch (const Refused& e) {
+      rc = e.rc;
+    }
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  return form == 1 ? tuple_of({y, saved}) : THPVariable_Wrap(y);
+}
+
+// feed_forward_backward(dy, saved, T, H, F, H_out, x_dtype, w1_dtype, w2_dtype, need_dx, need_dw1, need_dw2, mode)
+//   -> [dx [T, H], dw1, dw2] with None where not asked for, error code, or None
+PyObject* py_feed_forward_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 13) { PyErr_SetString(PyExc_TypeError, "feed_forward_backward takes 13 arguments"); return nullptr; }
+  if (!THPVariable_Check(a[0]) || !THPVariable_Check(a[1])) Py_RETURN_NONE;
+  const at::Tensor &dy = THPVariable_Unpack(a[0]), &saved = THPVariable_Unpack(a[1]);
+  const FfnSizes s = {PyLong_AsLongLong(a[2]), PyLong_AsLongLong(a[3]), PyLong_AsLongLong(a[4]), PyLong_AsLongLong(a[5])};
+  at::ScalarType types[3];
+  bool want[3];
+  for (int i = 0; i < 3; ++i) {
+    if (!THPDtype_Check(a[6 + i])) Py_RETURN_NONE;
+    types[i] = ((THPDtype*)a[6 + i])->scalar_type;
+    want[i] = PyObject_IsTrue(a[9 + i]) == 1;
+    if (out_code(types[i]) < 0) Py_RETURN_NONE;
+  }
+  const int mode = (int)PyLong_AsLong(a[12]);
+  if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  mx_tensor d;
+  if (dy.dim() < 2 || !on_current_device(dy) || saved.device() != dy.device() || !matrix(dy, float_code(dy.scalar_type()), &d) || d.shape[0] != s.T || d.shape[1] != s.Ho ||
+      !saved.is_contiguous() || saved.scalar_type() != at::kByte)
+    Py_RETURN_NONE;
+  std::vector<at::Tensor> r;
+  int rc = MX_OK;
+  {
+    NoGil nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    try {
+      r = ffn_backward(dy, saved, s, types, want, mode);
+    } catch (const Refused& e) {
+      rc = e.rc;
+    }
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  return tuple_of({r[0], r[1], r[2]});
+}
+
 // bind(handle of the loaded libmxgemm.so, PackedScales class)
 PyObject* py_bind(PyObject*, PyObject* args) {
   unsigned long long h;
@@ -430,6 +735,16 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   MX_FN(mx_silu_mul_quantize)
   MX_FN(mx_moe_forward)
   MX_FN(mx_moe_forward_workspace_bytes)
+  MX_FN(mx_last_error)
+  MX_FN(mx_quantize_both)
+  MX_FN(mx_gated_gemm)
+  MX_FN(mx_gated_gemm_workspace_bytes)
+  MX_FN(mx_silu_mul_backward_quantize)
+  MX_FN(mx_ffn_saved_bytes)
+  MX_FN(mx_ffn_forward)
+  MX_FN(mx_ffn_forward_workspace_bytes)
+  MX_FN(mx_ffn_backward)
+  MX_FN(mx_ffn_backward_workspace_bytes)
 #undef MX_FN
   Py_INCREF(cls);
   Py_XDECREF(packed_type);
@@ -452,6 +767,11 @@ PyMethodDef methods[] = {
     {"mma", (PyCFunction)(void (*)(void))guarded<py_mma>, METH_FASTCALL, nullptr},
     {"quantize", (PyCFunction)(void (*)(void))guarded<py_quantize>, METH_FASTCALL, nullptr},
     {"moe", (PyCFunction)(void (*)(void))guarded<py_moe>, METH_FASTCALL, nullptr},
+    {"quantize_both", (PyCFunction)(void (*)(void))guarded<py_quantize_both>, METH_FASTCALL, nullptr},
+    {"gated", (PyCFunction)(void (*)(void))guarded<py_gated>, METH_FASTCALL, nullptr},
+    {"silu_backward", (PyCFunction)(void (*)(void))guarded<py_silu_backward>, METH_FASTCALL, nullptr},
+    {"feed_forward", (PyCFunction)(void (*)(void))guarded<py_feed_forward>, METH_FASTCALL, nullptr},
+    {"feed_forward_backward", (PyCFunction)(void (*)(void))guarded<py_feed_forward_backward>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mxhost", nullptr, -1, methods};
 

@@ -95,6 +95,11 @@ def block_quantize_both(x: torch.Tensor, dtype=torch.float8_e4m3fn, *, scale_mod
     backward pass, ``xt_q`` is a checkpoint of 8.25 bits an element.  ``dtype``: ``torch.float8_e4m3fn`` or
     ``torch.float8_e5m2`` for both; ``scale_mode`` as in :func:`block_quantize`."""
     mode = _mode(scale_mode)
+    r = L.host().quantize_both(x, dtype, mode)
+    if type(r) is tuple:
+        return r
+    if r is not None:
+        _raise_code(r)
     fmt = dtype if isinstance(dtype, str) else _DTYPE_FMT.get(dtype)
     if fmt not in _ELEM8:
         raise TileTypeError(f"Unsupported quantisation dtype {dtype} for block_quantize_both, expected float8_e4m3fn or "
@@ -130,6 +135,12 @@ def gated_block_scaled_matmul(A: torch.Tensor, A_scale, W: torch.Tensor, W_scale
     projection.  With ``checkpoint`` also ``(gate_up_q, gate_up_scale)``, [G | U] in MXFP8 E4M3, which is all that
     :func:`silu_and_mul_backward_quantize` needs of the forward pass."""
     mode = _mode(scale_mode)
+    if kernel in L.KERNELS:
+        r = L.host().gated(A, A_scale, W, W_scale, a_format, w_format, out_dtype, mode, checkpoint, L.KERNELS[kernel])
+        if type(r) is int:
+            _raise_code(r)
+        if r is not None:
+            return r
     a_fmt, w_fmt = _elem_format(A, a_format), _elem_format(W, w_format)
     if a_fmt is None or w_fmt is None:
         bad = A if a_fmt is None else W
@@ -185,6 +196,11 @@ def silu_and_mul_backward_quantize(dh: torch.Tensor, gate_up_q: torch.Tensor, ga
     ``dx = d @ w1``, transposed along the tokens (2F, R) for ``dw1 = d.T @ x``, and the activation, recomputed, transposed
     along the tokens (F, R) for ``dw2 = dy.T @ a``; R is M rounded up to a multiple of 32, the tail zero."""
     mode = _mode(scale_mode)
+    r = L.host().silu_backward(dh, gate_up_q, gate_up_scale, mode)
+    if type(r) is tuple:
+        return r
+    if r is not None:
+        _raise_code(r)
     if dh.dtype != torch.bfloat16:
         raise TileTypeError(f"Unsupported gradient dtype {_dtype_name(dh.dtype)}, expected bfloat16")
     if gate_up_q.dtype not in (torch.float8_e4m3fn, torch.uint8) or _scale_code(gate_up_scale) != L.MX_E8M0:
@@ -241,6 +257,11 @@ def _check_block(x, w1, w2):
 
 
 def _forward(x, w1, w2, mode: int, train: bool):
+    r = L.host().feed_forward(x, w1, w2, mode, 1 if train else 0)
+    if type(r) is int:
+        _raise_code(r)
+    if r is not None:
+        return r if train else (r, None)
     dev, H, F, H_out = _check_block(x, w1, w2)
     x2, w1, w2 = _rows(x.detach()), _rows(w1.detach()), _rows(w2.detach())
     T = x2.shape[0]
@@ -269,6 +290,12 @@ def gated_feed_forward_backward(dy: torch.Tensor, state: FeedForwardState, *, ne
     in the dtypes of x, w1 and w2 (``dx`` in the shape of ``dy`` but for its last axis); None where not asked for.  Reads the state and
     leaves it as it is, so it can be called again with another ``dy``."""
     s = state
+    r = L.host().feed_forward_backward(dy, s.saved, s.T, s.H, s.F, s.H_out, s.x_dtype, s.w1_dtype, s.w2_dtype, need_dx, need_dw1,
+                                       need_dw2, _mode(s.scale_mode))
+    if type(r) is tuple:
+        return r if dy.dim() == 2 or not need_dx else (r[0].view(*dy.shape[:-1], s.H), r[1], r[2])
+    if r is not None:
+        _raise_code(r)
     if dy.dtype not in _FLOATS:
         raise TileTypeError(f"Unsupported gradient dtype {_dtype_name(dy.dtype)}, expected float32, bfloat16 or float16")
     if dy.dim() < 2 or dy.shape[-1] != s.H_out or dy.numel() != s.T * s.H_out:
@@ -320,6 +347,11 @@ def gated_feed_forward(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, *, s
     mode = _mode(scale_mode)
     if not (torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad)):
         return _forward(x, w1, w2, mode, False)[0]
+    r = L.host().feed_forward(x, w1, w2, mode, 2)
+    if type(r) is int:
+        _raise_code(r)
+    if r is not None:
+        return r
     if x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("gated_feed_forward with gradients cannot be captured into a graph: capture "
                            "gated_feed_forward_forward and gated_feed_forward_backward")
