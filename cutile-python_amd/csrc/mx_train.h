@@ -16,7 +16,7 @@ struct BothTensor {
   int32_t rows, K, x_dtype;
   int32_t s_kind, st_kind;           // kScale*
   // filled in by the launcher
-  int32_t first, tiles_k, vec;
+  int32_t first, tiles, tiles_k;
 };
 constexpr int kBothMax = 3;
 struct BothArgs {
@@ -47,7 +47,7 @@ struct SiluBackwardArgs {
   int64_t dh_ld, gu_ld, gus_ld, d_ld, ds_ld, dt_ld, dts_ld, at_ld, ats_ld;
   int32_t rows, F, scale_mode;
   int32_t ds_kind, dts_kind, ats_kind;   // kScale*; other than plain only with F % 64 == 0
-  int32_t tiles_k, vec;                  // filled in by the launcher
+  int32_t tiles_k;                       // filled in by the launcher
 };
 int launch_silu_backward(const SiluBackwardArgs& a, hipStream_t stream);
 
