@@ -1582,3 +1582,61 @@ int mx_silu_mul_quantize(const mx_tensor* gate_up, mx_tensor* xq, mx_tensor* sca
 }
 
 }  // extern "C"
+
+namespace mx {
+// A gated product on the ping-pong kernel, whose epilogue makes of gate and up what is asked for.  kGatedNotFused: it goes through
+// memory instead (nothing enqueued).  W [2 F, K]; the scales as o's layouts say, of W's rows.
+int gemm_gated_fused(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const GateOut& out, const mx_gemm_opts& o,
+                     void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  const int64_t M = A.shape[0], K = A.shape[1], N = W.shape[0];
+  if ((o.kernel != MX_KERNEL_AUTO && o.kernel != MX_KERNEL_MFMA_PINGPONG) || o.block_size != 32 || o.split_k > 1) return kGatedNotFused;
+  if (N != 2 * (int64_t)out.F || out.F % 64 != 0 || out.scale_mode != 1 || (out.h_fmt != MX_BF16 && out.h_fmt != MX_E4M3)) return kGatedNotFused;
+  if (!pair_supported_by_mfma(A.dtype, W.dtype) || As.dtype != MX_E8M0 || Ws.dtype != MX_E8M0 || K == 0 || K % 32 != 0 || W.shape[1] != K ||
+      M >= (1 << 30) || N >= (1 << 30) || K >= (1 << 30))
+    return kGatedNotFused;
+  if (mfma_operand_issue(A.ptr, M, K, A.stride[0], A.stride[1], A.dtype, A.packed_dim == 1) ||
+      mfma_operand_issue(W.ptr, N, K, W.stride[0], W.stride[1], W.dtype, W.packed_dim == 1))
+    return kGatedNotFused;
+  for (const int32_t l : {o.a_scale_layout, o.b_scale_layout})
+    if (l != MX_SCALE_2D && l != MX_SCALE_NATIVE && l != MX_SCALE_SWIZZLE_32_4_4) return kGatedNotFused;
+  const bool fp4 = A.dtype == MX_E2M1, pack_a = o.a_scale_layout != MX_SCALE_NATIVE, pack_w = o.b_scale_layout != MX_SCALE_NATIVE;
+  const PpRows pp = pp_rows(M, N, K, fp4, pack_a || pack_w, false);
+  if (o.kernel == MX_KERNEL_AUTO) {
+    if (M <= kStreamAutoM) return kGatedNotFused;
+    // through memory: the faster of the two kernels, then a pass over 4 bytes an element of gate and up read, up to 3 written.
+    // us, through memory | in one kernel, packed scales, E4M3 out: K 2048, F 7168, 512, 768, 1024, 2048 rows 25 | 26, 38 | 27, 41 | 33, 68 | 58;
+    // K 4096, F 14336, 256, 512, 1024, 2048 rows 39 | 40, 61 | 51, 108 | 95, 208 | 184; K 4096, F 4096, 512, 1024, 2048 rows 26 | 37,
+    // 40 | 39, 63 | 55; K 1024, F 2048, 1024, 1531 rows 17 | 20, 22 | 20; K 512, F 8192, 512, 1024 rows 18 | 17, 28 | 20
+    float us = est_t128(M, N, K, plan_k_splits(M, N, K, o), fp4, W.dtype == MX_E2M1);
+    const float split = est_pp(M, N, K, fp4, pack_a || pack_w, true);
+    if (split < us) us = split;
+    if (pp.us < us) us = pp.us;
+    us += 3.f + (float)M * out.F * (4.f + (out.h_fmt == MX_BF16 ? 2.f : 1.f) + (out.c ? 2.f : 0.f)) / 5.2e6f;
+    if (pp.us * 1.05f + 1.f > us) return kGatedNotFused;
+  }
+  uint8_t* ws = (uint8_t*)workspace;
+  PackArgs pa, pb;
+  const int64_t need = (pack_a ? mx_packed_scale_bytes(M, K) : 0) + (pack_w ? mx_packed_scale_bytes(N, K) : 0);
+  if (need > 0 && (!ws || workspace_bytes < need || ((uintptr_t)ws) % 256 != 0)) return kGatedNotFused;   // (reported by the other form)
+  const uint32_t *as = (const uint32_t*)As.ptr, *bs = (const uint32_t*)Ws.ptr;
+  if (pack_a) {
+    if (int rc = make_pack_args(&As, o.a_scale_layout, M, K, ws, kPackA, pa)) return rc;
+    as = (const uint32_t*)ws;
+    ws += mx_packed_scale_bytes(M, K);
+  }
+  if (pack_w) {
+    if (int rc = make_pack_args(&Ws, o.b_scale_layout, N, K, ws, kPackB, pb)) return rc;
+    bs = (const uint32_t*)ws;
+  }
+  if (pack_a || pack_w)
+    if (int rc = launch_pack_scales_pair(pack_a ? &pa : nullptr, pack_w ? &pb : nullptr, stream)) return rc;
+  GemmArgs g = {};
+  g.A = (const uint8_t*)A.ptr; g.B = (const uint8_t*)W.ptr; g.As = as; g.Bs = bs;
+  g.lda = A.stride[0]; g.ldb = W.stride[0];
+  g.M = (int32_t)M; g.N = (int32_t)N; g.K = (int32_t)K;
+  g.a_fmt = A.dtype; g.b_fmt = W.dtype; g.c_dtype = MX_BF16;
+  g.a_rows = M;
+  g.tile_rows = pp.rows;
+  return launch_gemm_pingpong_gated(g, out, stream);
+}
+}  // namespace mx

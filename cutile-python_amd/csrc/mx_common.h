@@ -137,7 +137,21 @@ struct GemmArgs {
   int64_t c_split_stride;                     // elements of C
 };
 
+// what becomes of the gate and up columns of a product: silu(g) * u, and optionally [g|u] itself quantised to E4M3
+struct GateOut {
+  void* h;                           // [rows][F]: bf16 (h_fmt MX_BF16) or codes
+  uint8_t* hs;                       // [rows][F / 32]
+  uint8_t *c, *cs;                   // [rows][2 F], [rows][2 F / 32]; may be null
+  int64_t h_ld, hs_ld, c_ld, cs_ld;  // elements of h; bytes
+  int32_t F, h_fmt, scale_mode;
+};
+
 int launch_gemm_mfma(const GemmArgs& g, int kernel_id, hipStream_t stream);
+// the product of MX_KERNEL_MFMA_PINGPONG with that in the place of its output (mx_gemm_pp.hip); N = 2 F
+int launch_gemm_pingpong_gated(const GemmArgs& g, const GateOut& o, hipStream_t stream);
+constexpr int kGatedNotFused = 1;
+int gemm_gated_fused(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const GateOut& out, const mx_gemm_opts& o,
+                     void* workspace, int64_t workspace_bytes, hipStream_t stream);
 int launch_gemm_pingpong(const GemmArgs& g, hipStream_t stream);
 // the 32x32x64-instruction variant: 8-bit element formats only
 bool pingpong32_supports(int a_fmt, int b_fmt);

@@ -82,17 +82,16 @@ int check_room(const char* name, const void* ptr, int64_t given, int64_t need) {
 int64_t gated_workspace(int64_t M, int64_t F, int64_t K, const mx_gemm_opts& o) {
   return round256(M * 2 * F * 2) + round256(mx_gemm_workspace_bytes(M, 2 * F, K, &o));
 }
-int run_gated(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const GateUpArgs& out, const mx_gemm_opts& o,
+int run_gated(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const GateOut& out, const mx_gemm_opts& o,
               void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   const int64_t M = A.shape[0], N = W.shape[0];
+  if (M > 0)
+    if (const int rc = gemm_gated_fused(A, As, W, Ws, out, o, workspace, workspace_bytes, stream); rc != kGatedNotFused) return rc;
   Deal ws = {(uint8_t*)workspace};
   mx_tensor gu = tensor2d(ws.take(M * N * 2), MX_BF16, M, N, N);
   const mx_tensor B = transposed(W), Bs = o.b_scale_layout == MX_SCALE_2D ? transposed(Ws) : Ws;
   if (int rc = mx_gemm(&A, &As, &B, &Bs, &gu, &o, ws.base + ws.at, workspace_bytes - ws.at, stream)) return rc;
-  GateUpArgs g = out;
-  g.gu = (const uint16_t*)gu.ptr;
-  g.gu_ld = N;
-  return launch_gate_up(g, stream);
+  return launch_gate_up(GateUpArgs{(const uint16_t*)gu.ptr, N, M, out}, stream);
 }
 
 // ---- the whole block ------------------------------------------------------------------------------------------------------------
@@ -260,10 +259,10 @@ int mx_gated_gemm(const mx_tensor* A, const mx_tensor* As, const mx_tensor* W, c
   if (F == 0 || F % 32 != 0) return set_error(MX_ERR_SHAPE, "F (%lld) must be a multiple of 32", (long long)F);
   if (M >= kMaxExtent || F >= kMaxExtent / 2 || K >= kMaxExtent) return set_error(MX_ERR_SHAPE, "mx_gated_gemm: extent out of range");
   if (int rc = check_mode(scale_mode)) return rc;
-  GateUpArgs g = {};
+  GateOut g = {};
   if (int rc = check2d(out, "out", M, F)) return rc;
   g.h = out->ptr; g.h_ld = out->stride[0]; g.h_fmt = out->dtype;
-  g.rows = M; g.F = (int32_t)F; g.scale_mode = scale_mode;
+  g.F = (int32_t)F; g.scale_mode = scale_mode;
   if (out->dtype == MX_BF16) {
     if (out_scale) return set_error(MX_ERR_INVALID, "out_scale: an MX_BF16 output has none");
     if ((uintptr_t)out->ptr % 16 != 0 || (M > 1 && (out->stride[0] % 8 != 0 || out->stride[0] < F)))
@@ -355,10 +354,10 @@ int mx_ffn_forward(const mx_tensor* x, const mx_tensor* w1, const mx_tensor* w2,
                               both(w1, f.w1, f.w1s, kScaleNativeB, k.w1t, k.w1ts, kScaleNativeB),
                               both(w2, f.w2, f.w2s, kScaleNativeB, k.w2t, k.w2ts, kScaleNativeB)};
   if (int rc = launch_quantize_both(list, 3, MX_E4M3, scale_mode, st)) return rc;
-  GateUpArgs g = {};
+  GateOut g = {};
   g.h = f.h; g.h_ld = s.F; g.h_fmt = MX_E4M3; g.hs = f.hs; g.hs_ld = s.F / 32;
   g.c = k.gu; g.c_ld = 2 * s.F; g.cs = k.gus; g.cs_ld = 2 * s.F / 32;
-  g.rows = s.T; g.F = (int32_t)s.F; g.scale_mode = scale_mode;
+  g.F = (int32_t)s.F; g.scale_mode = scale_mode;
   const mx_gemm_opts up = layouts(nat, true), down = layouts(false, true);
   if (int rc = run_gated(tensor2d(f.xq, MX_E4M3, s.T, s.H, s.H), tensor2d(f.xs, MX_E8M0, s.T, s.H / 32, s.H / 32),
                          tensor2d(f.w1, MX_E4M3, 2 * s.F, s.H, s.H), tensor2d(f.w1s, MX_E8M0, 2 * s.F, s.H / 32, s.H / 32), g, up, f.work,

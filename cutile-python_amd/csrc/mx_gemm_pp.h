@@ -172,5 +172,7 @@ inline int64_t pp_tail_bytes(int64_t M, int64_t N, int64_t K, bool fp4, bool til
 // the ping-pong kernels of one element-format pair (mx_gemm_pp.hip, compiled once per pair)
 template <int AF, int BF>
 int launch_pp_pair(const GemmArgs& g, hipStream_t stream);
+template <int AF, int BF>
+int launch_pp_gated_pair(const GemmArgs& g, const GateOut& o, hipStream_t stream);
 
 }  // namespace mx

@@ -37,20 +37,84 @@
 
 #include <type_traits>
 
+#include "mx_encode.h"
 #include "mx_gemm_pp.h"
 
 namespace mx {
 namespace {
+
+// GATED: the columns are gate and up of a feed-forward block, and silu(gate) * up is what leaves (GateOut).  A wave's 64 B rows are 32
+// gate rows and the 32 up rows F further on, so that a lane holds both of the same eight columns, and the four lanes l ^ 16, l ^ 32
+// hold the 32 columns of an MX block.  The epilogue is some 1200 vector instructions a wave and tile, which stand in the
+// memory phase; the other team has but one MFMA phase to put beside them.  8192 x 28672 x 4096 MXFP8, bf16 out: 678 us (2.84 PFLOP/s),
+// where a bf16 product and a pass over it take 831; 1531 rows, E4M3 out: 139 against 159 (with the scales re-laid 150 against 168).
+struct Ungated {};
+// one MX block's eight values of this lane: codes (E4M3, the floor rule) and scale byte; NaN is NaN among its block's other values
+__device__ __forceinline__ u2 gated_encode(const float (&v)[8], uint32_t& byte) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fmax_abs(m, v[e]);
+  const BlockScale b = block_scale<MX_E4M3, true>(max_xor_16_32(__builtin_bit_cast(uint32_t, m)));
+  byte = b.byte;
+  return (u2){encode4<MX_E4M3>(v[0], v[1], v[2], v[3], b.scale), encode4<MX_E4M3>(v[4], v[5], v[6], v[7], b.scale)};
+}
+// Row `row` (of C, if live), columns col .. col + 7 of gate and up.  (The floor rule, bf16 or E4M3: with the other rule and format
+// beside them the eight copies of this in a kernel are more than the instruction cache; such calls go through memory.)
+__device__ __forceinline__ void gated_store(const GateOut& o, const v4f (&acc)[4], int64_t row, int col, bool live, bool scale_lane) {
+  float g[8], u[8], h[8];
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {                        // through bf16, the precision of the activation between the projections
+    const uint32_t pg = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){acc[k / 2][2 * (k & 1)], acc[k / 2][2 * (k & 1) + 1]}, b2));
+    const uint32_t pu = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){acc[2 + k / 2][2 * (k & 1)], acc[2 + k / 2][2 * (k & 1) + 1]}, b2));
+    g[2 * k] = __builtin_bit_cast(float, pg << 16);
+    g[2 * k + 1] = __builtin_bit_cast(float, pg & 0xFFFF0000u);
+    u[2 * k] = __builtin_bit_cast(float, pu << 16);
+    u[2 * k + 1] = __builtin_bit_cast(float, pu & 0xFFFF0000u);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)   // (the hardware's 2^x and reciprocal: a few units in the last place)
+    h[e] = g[e] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g[e])) * u[e];
+  if (o.h_fmt == MX_BF16) {
+    if (live)
+      store8_full<uint16_t>((uint16_t*)o.h + row * o.h_ld + col, (v4f){h[0], h[1], h[2], h[3]}, (v4f){h[4], h[5], h[6], h[7]});
+  } else {
+    uint32_t byte;
+    const u2 c = gated_encode(h, byte);
+    if (live) {
+      *(u2*)((uint8_t*)o.h + row * o.h_ld + col) = c;
+      if (scale_lane) o.hs[row * o.hs_ld + col / 32] = (uint8_t)byte;
+    }
+  }
+  if (o.c) {
+    uint32_t bg, bu;
+    const u2 cg = gated_encode(g, bg), cu = gated_encode(u, bu);
+    if (live) {
+      uint8_t* const c = o.c + row * o.c_ld + col;
+      *(u2*)c = cg;
+      *(u2*)(c + o.F) = cu;
+      if (scale_lane) {
+        uint8_t* const cs = o.cs + row * o.cs_ld + col / 32;
+        cs[0] = (uint8_t)bg;
+        cs[o.F / 32] = (uint8_t)bu;
+      }
+    }
+  }
+}
 
 // KTAIL: K is not a whole number of stages (or there is a single stage): the 16-byte chunks beyond the end of K are
 // masked lane by lane at issue time.  Without it the loads take their precomputed offsets as they are, which keeps a
 // compare and a select per DMA instruction out of the memory phase.
 // SPLIT: the walk may end with a K range of one more tile, whose sums go to g.tail.  (An instance of its own: the few scalars
 // more cost the whole-round products, MXFP4 8192^3 232.2 -> 234.0 us.)
-template <class C, typename OutT, bool GROUPED, bool SPLIT, int TEAM, bool KTAIL>
-__device__ __forceinline__ void pp_body(const GemmArgs& g, lds_u8* const smem, const int wn,
+// Gate: Ungated or GateOut
+template <class C, typename OutT, bool GROUPED, bool SPLIT, int TEAM, bool KTAIL, class Gate>
+__device__ __forceinline__ void pp_body(const GemmArgs& g, const Gate& gate, lds_u8* const smem, const int wn,
                                         const int lane, const TileWalk& walk) {
   using P = PP<C>;
+  constexpr bool GATED = !std::is_same<Gate, Ungated>::value;
+  static_assert(!GATED || (!GROUPED && !SPLIT), "");
   constexpr int AL = P::AL, BL = P::BL;
   // A tiles (of 8) whose fragments are read in the memory phase; the others are read inside the MFMA phase,
   // 8 MFMAs ahead of their use.  Two measured best (four: 1.5 % slower on MXFP8, 5 % on the grouped
@@ -86,17 +150,27 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, lds_u8* const smem, c
   // descriptors, the (group, quad) part of the address in the scalar offset.
   // as / bs _cur, _nxt: byte offset of (group, K-quad 0) for the tile being computed / being fetched.
   int as_cur[2], bs_cur, as_nxt[2], bs_nxt;
+  int us_cur = 0, us_nxt = 0;        // gated: the same of the up rows' group; bit 0: the wave's rows are the groups' second halves
   const __amdgpu_buffer_rsrc_t rsAs = make_rsrc(g.As, (uint32_t)(packed_scale_dwords(g.M, g.K) * 4));
   const __amdgpu_buffer_rsrc_t rsBs =
       make_rsrc(g.Bs, (uint32_t)((GROUPED ? (int64_t)(g.num_experts - 1) * g.bs_expert_stride * 4 : 0) +
                                  packed_scale_dwords(g.N, g.K) * 4));
   const int sc_voff = lane * 16;
-  constexpr int NSC = 3;           // scale load instructions per K-quad
-  v4i sa[2], sb;
+  constexpr int NSC = GATED ? 4 : 3;   // scale load instructions per K-quad
+  v4i sa[2], sb, su;
   auto load_scales = [&](const int* as_off, int bs_off, int Qn) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) sa[u] = __builtin_amdgcn_raw_buffer_load_b128(rsAs, sc_voff, as_off[u] + Qn * 1024, 0);
     sb = __builtin_amdgcn_raw_buffer_load_b128(rsBs, sc_voff, bs_off + Qn * 1024, 0);
+    if constexpr (GATED) su = __builtin_amdgcn_raw_buffer_load_b128(rsBs, sc_voff, (us_cur & ~1) + Qn * 1024, 0);
+  };
+  // gated: tiles 0, 1 are the wave's 32 rows of the gate group, 2, 3 of the up group
+  auto join_scales = [&]() {
+    if constexpr (GATED) {
+      const uint32_t sel = us_cur & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) sb[t] = (int)__builtin_amdgcn_perm((uint32_t)su[t], (uint32_t)sb[t], sel);
+    }
   };
   bool fetch_valid = true;   // false once the walk has no further tile: loads become zero-fill no-ops
   // grouped: none of this team's 128 slots of the tile holds a routed row (every slot is looked at: two per lane,
@@ -183,7 +257,11 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, lds_u8* const smem, c
 #pragma unroll
       for (int q = 0; q < BL; ++q) {
         const int col = b_col(q, ln);
-        const int64_t grow = n0 + b_row0 + q * P::B_RPI;
+        int64_t grow = n0 + b_row0 + q * P::B_RPI;
+        if constexpr (GATED) {   // row n of the wave's 64: gate row n of its 32 columns, or up row n - 32
+          const int n = ln / C::B_CPR + q * P::B_RPI, c = n0 / 2 + 32 * wn + (n & 31);
+          grow = c < gate.F ? c + (n >= 32 ? gate.F : 0) : g.N;
+        }
         b_voff[q] = (fetch_valid && grow < g.N) ? (uint32_t)(grow * g.ldb + col) + kb0 : kOobOffset;
       }
     }
@@ -192,6 +270,12 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, lds_u8* const smem, c
     for (int u = 0; u < 2; ++u) {
       const int grp = (m0 + wm0) / 64 + u;
       as_nxt[u] = ((grp < a_groups ? grp : a_groups - 1) * KQ + qb) * 1024;
+    }
+    if constexpr (GATED) {   // (F is a multiple of 64: gate and up rows begin at a group)
+      const int c = n0 / 2 + 32 * wn, last = gate.F / 64 - 1, grp = c / 64 < last ? c / 64 : last;
+      bs_nxt = (grp * KQ + qb) * 1024;
+      us_nxt = ((gate.F / 64 + grp) * KQ + qb) * 1024 + (c / 32 & 1);
+      return;
     }
     const int grp = (n0 + wn0) / 64;
     bs_nxt = (GROUPED ? (int)(expert * (g.bs_expert_stride * 4)) : 0) +
@@ -244,7 +328,24 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, lds_u8* const smem, c
   const bool vec8_ok = ((g.ldc * (int64_t)sizeof(OutT)) % 16 == 0) && (((uintptr_t)g.C) % 16 == 0);
   const bool accumulate = g.accumulate != 0;
   auto write_tile = [&](int m0, int n0) {
-    if constexpr (!GROUPED) {
+    if constexpr (GATED) {
+      const int col = n0 / 2 + 32 * wn + 8 * gq;
+      // (only here: with that mode bit the scaled MFMA takes NaN elements and scales for numbers)
+      saturate_conversions(true);
+      if (col < gate.F) {   // uniform: F is a multiple of 32
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int64_t row = m0 + wm0 + 16 * i + r;
+          gated_store(gate, acc[i], row, col, row < g.M, gq == 0);
+        }
+      }
+      saturate_conversions(false);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+      return;
+    } else if constexpr (!GROUPED) {
       // interior tile, plain store: one address per lane, everything else immediate offsets
       if (m0 + C::BM <= g.M && n0 + 256 <= g.N && vec8_ok && !accumulate) {
         OutT* p = Cp + (int64_t)(m0 + wm0 + r) * g.ldc + (n0 + wn0 + 8 * gq);
@@ -409,6 +510,7 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, lds_u8* const smem, c
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // fragments are in registers
     __builtin_amdgcn_sched_barrier(0);
     // =============================== MFMA phase ====================================================
+    if constexpr (t0 == 0) join_scales();
     __builtin_amdgcn_s_setprio(1);
     auto read_pair = [&](int i0) {
 #pragma unroll
@@ -469,6 +571,7 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, lds_u8* const smem, c
     as_cur[0] = as_nxt[0];
     as_cur[1] = as_nxt[1];
     bs_cur = bs_nxt;
+    us_cur = us_nxt;
     for (Q = 0; Q < kq; ++Q) {
       stage(std::integral_constant<int, 0>{});
       if constexpr (C::KSUB == 1) stage(std::integral_constant<int, 1>{});
@@ -511,8 +614,8 @@ __device__ __forceinline__ TileWalk pp_walk(const GemmArgs& g) {
   else return make_tile_walk(M, g.N, C::BM);
 }
 
-template <class C, typename OutT, bool GROUPED, bool SPLIT>
-__global__ __launch_bounds__(512) void gemm_pp_kernel(const GemmArgs g) {
+template <class C, typename OutT, bool GROUPED, bool SPLIT, class Gate = Ungated>
+__device__ __forceinline__ void pp_kernel(const GemmArgs& g, const Gate& gate) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem_generic[];
   lds_u8* const smem = (lds_u8*)smem_generic;
   const int lane = threadIdx.x & 63;
@@ -526,15 +629,24 @@ __global__ __launch_bounds__(512) void gemm_pp_kernel(const GemmArgs g) {
   const bool ktail = C::KSUB != 1 || (!SPLIT && (g.K % 128 != 0 || ksteps < 2));
   if (ktail) {
     if (wave < 4)
-      pp_body<C, OutT, GROUPED, SPLIT, 0, true>(g, smem, wave, lane, walk);
+      pp_body<C, OutT, GROUPED, SPLIT, 0, true>(g, gate, smem, wave, lane, walk);
     else
-      pp_body<C, OutT, GROUPED, SPLIT, 1, true>(g, smem, wave - 4, lane, walk);
+      pp_body<C, OutT, GROUPED, SPLIT, 1, true>(g, gate, smem, wave - 4, lane, walk);
   } else if constexpr (C::KSUB == 1) {
     if (wave < 4)
-      pp_body<C, OutT, GROUPED, SPLIT, 0, false>(g, smem, wave, lane, walk);
+      pp_body<C, OutT, GROUPED, SPLIT, 0, false>(g, gate, smem, wave, lane, walk);
     else
-      pp_body<C, OutT, GROUPED, SPLIT, 1, false>(g, smem, wave - 4, lane, walk);
+      pp_body<C, OutT, GROUPED, SPLIT, 1, false>(g, gate, smem, wave - 4, lane, walk);
   }
+}
+
+template <class C, typename OutT, bool GROUPED, bool SPLIT>
+__global__ __launch_bounds__(512) void gemm_pp_kernel(const GemmArgs g) {
+  pp_kernel<C, OutT, GROUPED, SPLIT>(g, Ungated{});
+}
+template <class C>
+__global__ __launch_bounds__(512) void gemm_pp_gated_kernel(const GemmArgs g, const GateOut gate) {
+  pp_kernel<C, uint16_t, false, false>(g, gate);
 }
 
 // Adds up the partial sums of the tiles that gemm_pp_kernel split along K, in the order of their slices, and writes them.
@@ -612,7 +724,30 @@ int launch_pp(const GemmArgs& g, hipStream_t stream) {
   return MX_OK;
 }
 
+template <class C>
+int launch_pp_gated(const GemmArgs& g, const GateOut& o, hipStream_t stream) {
+  auto kern = gemm_pp_gated_kernel<C>;
+  static int attr_done = 0;   // (as above)
+  if (!attr_done) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, PP<C>::LDS_BYTES);
+    if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "hipFuncSetAttribute(%d bytes LDS): %s", PP<C>::LDS_BYTES, hipGetErrorString(e));
+    attr_done = 1;
+  }
+  const int64_t grid = pp_grid(g.M, g.N, g.K, C::KSUB, C::BM);
+  if (grid <= 0) return MX_OK;
+  const hipError_t e = launch_kernel(kern, dim3((unsigned)grid), dim3(512), PP<C>::LDS_BYTES, stream, g, o);
+  if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "gemm_pp_gated_kernel launch: %s", hipGetErrorString(e));
+  return MX_OK;
+}
+
 }  // namespace
+
+// The gated form of one element-format pair.
+template <int AF, int BF>
+int launch_pp_gated_pair(const GemmArgs& g, const GateOut& o, hipStream_t stream) {
+  if (g.tile_rows == 192) return launch_pp_gated<Cfg<AF, BF, 192, 256, 2, 4>>(g, o, stream);
+  return launch_pp_gated<Cfg<AF, BF, 256, 256, 2, 4>>(g, o, stream);
+}
 
 // One element-format pair (grouped and plain, fp32 and bf16 output) per compilation of this file, so that the pairs
 // build in parallel: MX_PP_PAIR names it.
@@ -632,8 +767,26 @@ int launch_pp_pair(const GemmArgs& g, hipStream_t stream) {
   }
   return g.tail ? run(std::true_type{}) : run(std::false_type{});
 }
-#if MX_PP_PAIR == 0
+#if MX_PP_PAIR >= 4
+template int launch_pp_gated_pair<MX_PP_PAIR == 4 || MX_PP_PAIR == 7 ? MX_E4M3 : MX_PP_PAIR == 5 ? MX_E5M2 : MX_E2M1,
+                                  MX_PP_PAIR == 4 ? MX_E4M3 : MX_PP_PAIR == 5 ? MX_E5M2 : MX_E2M1>(const GemmArgs&, const GateOut&, hipStream_t);
+#elif MX_PP_PAIR == 0
 template int launch_pp_pair<MX_E4M3, MX_E4M3>(const GemmArgs&, hipStream_t);
+extern template int launch_pp_gated_pair<MX_E4M3, MX_E4M3>(const GemmArgs&, const GateOut&, hipStream_t);
+extern template int launch_pp_gated_pair<MX_E5M2, MX_E5M2>(const GemmArgs&, const GateOut&, hipStream_t);
+extern template int launch_pp_gated_pair<MX_E2M1, MX_E2M1>(const GemmArgs&, const GateOut&, hipStream_t);
+extern template int launch_pp_gated_pair<MX_E4M3, MX_E2M1>(const GemmArgs&, const GateOut&, hipStream_t);
+
+int launch_gemm_pingpong_gated(const GemmArgs& g, const GateOut& o, hipStream_t stream) {
+#define MX_CASE(AFMT, BFMT) \
+  if (g.a_fmt == AFMT && g.b_fmt == BFMT) return launch_pp_gated_pair<AFMT, BFMT>(g, o, stream);
+  MX_CASE(MX_E4M3, MX_E4M3)
+  MX_CASE(MX_E5M2, MX_E5M2)
+  MX_CASE(MX_E2M1, MX_E2M1)
+  MX_CASE(MX_E4M3, MX_E2M1)
+#undef MX_CASE
+  return set_error(MX_ERR_DTYPE, "MFMA kernel: unsupported element format pair (%d, %d)", g.a_fmt, g.b_fmt);
+}
 extern template int launch_pp_pair<MX_E5M2, MX_E5M2>(const GemmArgs&, hipStream_t);
 extern template int launch_pp_pair<MX_E2M1, MX_E2M1>(const GemmArgs&, hipStream_t);
 extern template int launch_pp_pair<MX_E4M3, MX_E2M1>(const GemmArgs&, hipStream_t);

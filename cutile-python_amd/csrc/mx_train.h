@@ -16,7 +16,7 @@ struct BothTensor {
   int32_t rows, K, x_dtype;
   int32_t s_kind, st_kind;           // kScale*
   // filled in by the launcher
-  int32_t first, tiles, tiles_k;
+  int32_t first, tiles, tiles_k, once;
 };
 constexpr int kBothMax = 3;
 struct BothArgs {
@@ -29,13 +29,8 @@ int launch_quantize_both(const BothTensor* list, int n, int fmt, int scale_mode,
 // [g|u] (bf16 [rows, 2 F]) -> silu(g) * u, as bf16 or quantised, and optionally [g|u] quantised to E4M3
 struct GateUpArgs {
   const uint16_t* gu;
-  int64_t gu_ld;
-  void* h;                           // bf16 (h_fmt MX_BF16) or codes
-  uint8_t* hs;
-  uint8_t *c, *cs;                   // checkpoint; may be null
-  int64_t h_ld, hs_ld, c_ld, cs_ld;  // elements of h; bytes
-  int64_t rows;
-  int32_t F, h_fmt, scale_mode;
+  int64_t gu_ld, rows;
+  GateOut out;
 };
 int launch_gate_up(const GateUpArgs& a, hipStream_t stream);
 

@@ -1,14 +1,16 @@
 // Kernels of the gated feed-forward block that is trained in 8 bits: quantisation along both axes of a matrix, the activation
 // between the projections with its checkpoint, and the activation's backward pass.  What they quantise follows encode_block
 // (mx_quant.h) to the bit.
+#include <type_traits>
+
+#include "mx_encode.h"
 #include "mx_gemm_tile.h"   // make_rsrc, kOobOffset
-#include "mx_quant.h"
+#include "mx_load_once.h"
 #include "mx_train.h"
 
 namespace mx {
 namespace {
 
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 
@@ -24,120 +26,6 @@ __device__ __forceinline__ void tile_of(uint32_t id, uint32_t n, uint32_t tiles_
   const uint32_t rows = left < ROWS ? left : ROWS;
   tk = in / rows;
   tr = first + in - tk * rows;
-}
-
-// ---- maxima over lanes ------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint32_t umin(uint32_t a, uint32_t b) { return a < b ? a : b; }
-__device__ __forceinline__ uint32_t max_quad(uint32_t m) {            // lanes 4 n .. 4 n + 3
-  m = umax(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xF, 0xF, true));
-  return umax(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xF, 0xF, true));
-}
-__device__ __forceinline__ uint32_t max_xor_8(uint32_t m) {           // lanes l, l ^ 8: a rotation of the 16-lane row by 8
-  return umax(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x128, 0xF, 0xF, true));
-}
-__device__ __forceinline__ uint32_t max_xor_16_32(uint32_t m) {       // lanes l, l ^ 16, l ^ 32, l ^ 48
-  const auto a = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-  m = umax(a[0], a[1]);
-  const auto b = __builtin_amdgcn_permlane16_swap(m, m, false, false);
-  return umax(b[0], b[1]);
-}
-// Maxima of eight columns over lanes l, l ^ 16, l ^ 32, l ^ 48, of which every lane gets two: half of the columns go away with each
-// exchange.  r[e] is column e + own_column(lane); spread_columns hands what has been made of them back to all four lanes.
-__device__ __forceinline__ int own_column(int lane) { return (lane >> 4 & 1) * 2 + (lane >> 5) * 4; }
-__device__ __forceinline__ void max_columns(const uint32_t (&m)[8], uint32_t (&r)[2]) {
-  uint32_t t[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const auto a = __builtin_amdgcn_permlane32_swap(m[e], m[e + 4], false, false);
-    t[e] = umax(a[0], a[1]);
-  }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const auto a = __builtin_amdgcn_permlane16_swap(t[e], t[e + 2], false, false);
-    r[e] = umax(a[0], a[1]);
-  }
-}
-__device__ __forceinline__ void spread_columns(const float (&s)[2], float (&all)[8]) {
-  uint32_t t[4];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const uint32_t v = __builtin_bit_cast(uint32_t, s[e]);
-    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    t[e] = a[0];
-    t[e + 2] = a[1];
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const auto a = __builtin_amdgcn_permlane32_swap(t[e], t[e], false, false);
-    all[e] = __builtin_bit_cast(float, (uint32_t)a[0]);
-    all[e + 4] = __builtin_bit_cast(float, (uint32_t)a[1]);
-  }
-}
-__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
-
-// ---- encoding ---------------------------------------------------------------------------------------------------------------
-// What the hardware conversions need of a block whose largest magnitude has the bits `am`: its scale, as a number and as a byte.
-// For the blocks that AmaxRange names (subnormal or non-finite amax, extreme scale) both are meaningless: they are encode_block's.  A
-// block of zeros is zeros at any scale.  The floor rule saturates: the conversions do so with saturate_conversions(), the same
-// codes as a clamp ahead of them.
-struct BlockScale {
-  float scale;
-  uint32_t byte;
-};
-template <int FMT, bool FLOOR>
-__device__ __forceinline__ BlockScale block_scale(uint32_t am) {
-  constexpr uint32_t EMAX = FMT == MX_E4M3 ? 8 : 15;
-  BlockScale b;
-  if constexpr (FLOOR) {
-    b.byte = __builtin_elementwise_sub_sat(am >> 23, EMAX);
-    b.scale = __builtin_bit_cast(float, umax(b.byte, 1u) << 23);
-  } else {
-    const uint32_t t = __builtin_bit_cast(uint32_t, fmaxf(__fdiv_rn(__builtin_bit_cast(float, am), 448.0f), 1e-12f));
-    b.byte = (t >> 23) + ((t & 0x7FFFFFu) ? 1 : 0);   // (88 or more)
-    b.scale = __builtin_bit_cast(float, b.byte << 23);
-  }
-  return b;
-}
-// Mode bit FP16_OVFL of the wave: conversions to 8-bit formats end at the largest finite number instead of NaN or infinity (NaN
-// stays).  (The ceiling rule never gets there.)
-__device__ __forceinline__ void saturate_conversions() { __builtin_amdgcn_s_setreg(1 | 23 << 6, 1); }
-// The range of the amax of the blocks that a lane has seen; zero does not count as small.
-struct AmaxRange {
-  uint32_t least = ~0u, most = 0;   // least: minus one, so that zero wraps
-  __device__ __forceinline__ void add(uint32_t am) {
-    least = umin(least, am - 1);
-    most = umax(most, am);
-  }
-  template <int FMT, bool FLOOR>
-  __device__ __forceinline__ bool odd() const {
-    constexpr uint32_t EMAX = FMT == MX_E4M3 ? 8 : 15;
-    // floor: scales 2^-126 .. 2^119 (E4M3) of a finite amax; ceil: a normal amax whose scale, amax / 448 rounded up, is at most 2^119
-    return FLOOR ? least < ((EMAX + 1) << 23) - 1 || most >= 0x7F800000u : least < 0x007FFFFFu || most > 0x7F600000u;
-  }
-};
-// four values of a block as codes, lowest byte first
-template <int FMT>
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float scale) {
-  typedef short s2 __attribute__((ext_vector_type(2)));
-  s2 r = {0, 0};
-  if constexpr (FMT == MX_E4M3) {
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
-  } else {
-    r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(r, a, b, scale, false);
-    r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(r, c, d, scale, true);
-  }
-  return __builtin_bit_cast(uint32_t, r);
-}
-template <int N>
-__device__ inline void encode_slow(const float* v, uint32_t am, int fmt, int scale_mode, uint32_t* packed, uint32_t& byte) {
-  uint32_t code[N];
-  uint8_t sb;
-  encode_block<N>(v, am, fmt, scale_mode, code, sb);
-#pragma unroll
-  for (int h = 0; h < N / 4; ++h) packed[h] = code[4 * h] | (code[4 * h + 1] << 8) | (code[4 * h + 2] << 16) | (code[4 * h + 3] << 24);
-  byte = sb;
 }
 
 // Scale bytes [rows of the tile][4 blocks] of a 128-row tile, from LDS to where they belong: row0, block0 = first row and block
@@ -222,7 +110,8 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(const BothArgs a) {
   uint8_t* const srow_b = (uint8_t*)srow;
   uint8_t* const scol_b = (uint8_t*)scol;
   if constexpr (FLOOR) saturate_conversions();
-  if (r0 < rows && k0 < Kpad) {                       // (else: padding of native scales only)
+  const bool inside = r0 < rows && k0 < Kpad;         // (else: padding of native scales only)
+  if (inside && r0 + 32 * wave < rows) {              // (waves without rows have nothing to do)
     const int64_t row = r0 + 32 * wave + 8 * rg, col = k0 + 8 * cg;   // of the lane's first element
     const int n_rows = rows - r0 < 128 ? (int)(rows - r0) : 128, n_cols = Kpad - k0 < 128 ? (int)(Kpad - k0) : 128;
     float v[8][8];
@@ -232,12 +121,16 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(const BothArgs a) {
       const __amdgpu_buffer_rsrc_t rs = make_rsrc((const uint8_t*)t.x + (r0 * t.x_ld + k0) * ESZ, (n_rows - 1) * pitch + n_cols * ESZ);
       uint32_t vo = 8 * cg < n_cols ? (32 * wave + 8 * rg) * pitch + 8 * cg * ESZ : kOobOffset;
       v4i raw[8][NL];
+      auto load = [&](auto once) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; ++i) {
 #pragma unroll
-        for (int h = 0; h < NL; ++h) raw[i][h] = __builtin_amdgcn_raw_buffer_load_b128(rs, vo + 16 * h, 0, 0);
-        vo += pitch;
-      }
+          for (int h = 0; h < NL; ++h) raw[i][h] = __builtin_amdgcn_raw_buffer_load_b128(rs, vo + 16 * h, 0, decltype(once)::value);
+          vo += pitch;
+        }
+      };
+      if (t.once) load(std::integral_constant<int, kLoadOnce>{});
+      else load(std::integral_constant<int, 0>{});
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
 #pragma unroll
@@ -264,7 +157,7 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(const BothArgs a) {
           if (row + i < rows && col + e < K) v[i][e] = load_one<SRC>(t.x, (row + i) * t.x_ld + col + e);
         }
     }
-    AmaxRange range;
+    uint32_t most = 0;
     // (scale bytes are written by all lanes of a block, the same byte to the same place: a branch around each costs more)
     if (t.q) {
       const __amdgpu_buffer_rsrc_t rq = make_rsrc(t.q + r0 * t.q_ld + k0, PLAIN ? (uint32_t)((n_rows - 1) * t.q_ld + n_cols) : 0u);
@@ -280,7 +173,7 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(const BothArgs a) {
           for (int e = 0; e < 8; ++e) am = umax(am, magnitude(v[i][e]));
           am = max_quad(am);
         }
-        range.add(am);
+        most = umax(most, am);
         const BlockScale b = block_scale<FMT, FLOOR>(am);
         const u2 c = {encode4<FMT>(v[i][0], v[i][1], v[i][2], v[i][3], b.scale), encode4<FMT>(v[i][4], v[i][5], v[i][6], v[i][7], b.scale)};
         if constexpr (PLAIN) {
@@ -322,7 +215,7 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(const BothArgs a) {
       float scale[2], s[8];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        range.add(own[e]);
+        most = umax(most, own[e]);
         const BlockScale b = block_scale<FMT, FLOOR>(own[e]);
         scale[e] = b.scale;
         scol_b[(8 * cg + own_column(lane) + e) * 4 + wave] = (uint8_t)b.byte;
@@ -332,7 +225,7 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(const BothArgs a) {
       for (int e = 0; e < 8; ++e)
         place(e, (u2){encode4<FMT>(v[0][e], v[1][e], v[2][e], v[3][e], s[e]), encode4<FMT>(v[4][e], v[5][e], v[6][e], v[7][e], s[e])});
     }
-    if (__builtin_amdgcn_ballot_w64(range.odd<FMT, FLOOR>())) {   // a wave with such a block does all of its blocks again, from memory
+    if (__builtin_amdgcn_ballot_w64(odd_block<FLOOR>(most))) {   // a wave with such a block does all of its blocks again, from memory
 #pragma unroll 1
       for (int i = 0; t.q && i < 8; ++i) {
         float w[8];
@@ -360,7 +253,9 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(const BothArgs a) {
         if (rg == 0) scol_b[(8 * cg + e) * 4 + wave] = (uint8_t)byte;
       }
     }
-    __syncthreads();
+  }
+  __syncthreads();
+  if (inside) {
     if (t.qt) {
       const int m_cols = K - k0 < 128 ? (int)(K - k0) : 128, m_rows = Rpad - r0 < 128 ? (int)(Rpad - r0) : 128;   // of the transposed tile
       const __amdgpu_buffer_rsrc_t rt = make_rsrc(t.qt + k0 * t.qt_ld + r0, PLAIN ? (uint32_t)((m_cols - 1) * t.qt_ld + m_rows) : 0u);
@@ -398,9 +293,7 @@ __device__ __forceinline__ void store_row_block(const float (&v)[8], uint8_t* q,
   for (int e = 0; e < 8; ++e) am = umax(am, magnitude(v[e]));
   am = max_quad(am);
   const BlockScale b = block_scale<FMT, FLOOR>(am);
-  AmaxRange range;
-  range.add(am);
-  if (!range.odd<FMT, FLOOR>()) {
+  if (!odd_block<FLOOR>(am)) {
     c[0] = encode4<FMT>(v[0], v[1], v[2], v[3], b.scale);
     c[1] = encode4<FMT>(v[4], v[5], v[6], v[7], b.scale);
     byte = b.byte;
@@ -414,14 +307,15 @@ __device__ __forceinline__ void store_row_block(const float (&v)[8], uint8_t* q,
 // OUT: MX_BF16, MX_E4M3 or MX_E5M2
 template <int OUT, bool FLOOR>
 __global__ __launch_bounds__(256) void gate_up_kernel(const GateUpArgs a) {
+  const GateOut& o = a.out;
   if constexpr (FLOOR) saturate_conversions();
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, per = a.F / 8;   // (32 columns are four lanes of a wave)
+  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, per = o.F / 8;   // (32 columns are four lanes of a wave)
   const int64_t row = unit / per, col = (unit - row * per) * 8;
   if (row >= a.rows) return;
   const uint16_t* const p = a.gu + row * a.gu_ld + col;
   float g[8], u[8], h[8];
   unpack_bf16(*(const v4i*)p, g);
-  unpack_bf16(*(const v4i*)(p + a.F), u);
+  unpack_bf16(*(const v4i*)(p + o.F), u);
 #pragma unroll
   for (int e = 0; e < 8; ++e) h[e] = silu_mul_f32(g[e], u[e]);
   const bool first = (threadIdx.x & 3) == 0;
@@ -429,15 +323,15 @@ __global__ __launch_bounds__(256) void gate_up_kernel(const GateUpArgs a) {
     u4 w;
 #pragma unroll
     for (int k = 0; k < 4; ++k) w[k] = (uint32_t)f32_to_bf16(h[2 * k]) | ((uint32_t)f32_to_bf16(h[2 * k + 1]) << 16);
-    *(u4*)((uint16_t*)a.h + row * a.h_ld + col) = w;
+    *(u4*)((uint16_t*)o.h + row * o.h_ld + col) = w;
   } else {
-    store_row_block<OUT, FLOOR>(h, (uint8_t*)a.h + row * a.h_ld + col, a.hs + row * a.hs_ld + col / 32, first);
+    store_row_block<OUT, FLOOR>(h, (uint8_t*)o.h + row * o.h_ld + col, o.hs + row * o.hs_ld + col / 32, first);
   }
-  if (a.c) {
-    uint8_t* const c = a.c + row * a.c_ld + col;
-    uint8_t* const cs = a.cs + row * a.cs_ld + col / 32;
+  if (o.c) {
+    uint8_t* const c = o.c + row * o.c_ld + col;
+    uint8_t* const cs = o.cs + row * o.cs_ld + col / 32;
     store_row_block<MX_E4M3, FLOOR>(g, c, cs, first);
-    store_row_block<MX_E4M3, FLOOR>(u, c + a.F, cs + a.F / 32, first);
+    store_row_block<MX_E4M3, FLOOR>(u, c + o.F, cs + o.F / 32, first);
   }
 }
 
@@ -458,10 +352,10 @@ __device__ __forceinline__ void silu_slope(float g, float& gs, float& slope) {
   gs = g * s;
   slope = __builtin_fmaf(-gs, s, s + gs);
 }
-__device__ __forceinline__ float fmax_abs(float m, float a) { return __builtin_fmaxf(m, __builtin_fabsf(a)); }
 
 // Loads and stores through descriptors of the tile, as in quantize_both_kernel (the launcher's rule; PLAIN false: any pitch).
-template <bool FLOOR, bool PLAIN>
+// ONCE: dh and the checkpoint are loaded non-temporally (as the quantiser's input, mx_load_once.h: 4096 x 14336 146 -> 141 us).
+template <bool FLOOR, bool PLAIN, bool ONCE>
 __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwardArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t tile[3][128 * 128];   // codes along columns: dg, du, a
   __shared__ uint32_t srow[2][128], scol[3][128];      // their scales, four blocks a row
@@ -481,7 +375,7 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
       const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.gu + r0 * a.gu_ld + at + k0, (uint32_t)((n_rows - 1) * pg + F - k0));
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        q[i] = __builtin_amdgcn_raw_buffer_load_b64(rs, (col_in && lr + i < n_rows ? 0 : kOobOffset) | ((lr + i) * pg + lc), 0, 0);
+        q[i] = __builtin_amdgcn_raw_buffer_load_b64(rs, (col_in && lr + i < n_rows ? 0 : kOobOffset) | ((lr + i) * pg + lc), 0, ONCE ? kLoadOnce : 0);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -498,7 +392,7 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
       const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.dh + r0 * a.dh_ld + k0, (uint32_t)((n_rows - 1) * pd + (F - k0) * 2));
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        rdh[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (col_in && lr + i < n_rows ? 0 : kOobOffset) | ((lr + i) * pd + lc * 2), 0, 0);
+        rdh[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (col_in && lr + i < n_rows ? 0 : kOobOffset) | ((lr + i) * pd + lc * 2), 0, ONCE ? kLoadOnce : 0);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -534,11 +428,10 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
       sin[o][r] = w;
     }
     __syncthreads();
+    if (lr - 4 * rg < n_rows) {                        // (waves without rows have nothing to do)
     auto scale_in = [&](int o, int i) { return (uint32_t)((const uint8_t*)sin[o])[(lr + i) * 4 + lc / 32]; };
     const __amdgpu_buffer_rsrc_t rd = make_rsrc(a.d + r0 * a.d_ld + k0, PLAIN ? (uint32_t)((n_rows - 1) * a.d_ld + F + n_cols) : 0u);
-    AmaxRange range;
-    // The maxima below pass over NaN: it shows here.  What makes a NaN of any result makes NaN or infinity of dg.
-    float probe = 0.f;
+    // (The maxima pass over NaN: it is NaN among codes of its block's other values.)
     // one result at a time, 32 numbers of a lane: out along the rows (dg, du), then along the columns
     auto row_out = [&](int o, const float (&v)[4][8]) {
 #pragma unroll
@@ -546,9 +439,7 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
         float m = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) m = fmax_abs(m, v[i][e]);
-        const uint32_t am = max_quad(__builtin_bit_cast(uint32_t, m));
-        range.add(am);
-        const BlockScale b = block_scale<MX_E4M3, FLOOR>(am);
+        const BlockScale b = block_scale<MX_E4M3, FLOOR>(max_quad(__builtin_bit_cast(uint32_t, m)));
         const float (&w)[8] = v[i];
         const u2 c = {encode4<MX_E4M3>(w[0], w[1], w[2], w[3], b.scale), encode4<MX_E4M3>(w[4], w[5], w[6], w[7], b.scale)};
         if constexpr (PLAIN) {
@@ -572,9 +463,7 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
       max_columns(m, own);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        own[e] = max_xor_8(own[e]);
-        range.add(own[e]);
-        const BlockScale b = block_scale<MX_E4M3, FLOOR>(own[e]);
+        const BlockScale b = block_scale<MX_E4M3, FLOOR>(max_xor_8(own[e]));
         scale[e] = b.scale;
         ((uint8_t*)scol[o])[(lc + own_column(lane) + e) * 4 + wave] = (uint8_t)b.byte;
       }
@@ -606,10 +495,7 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
       unpack_bf16(rdh[i], dh);
       decoded(rup[i], scale_in(1, i), u);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[i][e] = dh[e] * u[e] * v[i][e];
-        probe = __builtin_fmaf(v[i][e], 0.f, probe);
-      }
+      for (int e = 0; e < 8; ++e) v[i][e] = dh[e] * u[e] * v[i][e];
     }
     row_out(0, v);
     col_out(0, v);
@@ -640,44 +526,6 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
       for (int e = 0; e < 8; ++e) v[i][e] = gs[i][e] * u[e];
     }
     col_out(2, v);
-    if (probe != probe) range.most = ~0u;
-    if (__builtin_amdgcn_ballot_w64(range.odd<MX_E4M3, FLOOR>())) {   // a wave with a block for encode_block does all of its blocks again, from memory
-      auto value = [&](int o, int64_t r, int64_t c) {
-        if (r >= rows || !col_in) return 0.f;
-        const float fg = decode_e8m0(a.gus[r * a.gus_ld + c / 32]), fu = decode_e8m0(a.gus[r * a.gus_ld + (F + c) / 32]);
-        const float dh = bf16_to_f32(a.dh[r * a.dh_ld + c]), u = __builtin_amdgcn_cvt_pk_f32_fp8(a.gu[r * a.gu_ld + F + c], false)[0] * fu;
-        float gs, slope;
-        silu_slope(__builtin_amdgcn_cvt_pk_f32_fp8(a.gu[r * a.gu_ld + c], false)[0] * fg, gs, slope);
-        return o == 0 ? dh * u * slope : o == 1 ? dh * gs : gs * u;
-      };
-#pragma unroll 1
-      for (int n = 0; n < 8; ++n) {
-        const int o = n >> 2, i = n & 3;
-        float w[8];
-        uint32_t am = 0, c[2], byte;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          w[e] = value(o, row + i, col + e);
-          am = umax(am, magnitude(w[e]));
-        }
-        encode_slow<8>(w, max_quad(am), MX_E4M3, a.scale_mode, c, byte);
-        if (row + i < rows && col_in) *(u2*)(a.d + (row + i) * a.d_ld + o * F + col) = (u2){c[0], c[1]};
-        if ((lane & 3) == 0) ((uint8_t*)srow[o])[(lr + i) * 4 + lc / 32] = (uint8_t)byte;
-      }
-#pragma unroll 1
-      for (int n = 8; n < 32; ++n) {
-        const int o = (n >> 3) - 1, e = n & 7;
-        float w[4];
-        uint32_t am = 0, c[1], byte;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = value(o, row + i, col + e);
-          am = umax(am, magnitude(w[i]));
-        }
-        encode_slow<4>(w, max_xor_16_32(max_xor_8(am)), MX_E4M3, a.scale_mode, c, byte);
-        place(o, e, c[0]);
-        if (rg == 0) ((uint8_t*)scol[o])[(lc + e) * 4 + wave] = (uint8_t)byte;
-      }
     }
     __syncthreads();
 #pragma unroll
@@ -762,6 +610,7 @@ int launch_quantize_both(const BothTensor* list, int n, int fmt, int scale_mode,
       blocks += tiles;
       if (blocks > 0x7FFFFFFF) return set_error(MX_ERR_SHAPE, "quantize_both: tensor too large");
       t.tiles = (int32_t)tiles;
+      t.once = quantize_loads_once((int64_t)t.rows * t.K);
       a.t[a.n++] = t;
     }
     if (blocks == 0) continue;
@@ -781,12 +630,12 @@ int launch_quantize_both(const BothTensor* list, int n, int fmt, int scale_mode,
 }
 
 int launch_gate_up(const GateUpArgs& a, hipStream_t stream) {
-  const int64_t blocks = (a.rows * (a.F / 8) + 255) / 256;
+  const int64_t blocks = (a.rows * (a.out.F / 8) + 255) / 256;
   if (blocks <= 0) return MX_OK;
   if (blocks > 0x7FFFFFFF) return set_error(MX_ERR_SHAPE, "gate_up: tensor too large");
   hipError_t e = hipSuccess;
 #define MX_CASE(OUT, FLOOR) \
-  if (a.h_fmt == OUT && (a.scale_mode != 0) == FLOOR) e = launch_kernel(gate_up_kernel<OUT, FLOOR>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  if (a.out.h_fmt == OUT && (a.out.scale_mode != 0) == FLOOR) e = launch_kernel(gate_up_kernel<OUT, FLOOR>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
   MX_CASE(MX_BF16, true)
   MX_CASE(MX_BF16, false)
   MX_CASE(MX_E4M3, true)
@@ -809,9 +658,18 @@ int launch_silu_backward(const SiluBackwardArgs& args, hipStream_t stream) {
   const bool plain = (((uintptr_t)a.dh | (uintptr_t)(a.dh_ld * 2)) & 15) == 0 && a.dh_ld >= a.F && a.gu_ld >= 2 * a.F && a.gus_ld >= a.F / 16 &&
                      128 * a.dh_ld * 2 < lim && 128 * a.gu_ld < lim && 128 * a.gus_ld < lim && 128 * a.d_ld < lim;
   const dim3 grid((unsigned)blocks);
-  hipError_t e;
-  if (a.scale_mode) e = plain ? launch_kernel(silu_backward_kernel<true, true>, grid, dim3(512), 0, stream, a) : launch_kernel(silu_backward_kernel<true, false>, grid, dim3(512), 0, stream, a);
-  else e = plain ? launch_kernel(silu_backward_kernel<false, true>, grid, dim3(512), 0, stream, a) : launch_kernel(silu_backward_kernel<false, false>, grid, dim3(512), 0, stream, a);
+  const bool once = quantize_loads_once((int64_t)a.rows * a.F);
+  hipError_t e = hipSuccess;
+#define MX_CASE(FLOOR, PLAIN, ONCE) \
+  if ((a.scale_mode != 0) == FLOOR && plain == PLAIN && (plain && once) == ONCE) \
+    e = launch_kernel(silu_backward_kernel<FLOOR, PLAIN, ONCE>, grid, dim3(512), 0, stream, a);
+  MX_CASE(true, true, true)
+  MX_CASE(true, true, false)
+  MX_CASE(true, false, false)
+  MX_CASE(false, true, true)
+  MX_CASE(false, true, false)
+  MX_CASE(false, false, false)
+#undef MX_CASE
   if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "silu_backward_kernel launch: %s", hipGetErrorString(e));
   return MX_OK;
 }

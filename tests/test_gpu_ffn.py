@@ -45,6 +45,61 @@ def test_gated_product(ct, dev, M, K, F, w_fmt):
         assert torch.equal(u8(q2), u8(q)) and torch.equal(u8(s2), u8(s))
 
 
+@pytest.mark.parametrize("a_fmt,w_fmt", [("e4m3", "e4m3"), ("e4m3", "e2m1"), ("e5m2", "e5m2"), ("e2m1", "e2m1")])
+@pytest.mark.parametrize("M,K,F", [(1, 32, 64), (100, 544, 192), (257, 512, 128), (300, 1536, 448), (770, 1024, 2112), (1025, 2048, 2944)])
+def test_gated_product_in_one_kernel(ct, dev, M, K, F, a_fmt, w_fmt):
+    """Tiles that overhang rows and columns, one and several tiles a workgroup, K that is no whole number of stages."""
+    fmt = {"e4m3": O.E4M3, "e5m2": O.E5M2, "e2m1": O.E2M1}
+    a, w = randn_operand(M, K, fmt[a_fmt], M + K, dev), randn_operand(2 * F, K, fmt[w_fmt], F, dev, std=K ** -0.5)
+    gu = R.bf16(O.dequantize(a.codes, a.scales, a.fmt).double() @ O.dequantize(w.codes, w.scales, w.fmt).double().T)
+    kw = dict(a_format=a.fmt_kw, w_format=w.fmt_kw, kernel="pingpong")
+    for a_s, w_s in ((a.scale_t, w.scale_t), (ct.pack_scales(a.scale_t, operand="a"), ct.pack_scales(w.scale_t, operand="b"))):
+        h, cq, cs = ct.gated_block_scaled_matmul(a.storage, a_s, w.storage, w_s, checkpoint=True, **kw)
+        q, s = ct.gated_block_scaled_matmul(a.storage, a_s, w.storage, w_s, out_dtype="e4m3", **kw)
+        assert R.rel(h, R.silu_mul(gu)) <= R.HALF_BF16 + 2 * BF16_FLIPS
+        assert R.rel(R.value(q, s), R.rows(R.silu_mul(gu))) <= 2 * E4M3_FLIPS
+        assert R.rel(R.value(cq, cs), R.rows(gu)) <= 2 * E4M3_FLIPS
+    # its codes are those of the single operators for its own bf16 numbers, but where silu's last bits decide
+    wq, ws = ct.block_quantize(h, 32, torch.float8_e4m3fn, scale_mode="floor")
+    # (h was rounded to bf16 before: up to 2^-8 off, of which a share of 2^-8 / step elements move by a step of up to 2^-3)
+    assert R.rel(R.value(q, s), R.value(wq, ws)) <= (R.HALF_BF16 * 2.0 ** -3) ** 0.5
+
+
+def test_gated_product_in_one_kernel_extremes(ct, dev):
+    """Blocks of zeros, of subnormal and of very large numbers, NaN: rows and scales of the operands that lead to them."""
+    M, K, F = 300, 512, 512
+    a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(2 * F, K, O.E4M3, 2, dev, std=K ** -0.5)
+    u8(a.storage)[5] = 0
+    u8(a.scale_t)[6:9] = torch.tensor([[3], [20], [200]], dtype=torch.uint8, device=dev)
+    u8(a.storage)[10, 3] = 0x7F
+    u8(w.storage)[64:96] = 0
+    gu = ct.block_scaled_matmul(a.storage, a.scale_t, w.storage.T, w.scale_t.T, out_dtype=torch.bfloat16, kernel="pingpong")
+    h, cq, cs = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, checkpoint=True, kernel="pingpong")
+    wq, ws = ct.block_quantize(gu, 32, torch.float8_e4m3fn, scale_mode="floor")
+    keep = [i for i in range(M) if i != 10]
+    assert torch.equal(u8(cq)[keep], u8(wq)[keep]) and torch.equal(u8(cs)[keep], u8(ws)[keep])
+    assert bool(h[10].isnan().all()) and bool(cq[10].float().isnan().all()) and not bool(h[keep].isnan().any())
+    assert float(h[5].abs().max()) == 0 and float(h[:, 64:96][keep].abs().max()) == 0
+
+
+def test_gated_product_in_one_kernel_nan(ct, dev):
+    """A NaN element and a NaN scale reach their row's every column, in the first and in later tiles of a workgroup's walk, and no other row."""
+    M, K, F = 2400, 512, 4096                          # more tiles than workgroups
+    a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(2 * F, K, O.E4M3, 2, dev, std=K ** -0.5)
+    want = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, kernel="pingpong")
+    rows = list(range(3, M, 97))
+    for n, r in enumerate(rows):
+        if n % 2:
+            u8(a.scale_t)[r, n % 16] = 0xFF
+        else:
+            u8(a.storage)[r, 17 * n % K] = 0x7F
+    got, cq, cs = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, checkpoint=True, kernel="pingpong")
+    q, s = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, out_dtype="e4m3", kernel="pingpong")
+    keep = [i for i in range(M) if i not in set(rows)]
+    assert bool(got[rows].isnan().all()) and bool(cq[rows].float().isnan().all()) and bool(q[rows].float().isnan().all())
+    assert torch.equal(got[keep], want[keep]) and not bool(cq[keep].float().isnan().any())
+
+
 @pytest.mark.parametrize("M,K,F,mode", [(5, 256, 64, "ceil"), (300, 512, 512, "ceil"), (300, 512, 512, "floor")])
 def test_gated_product_is_the_pair_of_operators(ct, dev, M, K, F, mode):
     """The same bits as the projections in bf16, then silu_and_mul_quantize, and block_quantize of the former."""

@@ -145,6 +145,23 @@ def test_silu_backward_special_values(ct, dev):
         assert bool(((v - m).abs()[~nan] <= 0.141 * top[~nan] + 2.0 ** -126).all())
 
 
+def test_silu_backward_nan_in_the_checkpoint(ct, dev):
+    """NaN codes and NaN scales of the checkpoint, and nothing else, give NaN."""
+    M, F = 64, 64
+    g = torch.Generator().manual_seed(7)
+    gq, gs = checkpoint(ct, torch.randn((M, 2 * F), generator=g).to(dev))
+    gq.view(torch.uint8)[5, 7] = 0x7F
+    gq.view(torch.uint8)[6, F + 9] = 0xFF
+    gs.view(torch.uint8)[9, 1] = 0xFF
+    dh = torch.randn((M, F), generator=g).to(torch.bfloat16)
+    for mode in ("floor", "ceil"):
+        got = ct.silu_and_mul_backward_quantize(dh.to(dev), gq, gs, scale_mode=mode)
+        d, a = R.silu_mul_backward(dh.double(), torch.where(gq.cpu().float().isnan(), float("nan"), R.value(gq.cpu().float().nan_to_num(), gs))
+                                   + torch.where(gs.cpu().view(torch.uint8) == 255, float("nan"), 0.0).repeat_interleave(32, -1))
+        for got_q, m in ((got[0], d), (got[2], R.padded_t(d)), (got[4], R.padded_t(a))):
+            assert torch.equal(got_q.float().isnan().cpu(), m.isnan())
+
+
 def test_silu_backward_of_views(ct, dev):
     """Rows that are not aligned, or apart, give the bits of contiguous ones."""
     M, F = 50, 96
