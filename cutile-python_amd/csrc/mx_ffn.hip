@@ -178,6 +178,11 @@ FfnBackward ffn_backward(uint8_t* base, const FfnShape& s) {
   r.o_dw2 = layouts(true, act);
   r.work_bytes = std::max(std::max(mx_gemm_workspace_bytes(s.T, s.F, s.Ho, &r.o_dh), mx_gemm_workspace_bytes(s.T, s.H, 2 * s.F, &r.o_dx)),
                           std::max(mx_gemm_workspace_bytes(2 * s.F, s.H, s.Tp, &r.o_dw1), mx_gemm_workspace_bytes(s.Ho, s.F, s.Tp, &r.o_dw2)));
+  if (s.T <= 64) {   // the gradients of both weights in one launch
+    const mx_tensor A[2] = {tensor2d(nullptr, MX_E4M3, 2 * s.F, s.Tp, s.Tp), tensor2d(nullptr, MX_E4M3, s.Ho, s.Tp, s.Tp)};
+    const mx_tensor B[2] = {transposed(tensor2d(nullptr, MX_E4M3, s.H, s.Tp, s.Tp)), transposed(tensor2d(nullptr, MX_E4M3, s.F, s.Tp, s.Tp))};
+    r.work_bytes = std::max(r.work_bytes, mx_gemm_list_workspace_bytes(2, A, B, &r.o_dw1));
+  }
   r.work = d.take(r.work_bytes);
   r.bytes = d.at;
   return r;
@@ -407,6 +412,15 @@ int mx_ffn_backward(const mx_tensor* dy, const void* saved, int64_t saved_bytes,
   if (int rc = launch_silu_backward(a, st)) return rc;
   if (dx)
     if (int rc = product(b.d, b.ds, k.w1t, k.w1ts, *dx, s.T, s.H, 2 * s.F, b.o_dx, b.work, b.work_bytes, stream)) return rc;
+  // few tokens: the products of the weights' gradients are short and only their output takes time, so both go out in one launch
+  if (s.T <= 64 && dw1 && dw2 && b.native_act && dw1->dtype == dw2->dtype) {
+    const mx_tensor A[2] = {tensor2d(b.dt, MX_E4M3, 2 * s.F, s.Tp, s.Tp), tensor2d(b.dyt, MX_E4M3, s.Ho, s.Tp, s.Tp)};
+    const mx_tensor As[2] = {tensor2d(b.dts, MX_E8M0, 2 * s.F, s.Tp / 32, s.Tp / 32), tensor2d(b.dyts, MX_E8M0, s.Ho, s.Tp / 32, s.Tp / 32)};
+    const mx_tensor B[2] = {transposed(tensor2d(k.xt, MX_E4M3, s.H, s.Tp, s.Tp)), transposed(tensor2d(b.at, MX_E4M3, s.F, s.Tp, s.Tp))};
+    const mx_tensor Bs[2] = {transposed(tensor2d(k.xts, MX_E8M0, s.H, s.Tp / 32, s.Tp / 32)), transposed(tensor2d(b.ats, MX_E8M0, s.F, s.Tp / 32, s.Tp / 32))};
+    mx_tensor C[2] = {*dw1, *dw2};
+    return mx_gemm_list(2, A, As, B, Bs, C, &b.o_dw1, b.work, b.work_bytes, stream);
+  }
   if (dw1)
     if (int rc = product(b.dt, b.dts, k.xt, k.xts, *dw1, 2 * s.F, s.H, s.Tp, b.o_dw1, b.work, b.work_bytes, stream)) return rc;
   if (dw2)
