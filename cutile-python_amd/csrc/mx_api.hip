@@ -1584,13 +1584,41 @@ int mx_silu_mul_quantize(const mx_tensor* gate_up, mx_tensor* xq, mx_tensor* sca
 }  // extern "C"
 
 namespace mx {
-// A gated product on the ping-pong kernel, whose epilogue makes of gate and up what is asked for.  kGatedNotFused: it goes through
-// memory instead (nothing enqueued).  W [2 F, K]; the scales as o's layouts say, of W's rows.
+// The streaming kernel with the gate in its epilogue against the product through memory and a pass over it.  A workgroup of the fused
+// kernel owns 32 columns of the result and all of K, so what grows is each wave's share of a row of W; the separate kernels split K
+// over workgroups as well.  Measured, fused and through memory, us (K x F, rows; FP8 unless noted):
+//   2048 x 7168 1: 7.8 and 10.0; 4096 x 14336 1: 21.4 and 24.1, 32: 24.9 and 27.8; 8192 x 4096 1: 13.2 and 18.8; 8192 x 14336 32: 45.7 and 48.8
+//   rows of W over 8192 bytes:                      16384 x 4096 1: 34.3 and 31.5, 16384 x 7168 16: 50.2 and 43.8 (FP4, 8192 bytes: 25.8 and 29.0)
+//   fewer than 128 workgroups, rows over 4096:      8192 x 2048 1: 11.2 and 10.5, 32: 14.5 and 12.0; 4096 x 2048 32: 9.5 and 10.2
+//   FP4, 17 to 32 rows, K over 4096: X is as long as W's rows are twice over; 8192 x 2048 12.3 and 11.4, 8192 x 7168 14.6 and 18.9, and for
+//   8192 x 14336, where the decode kernel reads plain scales best, 31.3 and 25.7, with packed ones 29.3 and 31.3
+static bool stream_gated_wins(const StreamArgs& a, int F) {
+  const int64_t row = a.w_fmt == MX_E2M1 ? a.K / 2 : a.K;
+  const int blocks = F / 32;
+  if (row > (blocks >= 128 ? 8192 : 4096)) return false;
+  return a.w_fmt != MX_E2M1 || a.M <= 16 || a.K <= 4096 || (blocks >= 128 && (blocks <= 256 || a.ws_packed));
+}
+
+// A gated product on the streaming kernel (few rows) or on the ping-pong kernel, whose epilogues make of gate and up what is asked
+// for.  kGatedNotFused: it goes through memory instead (nothing enqueued).  W [2 F, K]; the scales as o's layouts say, of W's rows.
 int gemm_gated_fused(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const GateOut& out, const mx_gemm_opts& o,
                      void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   const int64_t M = A.shape[0], K = A.shape[1], N = W.shape[0];
-  if ((o.kernel != MX_KERNEL_AUTO && o.kernel != MX_KERNEL_MFMA_PINGPONG) || o.block_size != 32 || o.split_k > 1) return kGatedNotFused;
-  if (N != 2 * (int64_t)out.F || out.F % 64 != 0 || out.scale_mode != 1 || (out.h_fmt != MX_BF16 && out.h_fmt != MX_E4M3)) return kGatedNotFused;
+  if (o.block_size != 32 || o.split_k > 1) return kGatedNotFused;
+  if (N != 2 * (int64_t)out.F || out.F % 32 != 0 || out.scale_mode != 1 || (out.h_fmt != MX_BF16 && out.h_fmt != MX_E4M3)) return kGatedNotFused;
+  if (M <= kStreamGatedRows && (o.kernel == MX_KERNEL_AUTO || o.kernel == MX_KERNEL_STREAM) && As.dtype == MX_E8M0 && Ws.dtype == MX_E8M0 &&
+      W.shape[1] == K && K < (1 << 30) && N < (1 << 30) && A.stride[1] == 1 && W.stride[1] == 1 && (W.dtype != MX_E2M1 || W.packed_dim == 1) &&
+      o.a_scale_layout == MX_SCALE_2D && As.ndim == 2 && As.shape[0] == M && As.shape[1] == K / 32 && As.stride[1] == 1 &&
+      (o.b_scale_layout == MX_SCALE_NATIVE ||
+       (o.b_scale_layout == MX_SCALE_2D && Ws.ndim == 2 && Ws.shape[0] == N && Ws.shape[1] == K / 32 && Ws.stride[1] == 1))) {
+    StreamArgs sa = {};
+    sa.X = (const uint8_t*)A.ptr; sa.Xs = (const uint8_t*)As.ptr; sa.W = (const uint8_t*)W.ptr; sa.Ws = (const uint8_t*)Ws.ptr;
+    sa.M = (int32_t)M; sa.N = (int32_t)N; sa.K = (int32_t)K;
+    sa.ldx = A.stride[0]; sa.ldxs = As.stride[0]; sa.ldw = W.stride[0]; sa.ldws = Ws.stride[0];
+    sa.x_fmt = A.dtype; sa.w_fmt = W.dtype; sa.ws_packed = o.b_scale_layout == MX_SCALE_NATIVE;
+    if (!stream_issue(sa) && (o.kernel == MX_KERNEL_STREAM || stream_gated_wins(sa, out.F))) return launch_gemm_stream_gated(sa, out, stream);
+  }
+  if ((o.kernel != MX_KERNEL_AUTO && o.kernel != MX_KERNEL_MFMA_PINGPONG) || out.F % 64 != 0) return kGatedNotFused;
   if (!pair_supported_by_mfma(A.dtype, W.dtype) || As.dtype != MX_E8M0 || Ws.dtype != MX_E8M0 || K == 0 || K % 32 != 0 || W.shape[1] != K ||
       M >= (1 << 30) || N >= (1 << 30) || K >= (1 << 30))
     return kGatedNotFused;

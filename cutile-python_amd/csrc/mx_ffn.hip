@@ -259,11 +259,26 @@ int mx_gated_gemm(const mx_tensor* A, const mx_tensor* As, const mx_tensor* W, c
   mx_gemm_opts o = opts ? *opts : kPlainOpts;
   if (!A || !As || !W || !Ws) return set_error(MX_ERR_INVALID, "mx_gated_gemm: null descriptor");
   if (A->ndim != 2 || W->ndim != 2) return set_error(MX_ERR_SHAPE, "mx_gated_gemm: A and W must have 2 dimensions");
+  for (const mx_tensor* t : {A, W})
+    if (t->shape[0] < 0 || t->shape[1] < 0) return set_error(MX_ERR_SHAPE, "mx_gated_gemm: negative extent");
+  if (A->shape[1] != W->shape[1])
+    return set_error(MX_ERR_SHAPE, "Incompatible matrices: K dimension of A (%lld) must match K dimension of W (%lld)", (long long)A->shape[1],
+                     (long long)W->shape[1]);
   const int64_t M = A->shape[0], K = A->shape[1], F = W->shape[0] / 2;
   if (W->shape[0] % 2 != 0) return set_error(MX_ERR_SHAPE, "W must have 2F rows (gate and up projection), got %lld", (long long)W->shape[0]);
   if (F == 0 || F % 32 != 0) return set_error(MX_ERR_SHAPE, "F (%lld) must be a multiple of 32", (long long)F);
   if (M >= kMaxExtent || F >= kMaxExtent / 2 || K >= kMaxExtent) return set_error(MX_ERR_SHAPE, "mx_gated_gemm: extent out of range");
   if (int rc = check_mode(scale_mode)) return rc;
+  const struct { const mx_tensor* t; const char* name; int64_t rows, cols; bool plain; } ins[4] = {
+      {A, "A", M, K, true}, {W, "W", 2 * F, K, true}, {As, "A_scale", M, K / 32, o.a_scale_layout == MX_SCALE_2D},
+      {Ws, "W_scale", 2 * F, K / 32, o.b_scale_layout == MX_SCALE_2D}};
+  for (const auto& i : ins) {
+    if (i.plain && (i.t->ndim != 2 || i.t->shape[0] != i.rows || i.t->shape[1] != i.cols))
+      return set_error(MX_ERR_SHAPE, "%s must be [%lld, %lld]", i.name, (long long)i.rows, (long long)i.cols);
+    for (int n = 0; n < i.t->ndim && n < 4; ++n)
+      if (i.t->stride[n] < 0) return set_error(MX_ERR_LAYOUT, "%s: negative strides are not supported", i.name);
+    if (M > 0 && K > 0 && !i.t->ptr) return set_error(MX_ERR_INVALID, "%s: null data pointer", i.name);
+  }
   GateOut g = {};
   if (int rc = check2d(out, "out", M, F)) return rc;
   g.h = out->ptr; g.h_ld = out->stride[0]; g.h_fmt = out->dtype;

@@ -22,6 +22,10 @@ struct StreamPlan { int mt, m_tiles, nt, kw, units; float cost; };
 StreamPlan stream_plan(int64_t M, int64_t N, int64_t K, int w_fmt);
 int launch_gemm_stream(const StreamArgs& a, hipStream_t stream);
 
+// the gated form of up to kStreamGatedRows rows (mx_gemm_stream_gated.hip): N = 2 F, F % 32 == 0
+constexpr int64_t kStreamGatedRows = 32;
+int launch_gemm_stream_gated(const StreamArgs& a, const GateOut& o, hipStream_t stream);
+
 // mixture-of-experts layer at decode sizes (mx_moe.hip)
 // Routed ids that a workgroup sorts out by itself, in a list of 4 KiB of LDS.  With room for 8192 two workgroups of the FP4
 // form no longer fit on a CU and its layers take 10 - 40 % longer (8 experts of 4096 x 14336, 16 rows each: 156 -> 184 us).

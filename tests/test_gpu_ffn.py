@@ -65,6 +65,58 @@ def test_gated_product_in_one_kernel(ct, dev, M, K, F, a_fmt, w_fmt):
     assert R.rel(R.value(q, s), R.value(wq, ws)) <= (R.HALF_BF16 * 2.0 ** -3) ** 0.5
 
 
+@pytest.mark.parametrize("a_fmt,w_fmt", [("e4m3", "e4m3"), ("e4m3", "e2m1"), ("e5m2", "e5m2"), ("e5m2", "e2m1")])
+@pytest.mark.parametrize("M,K,F", [(1, 128, 32), (2, 640, 96), (7, 1152, 64), (16, 2048, 160), (17, 512, 32), (29, 1664, 224), (32, 4224, 96)])
+def test_gated_product_streamed(ct, dev, M, K, F, a_fmt, w_fmt):
+    """Few rows: one and two row tiles, one to four K ranges of unequal lengths, K within a range's last 512, F of odd multiples of 32, strided rows."""
+    fmt = {"e4m3": O.E4M3, "e5m2": O.E5M2, "e2m1": O.E2M1}
+    a, w = randn_operand(M, K, fmt[a_fmt], M + K, dev), randn_operand(2 * F, K, fmt[w_fmt], F, dev, std=K ** -0.5)
+    gu = R.bf16(O.dequantize(a.codes, a.scales, a.fmt).double() @ O.dequantize(w.codes, w.scales, w.fmt).double().T)
+    kw = dict(a_format=a.fmt_kw, w_format=w.fmt_kw, kernel="stream")
+    wide = torch.full((M, K + 48), 0x7F, dtype=torch.uint8, device=dev)      # rows with NaN codes behind them
+    wide[:, :K] = u8(a.storage)
+    strided = wide.view(a.storage.dtype)[:, :K]
+    first = None
+    for a_q, w_s in ((a.storage, w.scale_t), (strided, ct.pack_scales(w.scale_t, operand="b"))):
+        h, cq, cs = ct.gated_block_scaled_matmul(a_q, a.scale_t, w.storage, w_s, checkpoint=True, **kw)
+        q, s = ct.gated_block_scaled_matmul(a_q, a.scale_t, w.storage, w_s, out_dtype="e4m3", **kw)
+        assert R.rel(h, R.silu_mul(gu)) <= R.HALF_BF16 + 2 * BF16_FLIPS
+        assert R.rel(R.value(q, s), R.rows(R.silu_mul(gu))) <= 2 * E4M3_FLIPS
+        assert R.rel(R.value(cq, cs), R.rows(gu)) <= 2 * E4M3_FLIPS
+        got = [u8(t).clone() for t in (h, cq, cs, q, s)]
+        assert first is None or all(torch.equal(x, y) for x, y in zip(got, first))
+        first = got
+
+
+def test_gated_product_streamed_nan(ct, dev):
+    """NaN elements and scales of a row stay in it; a NaN in W reaches its column, and its MX block, of every row."""
+    M, K, F = 20, 1024, 256
+    a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(2 * F, K, O.E4M3, 2, dev, std=K ** -0.5)
+    want, wcq, wcs = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, checkpoint=True, kernel="stream")
+    u8(a.storage)[4, 1000] = 0x7F
+    u8(a.scale_t)[18, 3] = 0xFF
+    u8(w.storage)[70, 5] = 0xFF                       # a gate row
+    u8(w.scale_t)[F + 131, 31] = 0xFF                 # an up row
+    h, cq, cs = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, checkpoint=True, kernel="stream")
+    rows, cols = [i for i in range(M) if i not in (4, 18)], [j for j in range(F) if j not in (70, 131)]
+    assert bool(h[[4, 18]].isnan().all()) and bool(h[:, [70, 131]].isnan().all()) and bool(cq[[4, 18]].float().isnan().all())
+    assert torch.equal(h[rows][:, cols], want[rows][:, cols])
+    keep = [j for j in range(2 * F) if j // 32 not in (70 // 32, (F + 131) // 32)]
+    assert torch.equal(u8(cq)[rows][:, keep], u8(wcq)[rows][:, keep])
+    assert bool(cq[:, [70, F + 131]].float().isnan().all())
+
+
+def test_gated_product_is_chosen_by_size(ct, dev):
+    """Where the streaming kernel is taken by default, its bits; explicit kernels and the others agree to their bounds."""
+    for M, K, F, w_fmt in ((1, 2048, 4096, O.E4M3), (32, 8192, 2048, O.E4M3), (32, 8192, 1024, O.E2M1), (33, 1024, 512, O.E4M3)):
+        a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(2 * F, K, w_fmt, 2, dev, std=K ** -0.5)
+        got = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, w_format=w.fmt_kw)
+        for kernel in ("stream", "pingpong", "mfma128"):
+            other = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, w_format=w.fmt_kw, kernel=kernel)
+            # elements whose gate and up flip at no kernel are the same; a flip of each, and the result's own rounding behind them
+            assert R.rel(got, other.cpu().double()) <= 4 * BF16_FLIPS
+
+
 def test_gated_product_in_one_kernel_extremes(ct, dev):
     """Blocks of zeros, of subnormal and of very large numbers, NaN: rows and scales of the operands that lead to them."""
     M, K, F = 300, 512, 512
