@@ -13,8 +13,8 @@ from .errors import TileTypeError, TileValueError
 from .ops import (PackedScales, bench_block_scaled_matmul, block_quantize, clear_scale_cache, block_scaled_matmul, cutile_block_scaled_matmul,
                   cutile_moe_scaled, grouped_block_scaled_matmul, invoke_fused_moe_scaled, mma_scaled, moe_align_tile_size, pack_scales,
                   silu_and_mul_quantize, swizzle_32_4_4, unswizzle_32_4_4)
-from .ffn import (block_quantize_both, gated_block_scaled_matmul, gated_feed_forward, gated_feed_forward_backward,
-                  gated_feed_forward_forward, silu_and_mul_backward_quantize)
+from .ffn import (FeedForwardState, block_quantize_both, gated_block_scaled_matmul, gated_feed_forward,
+                  gated_feed_forward_backward, gated_feed_forward_forward, silu_and_mul_backward_quantize)
 
 __all__ = [
     "LIB_PATH", "MXLibraryError", "lib", "TileTypeError", "TileValueError", "PackedScales",
@@ -22,5 +22,5 @@ __all__ = [
     "mma_scaled", "moe_align_tile_size", "pack_scales", "swizzle_32_4_4", "unswizzle_32_4_4",
     "silu_and_mul_quantize", "cutile_moe_scaled", "grouped_block_scaled_matmul", "bench_block_scaled_matmul",
     "clear_scale_cache", "block_quantize_both", "gated_block_scaled_matmul", "silu_and_mul_backward_quantize",
-    "gated_feed_forward", "gated_feed_forward_forward", "gated_feed_forward_backward",
+    "gated_feed_forward", "gated_feed_forward_forward", "gated_feed_forward_backward", "FeedForwardState",
 ]
