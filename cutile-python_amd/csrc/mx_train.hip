@@ -68,7 +68,8 @@ __device__ __forceinline__ void store_scales(const uint32_t* lds, uint8_t* s, in
 // PLAIN: aligned rows of whole blocks that do not overlap, tiles of less than 2 GiB.  Loads and stores then go through buffer
 // descriptors of the tile, whose range takes the place of every comparison with the matrix's ends, and magnitudes of 16-bit input
 // are compared two at a time as they lie in memory.  The vector ALUs are what the rest of the time is spent on otherwise: with
-// the comparisons, 64-bit addresses and the scale rule decided per block 8192 x 8192 bf16 took 56 us, now KERNEL_BOTH_US.
+// the comparisons, 64-bit addresses and the scale rule decided per block 8192 x 8192 bf16 took 56 us, now 50 (5.4 TB/s); a copy of
+// 2 GiB reaches 5.1 TB/s, where what was just written is in no cache, and this kernel 4.4 of 32768 x 14336.
 template <int SRC>
 __device__ __forceinline__ float load_one(const void* x, int64_t at) {
   if constexpr (SRC == MX_F32) return ((const float*)x)[at];
@@ -342,9 +343,11 @@ __global__ __launch_bounds__(256) void gate_up_kernel(const GateUpArgs a) {
 // g and u are the checkpoint's values.  d[g|u] goes out quantised along the rows (for the product with w1) and along the columns
 // (for the gradient of w1), a along the columns (for the gradient of w2; the forward pass kept no copy of it, which saves 8.25 bits per element from
 // one pass to the other for one multiplication here).
-// Bound: memory, 4.06 bytes read and 5.16 written an element of dh.  A workgroup takes 128 rows x 128 columns (whole lines both ways), a wave 32 x 64, a lane 4 rows
-// x 8 columns (rows 4 (lane / 8) .., columns 8 (lane % 8) ..), one result after the other: 32 numbers that stay in registers until
-// their rows' and columns' maxima are known, beside g s, which the second and the third are made of.
+// Bound: memory, 4.06 bytes read and 5.16 written an element of dh.  A workgroup takes 128 rows x 128 columns (whole lines both
+// ways), a wave 32 x 64, a lane 4 rows x 8 columns (rows 4 (lane / 8) .., columns 8 (lane % 8) ..), one result after the other: 32
+// numbers that stay in registers until their rows' and columns' maxima are known, beside g s, which the second and the third are
+// made of.  4096 x 14336: 125 us where every call writes the same memory, 138 (3.9 TB/s) where it is another; a copy of 2 GiB reaches
+// 5.1 TB/s, and the difference goes into eight streams of one line a row each.
 // g -> g s and s (1 + g (1 - s)) = s + g s - g s s; exp through the hardware's 2^x and a reciprocal: a few units in the last
 // place, against the 2^-4 of what follows
 __device__ __forceinline__ void silu_slope(float g, float& gs, float& slope) {
@@ -415,7 +418,7 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
     load_dh(r0, k0);
     load_gate_or_up(r0, k0, F, rup);
     // the four blocks' scales of a row of g or u at a time: by the byte, each lane its own, they were as many requests as the codes
-    // (4096 x 14336 152 -> KERNEL_SILU_US us)
+    // (4096 x 14336 152 -> 145 us)
     if (tid < 256) {
       const int o = tid >> 7, r = tid & 127;
       uint32_t w = 0;
@@ -429,112 +432,113 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
     }
     __syncthreads();
     if (lr - 4 * rg < n_rows) {                        // (waves without rows have nothing to do)
-    auto scale_in = [&](int o, int i) { return (uint32_t)((const uint8_t*)sin[o])[(lr + i) * 4 + lc / 32]; };
-    const __amdgpu_buffer_rsrc_t rd = make_rsrc(a.d + r0 * a.d_ld + k0, PLAIN ? (uint32_t)((n_rows - 1) * a.d_ld + F + n_cols) : 0u);
-    // (The maxima pass over NaN: it is NaN among codes of its block's other values.)
-    // one result at a time, 32 numbers of a lane: out along the rows (dg, du), then along the columns
-    auto row_out = [&](int o, const float (&v)[4][8]) {
+      auto scale_in = [&](int o, int i) { return (uint32_t)((const uint8_t*)sin[o])[(lr + i) * 4 + lc / 32]; };
+      const __amdgpu_buffer_rsrc_t rd = make_rsrc(a.d + r0 * a.d_ld + k0, PLAIN ? (uint32_t)((n_rows - 1) * a.d_ld + F + n_cols) : 0u);
+      // (The maxima pass over NaN: it is NaN among codes of its block's other values.)
+      // one result at a time, 32 numbers of a lane: out along the rows (dg, du), then along the columns
+      auto row_out = [&](int o, const float (&v)[4][8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float m = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = fmax_abs(m, v[i][e]);
+          const BlockScale b = block_scale<MX_E4M3, FLOOR>(max_quad(__builtin_bit_cast(uint32_t, m)));
+          const float (&w)[8] = v[i];
+          const u2 c = {encode4<MX_E4M3>(w[0], w[1], w[2], w[3], b.scale), encode4<MX_E4M3>(w[4], w[5], w[6], w[7], b.scale)};
+          if constexpr (PLAIN) {
+            const uint32_t in = col_in && lr + i < n_rows ? 0 : kOobOffset;
+            __builtin_amdgcn_raw_buffer_store_b64(c, rd, in | ((lr + i) * (uint32_t)a.d_ld + o * (uint32_t)F + lc), 0, 0);
+          } else if (row + i < rows && col_in) {
+            *(u2*)(a.d + (row + i) * a.d_ld + o * F + col) = c;
+          }
+          ((uint8_t*)srow[o])[(lr + i) * 4 + lc / 32] = (uint8_t)b.byte;
+        }
+      };
+      auto place = [&](int o, int e, uint32_t c) {
+        *(uint32_t*)(tile[o] + (lc + e) * 128 + (((2 * wave + (rg >> 2)) ^ cg) << 4) + (rg & 3) * 4) = c;
+      };
+      auto col_out = [&](int o, const float (&v)[4][8]) {
+        uint32_t m[8], own[2];
+        float scale[2], s[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          m[e] = __builtin_bit_cast(uint32_t, fmax_abs(fmax_abs(fmax_abs(__builtin_fabsf(v[0][e]), v[1][e]), v[2][e]), v[3][e]));
+        max_columns(m, own);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const BlockScale b = block_scale<MX_E4M3, FLOOR>(max_xor_8(own[e]));
+          scale[e] = b.scale;
+          ((uint8_t*)scol[o])[(lc + own_column(lane) + e) * 4 + wave] = (uint8_t)b.byte;
+        }
+        spread_columns(scale, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) place(o, e, encode4<MX_E4M3>(v[0][e], v[1][e], v[2][e], v[3][e], s[e]));
+      };
+      // (zeros out of range make zeros: 2^-127 * 0, 0 * 0.5)
+      auto decoded = [](const u2& c, uint32_t byte, float (&out)[8]) {
+        const float scale = __builtin_bit_cast(float, byte << 23);   // (the conversion takes the exponent: 0 is 2^-127, 255 NaN)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const f2 p = (h & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[h >> 1], scale, true) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[h >> 1], scale, false);
+          out[2 * h] = p[0];
+          out[2 * h + 1] = p[1];
+        }
+      };
+      float v[4][8], gs[4][8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float m = 0.f;
+        float g[8];
+        decoded(rgt[i], scale_in(0, i), g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmax_abs(m, v[i][e]);
-        const BlockScale b = block_scale<MX_E4M3, FLOOR>(max_quad(__builtin_bit_cast(uint32_t, m)));
-        const float (&w)[8] = v[i];
-        const u2 c = {encode4<MX_E4M3>(w[0], w[1], w[2], w[3], b.scale), encode4<MX_E4M3>(w[4], w[5], w[6], w[7], b.scale)};
-        if constexpr (PLAIN) {
-          const uint32_t in = col_in && lr + i < n_rows ? 0 : kOobOffset;
-          __builtin_amdgcn_raw_buffer_store_b64(c, rd, in | ((lr + i) * (uint32_t)a.d_ld + o * (uint32_t)F + lc), 0, 0);
-        } else if (row + i < rows && col_in) {
-          *(u2*)(a.d + (row + i) * a.d_ld + o * F + col) = c;
-        }
-        ((uint8_t*)srow[o])[(lr + i) * 4 + lc / 32] = (uint8_t)b.byte;
+        for (int e = 0; e < 8; ++e) silu_slope(g[e], gs[i][e], v[i][e]);
       }
-    };
-    auto place = [&](int o, int e, uint32_t c) {
-      *(uint32_t*)(tile[o] + (lc + e) * 128 + (((2 * wave + (rg >> 2)) ^ cg) << 4) + (rg & 3) * 4) = c;
-    };
-    auto col_out = [&](int o, const float (&v)[4][8]) {
-      uint32_t m[8], own[2];
-      float scale[2], s[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        m[e] = __builtin_bit_cast(uint32_t, fmax_abs(fmax_abs(fmax_abs(__builtin_fabsf(v[0][e]), v[1][e]), v[2][e]), v[3][e]));
-      max_columns(m, own);
+      for (int i = 0; i < 4; ++i) {
+        float dh[8], u[8];
+        unpack_bf16(rdh[i], dh);
+        decoded(rup[i], scale_in(1, i), u);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const BlockScale b = block_scale<MX_E4M3, FLOOR>(max_xor_8(own[e]));
-        scale[e] = b.scale;
-        ((uint8_t*)scol[o])[(lc + own_column(lane) + e) * 4 + wave] = (uint8_t)b.byte;
+        for (int e = 0; e < 8; ++e) v[i][e] = dh[e] * u[e] * v[i][e];
       }
-      spread_columns(scale, s);
+      row_out(0, v);
+      col_out(0, v);
+      // (the next result is not begun before, and the inputs are unpacked again for it: more waves on a SIMD)
+      auto again = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) place(o, e, encode4<MX_E4M3>(v[0][e], v[1][e], v[2][e], v[3][e], s[e]));
-    };
-    // (zeros out of range make zeros: 2^-127 * 0, 0 * 0.5)
-    auto decoded = [](const u2& c, uint32_t byte, float (&out)[8]) {
-      const float scale = __builtin_bit_cast(float, byte << 23);   // (the conversion takes the exponent: 0 is 2^-127, 255 NaN)
+        for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(rup[i]));
+      };
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const f2 p = (h & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[h >> 1], scale, true) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[h >> 1], scale, false);
-        out[2 * h] = p[0];
-        out[2 * h + 1] = p[1];
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(rdh[i]));
+      again();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float dh[8];
+        unpack_bf16(rdh[i], dh);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = dh[e] * gs[i][e];
       }
-    };
-    float v[4][8], gs[4][8];
+      row_out(1, v);
+      col_out(1, v);
+      again();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float g[8];
-      decoded(rgt[i], scale_in(0, i), g);
+      for (int i = 0; i < 4; ++i) {
+        float u[8];
+        decoded(rup[i], scale_in(1, i), u);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) silu_slope(g[e], gs[i][e], v[i][e]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float dh[8], u[8];
-      unpack_bf16(rdh[i], dh);
-      decoded(rup[i], scale_in(1, i), u);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = dh[e] * u[e] * v[i][e];
-    }
-    row_out(0, v);
-    col_out(0, v);
-    // (the next result is not begun before, and the inputs are unpacked again for it: more waves on a SIMD)
-    auto again = [&]() {
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(rup[i]));
-    };
-#pragma unroll
-    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(rdh[i]));
-    again();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float dh[8];
-      unpack_bf16(rdh[i], dh);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = dh[e] * gs[i][e];
-    }
-    row_out(1, v);
-    col_out(1, v);
-    again();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float u[8];
-      decoded(rup[i], scale_in(1, i), u);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = gs[i][e] * u[e];
-    }
-    col_out(2, v);
+        for (int e = 0; e < 8; ++e) v[i][e] = gs[i][e] * u[e];
+      }
+      col_out(2, v);
     }
     __syncthreads();
+    // (whole lines that are not merged with others': not kept in the caches, 16384 x 14336 634 -> 570 us, 4096 x 14336 139 -> 125)
 #pragma unroll
     for (int n = 0; n < 6; ++n) {
       const int o = n >> 1, c = (n & 1) * 64 + (tid >> 3), j = tid & 7;
       if (c < n_cols && 16 * j < m_rows) {
         const u4 w = *(const u4*)(tile[o] + c * 128 + ((j ^ (c >> 3 & 7)) << 4));
         uint8_t* const p = o == 2 ? a.at + (k0 + c) * a.at_ld : a.dt + (o * F + k0 + c) * a.dt_ld;
-        *(u4*)(p + r0 + 16 * j) = w;
+        __builtin_nontemporal_store(w, (u4*)(p + r0 + 16 * j));
       }
     }
   }
