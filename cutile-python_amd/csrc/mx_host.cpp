@@ -641,8 +641,11 @@ struct FeedForward : torch::autograd::Function<FeedForward> {
     }
     const auto shape = ctx->saved_data["x"].toIntVector();
     if (want[0] && shape.size() != 2) r[0] = r[0].view(shape);
-    if (again)   // asked for a graph of the gradients: there is none
+    if (again) {   // asked for a graph of the gradients: there is none, and whoever differentiates them is to be told
+      for (at::Tensor& t : r)
+        if (t.defined()) t.set_requires_grad(true);
       r = torch::autograd::DelayedError("gated_feed_forward: its gradients cannot be differentiated", 3)(std::move(r));
+    }
     r.emplace_back();
     return r;
   }
