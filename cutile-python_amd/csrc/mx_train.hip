@@ -346,7 +346,7 @@ __global__ __launch_bounds__(256) void gate_up_kernel(const GateUpArgs a) {
 // Bound: memory, 4.06 bytes read and 5.16 written an element of dh.  A workgroup takes 128 rows x 128 columns (whole lines both
 // ways), a wave 32 x 64, a lane 4 rows x 8 columns (rows 4 (lane / 8) .., columns 8 (lane % 8) ..), one result after the other: 32
 // numbers that stay in registers until their rows' and columns' maxima are known, beside g s, which the second and the third are
-// made of.  4096 x 14336: 125 us where every call writes the same memory, 138 (3.9 TB/s) where it is another; a copy of 2 GiB reaches
+// made of.  4096 x 14336: 119 us where every call writes the same memory, 129 (4.2 TB/s) where it is another; a copy of 2 GiB reaches
 // 5.1 TB/s, and the difference goes into eight streams of one line a row each.
 // g -> g s and s (1 + g (1 - s)) = s + g s - g s s; exp through the hardware's 2^x and a reciprocal: a few units in the last
 // place, against the 2^-4 of what follows
@@ -357,7 +357,7 @@ __device__ __forceinline__ void silu_slope(float g, float& gs, float& slope) {
 }
 
 // Loads and stores through descriptors of the tile, as in quantize_both_kernel (the launcher's rule; PLAIN false: any pitch).
-// ONCE: dh and the checkpoint are loaded non-temporally (as the quantiser's input, mx_load_once.h: 4096 x 14336 146 -> 141 us).
+// ONCE: dh and the checkpoint are loaded non-temporally (as the quantiser's input, mx_load_once.h).
 template <bool FLOOR, bool PLAIN, bool ONCE>
 __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwardArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t tile[3][128 * 128];   // codes along columns: dg, du, a
@@ -370,20 +370,27 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
   // ---- the lane's inputs, of the tile that begins at (r0, k0): zeros outside of the matrix -------------------------------------
   v4i rdh[4];
   u2 rgt[4], rup[4];
-  auto load_gate_or_up = [&](int64_t r0, int64_t k0, int64_t at, u2 (&q)[4]) {   // at: 0 (gate), F (up)
-    const int n_rows = rows - r0 < 128 ? (int)(rows - r0) : 128;
-    const bool col_in = k0 + lc < F;
+  // at: 0 (gate), F (up).  PLAIN: 1 KiB of eight rows at a time into tile[o], 16-byte chunks swizzled by row / 4: a wave needs half lines
+  // only, and a line that two waves load non-temporally, half each, is fetched twice (4096 x 14336: 334 MB in place of 239,
+  // 142 us in place of 129; loaded plainly 134).
+  auto load_gate_or_up = [&](int64_t r0, int64_t k0, int o, u2 (&q)[4]) {
+    const int n_rows = rows - r0 < 128 ? (int)(rows - r0) : 128, n_cols = F - k0 < 128 ? (int)(F - k0) : 128;
+    const int64_t at = o * F;
     if constexpr (PLAIN) {
       const uint32_t pg = (uint32_t)a.gu_ld;
-      const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.gu + r0 * a.gu_ld + at + k0, (uint32_t)((n_rows - 1) * pg + F - k0));
+      const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.gu + r0 * a.gu_ld + at + k0, (uint32_t)((n_rows - 1) * pg + n_cols));
+      const int w8 = __builtin_amdgcn_readfirstlane(tid >> 6);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        q[i] = __builtin_amdgcn_raw_buffer_load_b64(rs, (col_in && lr + i < n_rows ? 0 : kOobOffset) | ((lr + i) * pg + lc), 0, ONCE ? kLoadOnce : 0);
+      for (int j = 0; j < 2; ++j) {
+        const int row = 16 * w8 + 8 * j + (lane >> 3), col = ((lane & 7) ^ (row >> 2 & 7)) * 16;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)((lds_u8*)tile[o] + (16 * w8 + 8 * j) * 128), 16,
+                                                 row < n_rows && col < n_cols ? row * pg + col : kOobOffset, 0, 0, ONCE ? kLoadOnce : 0);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         q[i] = (u2){0, 0};
-        if (lr + i < n_rows && col_in) q[i] = *(const u2*)(a.gu + (r0 + lr + i) * a.gu_ld + at + k0 + lc);
+        if (lr + i < n_rows && lc < n_cols) q[i] = *(const u2*)(a.gu + (r0 + lr + i) * a.gu_ld + at + k0 + lc);
       }
     }
   };
@@ -416,7 +423,7 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
     const bool col_in = lc < n_cols;
     load_gate_or_up(r0, k0, 0, rgt);
     load_dh(r0, k0);
-    load_gate_or_up(r0, k0, F, rup);
+    load_gate_or_up(r0, k0, 1, rup);
     // the four blocks' scales of a row of g or u at a time: by the byte, each lane its own, they were as many requests as the codes
     // (4096 x 14336 152 -> 145 us)
     if (tid < 256) {
@@ -430,7 +437,17 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
       }
       sin[o][r] = w;
     }
+    if constexpr (PLAIN) __builtin_amdgcn_s_waitcnt(0x0F70);   // the wave's share of g and u is in LDS
     __syncthreads();
+    if constexpr (PLAIN) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = (lr + i) * 128 + ((4 * half + (cg >> 1)) ^ rg) * 16 + (cg & 1) * 8;
+        rgt[i] = *(const u2*)(tile[0] + at);
+        rup[i] = *(const u2*)(tile[1] + at);
+      }
+      __syncthreads();                                 // codes along columns go there
+    }
     if (lr - 4 * rg < n_rows) {                        // (waves without rows have nothing to do)
       auto scale_in = [&](int o, int i) { return (uint32_t)((const uint8_t*)sin[o])[(lr + i) * 4 + lc / 32]; };
       const __amdgpu_buffer_rsrc_t rd = make_rsrc(a.d + r0 * a.d_ld + k0, PLAIN ? (uint32_t)((n_rows - 1) * a.d_ld + F + n_cols) : 0u);
@@ -659,7 +676,7 @@ int launch_silu_backward(const SiluBackwardArgs& args, hipStream_t stream) {
   const int64_t rows = native ? (a.rows + 511ll) / 512 * 512 : a.rows, blocks = (rows + 127) / 128 * a.tiles_k;
   if (blocks > 0x7FFFFFFF) return set_error(MX_ERR_SHAPE, "silu_backward: tensor too large");
   const int64_t lim = (int64_t)1 << 31;
-  const bool plain = (((uintptr_t)a.dh | (uintptr_t)(a.dh_ld * 2)) & 15) == 0 && a.dh_ld >= a.F && a.gu_ld >= 2 * a.F && a.gus_ld >= a.F / 16 &&
+  const bool plain = (((uintptr_t)a.dh | (uintptr_t)(a.dh_ld * 2) | (uintptr_t)a.gu | (uintptr_t)a.gu_ld | (uintptr_t)a.F) & 15) == 0 && a.dh_ld >= a.F && a.gu_ld >= 2 * a.F && a.gus_ld >= a.F / 16 &&
                      128 * a.dh_ld * 2 < lim && 128 * a.gu_ld < lim && 128 * a.gus_ld < lim && 128 * a.d_ld < lim;
   const dim3 grid((unsigned)blocks);
   const bool once = quantize_loads_once((int64_t)a.rows * a.F);

@@ -350,10 +350,14 @@ MX_API int mx_quantize_both(const mx_tensor* x, mx_tensor* xq, mx_tensor* scale,
  * the gate_up GEMM of samples/MoE.py:197-288 followed by silu_and_mul_kernel (test/kernels/fused_moe.py:85-108), dense.
  *   A [M,K], W [2F,K] (gate rows first; K contiguous), element formats, scales and layouts as in mx_gemm (Ws is
  *   [2F,K/32]; opts->a_scale_layout / b_scale_layout are As's / Ws's); F % 32 == 0
- *   out [M,F] MX_BF16 (out_scale NULL), or MX_E4M3 / MX_E5M2 with out_scale [M,F/32], as mx_silu_mul_quantize leaves it
+ *   out [M,F] MX_BF16 (out_scale NULL), or MX_E4M3 / MX_E5M2 with out_scale [M,F/32], in the format that
+ *   mx_silu_mul_quantize leaves.  SiLU is in 32 bits; where the product's own kernel finishes it (the floor rule, bf16 or
+ *   E4M3 out) by the hardware's 2^x and reciprocal, a few units in the last place from mx_silu_mul_quantize's
  *   gate_up [M,2F] MX_E4M3 with gate_up_scale [M,2F/32], optional (both NULL): [G|U] quantised, which is what
  *   mx_silu_mul_backward_quantize takes (8.25 bits an element from the forward to the backward pass)
- * Workspace: mx_gated_gemm_workspace_bytes().
+ * Kernels: opts->kernel MX_KERNEL_STREAM (M <= 32) or MX_KERNEL_MFMA_PINGPONG do all in one launch where they can, any
+ * other the product into the workspace and a pass over it; MX_KERNEL_AUTO takes what is faster.
+ * Workspace: mx_gated_gemm_workspace_bytes(), which holds every form; it is asked for whichever is taken.
  */
 MX_API int64_t mx_gated_gemm_workspace_bytes(int64_t M, int64_t F, int64_t K, const mx_gemm_opts* opts);
 MX_API int mx_gated_gemm(const mx_tensor* A, const mx_tensor* A_scale, const mx_tensor* W, const mx_tensor* W_scale,
