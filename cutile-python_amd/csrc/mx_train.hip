@@ -346,7 +346,7 @@ __global__ __launch_bounds__(256) void gate_up_kernel(const GateUpArgs a) {
 // Bound: memory, 4.06 bytes read and 5.16 written an element of dh.  A workgroup takes 128 rows x 128 columns (whole lines both
 // ways), a wave 32 x 64, a lane 4 rows x 8 columns (rows 4 (lane / 8) .., columns 8 (lane % 8) ..), one result after the other: 32
 // numbers that stay in registers until their rows' and columns' maxima are known, beside g s, which the second and the third are
-// made of.  4096 x 14336: 119 us where every call writes the same memory, 129 (4.2 TB/s) where it is another; a copy of 2 GiB reaches
+// made of.  4096 x 14336: 109 us where every call writes the same memory, 123 (4.4 TB/s) where it is another; a copy of 2 GiB reaches
 // 5.1 TB/s, and the difference goes into eight streams of one line a row each.
 // g -> g s and s (1 + g (1 - s)) = s + g s - g s s; exp through the hardware's 2^x and a reciprocal: a few units in the last
 // place, against the 2^-4 of what follows
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
   u2 rgt[4], rup[4];
   // at: 0 (gate), F (up).  PLAIN: 1 KiB of eight rows at a time into tile[o], 16-byte chunks swizzled by row / 4: a wave needs half lines
   // only, and a line that two waves load non-temporally, half each, is fetched twice (4096 x 14336: 334 MB in place of 239,
-  // 142 us in place of 129; loaded plainly 134).
+  // 142 us in place of 123; loaded plainly 134).
   auto load_gate_or_up = [&](int64_t r0, int64_t k0, int o, u2 (&q)[4]) {
     const int n_rows = rows - r0 < 128 ? (int)(rows - r0) : 128, n_cols = F - k0 < 128 ? (int)(F - k0) : 128;
     const int64_t at = o * F;
@@ -421,24 +421,32 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
   if (r0 < rows) {                                     // (else: padding of native scales only)
     const int64_t row = r0 + lr, col = k0 + lc;
     const bool col_in = lc < n_cols;
-    load_gate_or_up(r0, k0, 0, rgt);
-    load_dh(r0, k0);
-    load_gate_or_up(r0, k0, 1, rup);
     // the four blocks' scales of a row of g or u at a time: by the byte, each lane its own, they were as many requests as the codes
     // (4096 x 14336 152 -> 145 us)
-    if (tid < 256) {
-      const int o = tid >> 7, r = tid & 127;
-      uint32_t w = 0;
-      if (r < n_rows) {
-        const uint8_t* const p = a.gus + (r0 + r) * a.gus_ld + (o * F + k0) / 32;
-        if (n_cols == 128 && ((uintptr_t)p & 3) == 0) w = *(const uint32_t*)p;
-        else
-          for (int k = 0; k < n_cols / 32; ++k) w |= (uint32_t)p[k] << (8 * k);
-      }
-      sin[o][r] = w;
+    uint32_t scales = 0;
+    const int so = tid >> 7 & 1, sr = tid & 127;
+    if (tid < 256 && sr < n_rows) {
+      const uint8_t* const p = a.gus + (r0 + sr) * a.gus_ld + (so * F + k0) / 32;
+      if (n_cols == 128 && ((uintptr_t)p & 3) == 0) scales = *(const uint32_t*)p;
+      else
+        for (int k = 0; k < n_cols / 32; ++k) scales |= (uint32_t)p[k] << (8 * k);
     }
-    if constexpr (PLAIN) __builtin_amdgcn_s_waitcnt(0x0F70);   // the wave's share of g and u is in LDS
-    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    load_gate_or_up(r0, k0, 0, rgt);
+    load_gate_or_up(r0, k0, 1, rup);
+    // (what the wait below may leave in flight are the four loads of dh, requested last)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    load_dh(r0, k0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if (tid < 256) sin[so][sr] = scales;
+    if constexpr (PLAIN) {
+      __builtin_amdgcn_s_waitcnt(0x0F70 | 4);          // the wave's share of g and u is in LDS
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // (a fence would wait for dh as well)
+    } else {
+      __syncthreads();
+    }
     if constexpr (PLAIN) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
