@@ -684,8 +684,8 @@ int launch_silu_backward(const SiluBackwardArgs& args, hipStream_t stream) {
   const int64_t rows = native ? (a.rows + 511ll) / 512 * 512 : a.rows, blocks = (rows + 127) / 128 * a.tiles_k;
   if (blocks > 0x7FFFFFFF) return set_error(MX_ERR_SHAPE, "silu_backward: tensor too large");
   const int64_t lim = (int64_t)1 << 31;
-  const bool plain = (((uintptr_t)a.dh | (uintptr_t)(a.dh_ld * 2) | (uintptr_t)a.gu | (uintptr_t)a.gu_ld | (uintptr_t)a.F) & 15) == 0 && a.dh_ld >= a.F && a.gu_ld >= 2 * a.F && a.gus_ld >= a.F / 16 &&
-                     128 * a.dh_ld * 2 < lim && 128 * a.gu_ld < lim && 128 * a.gus_ld < lim && 128 * a.d_ld < lim;
+  const bool plain = (((uintptr_t)a.dh | (uintptr_t)(a.dh_ld * 2) | (uintptr_t)a.gu | (uintptr_t)a.gu_ld) & 15) == 0 &&   // (F % 32 == 0)
+                     a.dh_ld >= a.F && a.gu_ld >= 2 * a.F && a.gus_ld >= a.F / 16 && 128 * a.dh_ld * 2 < lim && 128 * a.gu_ld < lim && 128 * a.gus_ld < lim && 128 * a.d_ld < lim;
   const dim3 grid((unsigned)blocks);
   const bool once = quantize_loads_once((int64_t)a.rows * a.F);
   hipError_t e = hipSuccess;
