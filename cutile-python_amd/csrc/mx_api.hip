@@ -1590,8 +1590,8 @@ namespace mx {
 //   2048 x 7168 1: 7.8 and 10.0; 4096 x 14336 1: 21.4 and 24.1, 32: 24.9 and 27.8; 8192 x 4096 1: 13.2 and 18.8; 8192 x 14336 32: 45.7 and 48.8
 //   rows of W over 8192 bytes:                      16384 x 4096 1: 34.3 and 31.5, 16384 x 7168 16: 50.2 and 43.8 (FP4, 8192 bytes: 25.8 and 29.0)
 //   fewer than 128 workgroups, rows over 4096:      8192 x 2048 1: 11.2 and 10.5, 32: 14.5 and 12.0; 4096 x 2048 32: 9.5 and 10.2
-//   FP4, 17 to 32 rows, K over 4096: X is as long as W's rows are twice over; 8192 x 2048 12.3 and 11.4, 8192 x 7168 14.6 and 18.9, and for
-//   8192 x 14336, where the decode kernel reads plain scales best, 31.3 and 25.7, with packed ones 29.3 and 31.3
+//   FP4, 17 to 32 rows, K over 4096: X is twice as long as W's rows; 8192 x 2048 12.3 and 11.4, 8192 x 7168 14.6 and 18.9, and for
+//   8192 x 14336, where the separate decode kernel reads plain scales best, 31.3 and 25.7, with packed ones 29.3 and 31.3
 static bool stream_gated_wins(const StreamArgs& a, int F) {
   const int64_t row = a.w_fmt == MX_E2M1 ? a.K / 2 : a.K;
   const int blocks = F / 32;
@@ -1599,13 +1599,38 @@ static bool stream_gated_wins(const StreamArgs& a, int F) {
   return a.w_fmt != MX_E2M1 || a.M <= 16 || a.K <= 4096 || (blocks >= 128 && (blocks <= 256 || a.ws_packed));
 }
 
-// A gated product on the streaming kernel (few rows) or on the ping-pong kernel, whose epilogues make of gate and up what is asked
+// The decode kernel with the gate in its epilogue (FP4 weights, plain scales) against the streaming one and through memory.  It reads X
+// once per workgroup, not per unit of 32 columns, but deals whole units, four weight tiles, to 256 workgroups.  us, it and the
+// better of the others (K x F, rows): 4096 x 4096 32: 8.0 and 9.0; 4096 x 14336 32: 14.3 and 16.0, 16: 14.2 and 13.1; 2048 x 7168 32: 7.7 and 7.6;
+// 8192 x 14336 (1.75 units to a workgroup) 32: 24.7 and 25.9, 16: 24.5 and 26.4, 8: 24.4 and 24.3; 8192 x 16384 16: 24.8 and 27.4;
+// 8192 x 28672 32: 43.4 and 45.6; 8192 x 8192 (one unit: half of the time is filling and emptying) 32: 16.8 and 15.5; 8192 x 10240 (1.25) 22.3 and 21.8
+static bool decode_gated_wins(int64_t M, int F, int64_t K) {
+  if (K <= 4096) return M > 16 && K > 2048;
+  const int units = F / 32, rounds = (units + 255) / 256;
+  return M > 8 && rounds >= 2 && rounds * 256 * 4 <= units * 5;
+}
+
+// A gated product on the decode or the streaming kernel (few rows) or on the ping-pong kernel, whose epilogues make of gate and up what is asked
 // for.  kGatedNotFused: it goes through memory instead (nothing enqueued).  W [2 F, K]; the scales as o's layouts say, of W's rows.
 int gemm_gated_fused(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const GateOut& out, const mx_gemm_opts& o,
                      void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   const int64_t M = A.shape[0], K = A.shape[1], N = W.shape[0];
   if (o.block_size != 32 || o.split_k > 1) return kGatedNotFused;
   if (N != 2 * (int64_t)out.F || out.F % 32 != 0 || out.scale_mode != 1 || (out.h_fmt != MX_BF16 && out.h_fmt != MX_E4M3)) return kGatedNotFused;
+  if (M <= 32 && (o.kernel == MX_KERNEL_AUTO || o.kernel == MX_KERNEL_DECODE) && (A.dtype == MX_E4M3 || A.dtype == MX_E5M2) && W.dtype == MX_E2M1 &&
+      W.packed_dim == 1 && As.dtype == MX_E8M0 && Ws.dtype == MX_E8M0 && K > 0 && K % 512 == 0 && K <= kDecodeMaxK && W.shape[1] == K &&
+      o.a_scale_layout == MX_SCALE_2D && o.b_scale_layout == MX_SCALE_2D && A.stride[1] == 1 && W.stride[1] == 1 && As.stride[1] == 1 &&
+      Ws.stride[1] == 1 && N * W.stride[0] < (int64_t)1 << 31 && N * Ws.stride[0] < (int64_t)1 << 31 &&
+      (((uintptr_t)A.ptr | (uintptr_t)As.ptr | (uintptr_t)W.ptr | (uintptr_t)Ws.ptr | (uintptr_t)A.stride[0] | (uintptr_t)As.stride[0] |
+        (uintptr_t)W.stride[0] | (uintptr_t)Ws.stride[0]) % 16) == 0 &&
+      (o.kernel == MX_KERNEL_DECODE || decode_gated_wins(M, out.F, K))) {
+    DecodeArgs d = {};
+    d.X = (const uint8_t*)A.ptr; d.Xs = (const uint8_t*)As.ptr; d.W = (const uint8_t*)W.ptr; d.Ws = (const uint8_t*)Ws.ptr;
+    d.M = (int32_t)M; d.N = (int32_t)N; d.K = (int32_t)K;
+    d.ldx = A.stride[0]; d.ldxs = As.stride[0]; d.ldw = W.stride[0]; d.ldws = Ws.stride[0];
+    d.x_fmt = A.dtype; d.w_fmt = W.dtype; d.c_dtype = MX_BF16;
+    return launch_gemm_decode_gated(d, out, stream);
+  }
   if (M <= kStreamGatedRows && (o.kernel == MX_KERNEL_AUTO || o.kernel == MX_KERNEL_STREAM) && As.dtype == MX_E8M0 && Ws.dtype == MX_E8M0 &&
       W.shape[1] == K && K < (1 << 30) && N < (1 << 30) && A.stride[1] == 1 && W.stride[1] == 1 && (W.dtype != MX_E2M1 || W.packed_dim == 1) &&
       o.a_scale_layout == MX_SCALE_2D && As.ndim == 2 && As.shape[0] == M && As.shape[1] == K / 32 && As.stride[1] == 1 &&

@@ -220,5 +220,6 @@ struct DecodeArgs {
   int32_t x_fmt, w_fmt, c_dtype, accumulate;
 };
 int launch_gemm_decode(const DecodeArgs& d, hipStream_t stream);
+int launch_gemm_decode_gated(const DecodeArgs& d, const GateOut& o, hipStream_t stream);   // N = 2 F, F % 32 == 0
 
 }  // namespace mx

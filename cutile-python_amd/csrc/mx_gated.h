@@ -14,9 +14,20 @@ __device__ __forceinline__ u2 gated_encode(const float (&v)[8], uint32_t& byte) 
   byte = b.byte;
   return (u2){encode4<MX_E4M3>(v[0], v[1], v[2], v[3], b.scale), encode4<MX_E4M3>(v[4], v[5], v[6], v[7], b.scale)};
 }
-// Row `row` (of C, if live), columns col .. col + 7 of gate and up.  (The floor rule, bf16 or E4M3: with the other rule and format
+struct Ungated {};
+
+// Row `row` (of C, if live), columns col .. col + 7 of gate and up (HALVES: col .. col + 3 and col + 16 .. col + 19).  (The floor rule, bf16 or E4M3: with the other rule and format
 // beside them the eight copies of this in a kernel are more than the instruction cache; such calls go through memory.)
+template <bool HALVES = false>
 __device__ __forceinline__ void gated_store(const GateOut& o, const v4f (&acc)[4], int64_t row, int col, bool live, bool scale_lane) {
+  auto put = [](uint8_t* p, const u2& c) {
+    if constexpr (HALVES) {
+      *(uint32_t*)p = c[0];
+      *(uint32_t*)(p + 16) = c[1];
+    } else {
+      *(u2*)p = c;
+    }
+  };
   float g[8], u[8], h[8];
   typedef float f2 __attribute__((ext_vector_type(2)));
   typedef __bf16 b2 __attribute__((ext_vector_type(2)));
@@ -33,13 +44,22 @@ __device__ __forceinline__ void gated_store(const GateOut& o, const v4f (&acc)[4
   for (int e = 0; e < 8; ++e)   // (the hardware's 2^x and reciprocal: a few units in the last place)
     h[e] = g[e] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g[e])) * u[e];
   if (o.h_fmt == MX_BF16) {
-    if (live)
-      store8_full<uint16_t>((uint16_t*)o.h + row * o.h_ld + col, (v4f){h[0], h[1], h[2], h[3]}, (v4f){h[4], h[5], h[6], h[7]});
+    uint16_t* const p = (uint16_t*)o.h + row * o.h_ld + col;
+    if constexpr (HALVES) {
+      if (live)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+          *(b4*)(p + 16 * k) = __builtin_convertvector((v4f){h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]}, b4);
+        }
+    } else if (live) {
+      store8_full<uint16_t>(p, (v4f){h[0], h[1], h[2], h[3]}, (v4f){h[4], h[5], h[6], h[7]});
+    }
   } else {
     uint32_t byte;
     const u2 c = gated_encode(h, byte);
     if (live) {
-      *(u2*)((uint8_t*)o.h + row * o.h_ld + col) = c;
+      put((uint8_t*)o.h + row * o.h_ld + col, c);
       if (scale_lane) o.hs[row * o.hs_ld + col / 32] = (uint8_t)byte;
     }
   }
@@ -48,8 +68,8 @@ __device__ __forceinline__ void gated_store(const GateOut& o, const v4f (&acc)[4
     const u2 cg = gated_encode(g, bg), cu = gated_encode(u, bu);
     if (live) {
       uint8_t* const c = o.c + row * o.c_ld + col;
-      *(u2*)c = cg;
-      *(u2*)(c + o.F) = cu;
+      put(c, cg);
+      put(c + o.F, cu);
       if (scale_lane) {
         uint8_t* const cs = o.cs + row * o.cs_ld + col / 32;
         cs[0] = (uint8_t)bg;

@@ -21,23 +21,19 @@
 // waves all split K and need no barrier while streaming measured 5 - 25 % slower at every K and is gone.)
 #include <stdlib.h>
 
-#include "mx_common.h"
+#include <type_traits>
+
+#include "mx_gated.h"
 #include "mx_load_once.h"
 
 namespace mx {
 namespace {
 
-typedef __attribute__((address_space(3))) uint8_t lds_u8;
-typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) const v4i lds_cv4i;
 typedef __attribute__((address_space(3))) v4f lds_v4f;
 
 constexpr int kWaves = 8;
 constexpr uint32_t kOob = 0x80000000u;         // beyond num_records of the descriptors built here
-
-__device__ inline __amdgpu_buffer_rsrc_t make_rsrc(const void* p, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
-}
 
 // ---- configuration for K-slices of SPW K-steps (K <= 4 * SPW * 128) ------------------------------------------------
 // The two waves of a K-slice multiply the same
@@ -69,6 +65,9 @@ struct DecodeCfg {
   static constexpr int XSCALE_OFF = RING;
   static constexpr int LDS_BYTES = XSTAGE <= SLOT ? RING + 2 * RED : RING + 2 * RED + XSTAGE;
   static_assert(kWaves * 1024 <= 2 * RED, "X scale staging");
+  // gated: sums of a unit's first three tiles, [tile][thread of the first two waves] float4
+  static constexpr int SUMS_OFF = RING + 2 * RED;
+  static constexpr int GATED_LDS_BYTES = LDS_BYTES > SUMS_OFF + 3 * 2048 ? LDS_BYTES : SUMS_OFF + 3 * 2048;
 };
 
 // The weight and scale DMA of one wave for one tile.  Instruction j of the wave covers rows
@@ -111,9 +110,13 @@ __device__ inline void issue_xs_dma(const uint8_t* Xs, uint32_t bytes, lds_u8* d
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)dst, 16, voff, soff, 0, 0);
 }
 
-template <int XF, int SPW, typename OutT, bool ONCE>
-__global__ __launch_bounds__(kWaves * 64) void decode_kernel(const DecodeArgs d) {
+// Gate: Ungated, or GateOut: W's rows are gate and up of a feed-forward block, a unit of 32 columns four tiles in sequence (two of gate
+// rows, two of the up rows F further on), and silu(gate) * up is what leaves.  Sums of three tiles wait in LDS for the fourth, each
+// read by the thread that wrote it.
+template <int XF, int SPW, typename OutT, bool ONCE, class Gate>
+__device__ __forceinline__ void decode_body(const DecodeArgs& d, const Gate& gate) {
   using Cf = DecodeCfg<SPW>;
+  constexpr bool GATED = !std::is_same<Gate, Ungated>::value;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem_generic[];
   lds_u8* const smem = (lds_u8*)smem_generic;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -140,16 +143,20 @@ __global__ __launch_bounds__(kWaves * 64) void decode_kernel(const DecodeArgs d)
   // takes the x-th eighth of every window, so that every XCD reads from all address slices instead of always the
   // same eighth of them (measured 1.1 us of 29 at the 28672 x 8192 weights; two windows of 8-row half tiles, which
   // a pure streaming test prefers, measure 2 us slower here).
-  const int tiles = d.N / 16;
+  const int tiles = GATED ? d.N / 64 : d.N / 16;   // gated: units
   const int G = gridDim.x;
   const int t_first = G % 8 == 0 ? (blockIdx.x % 8) * (G / 8) + blockIdx.x / 8 : blockIdx.x;
-  const int t_count = t_first < tiles ? (tiles - t_first + G - 1) / G : 0;
+  const int t_count = (t_first < tiles ? (tiles - t_first + G - 1) / G : 0) * (GATED ? 4 : 1);
+  auto row_of = [&](int i) {                   // first row of local tile i
+    if constexpr (GATED) return (t_first + (i >> 2) * G) * 32 + (i & 1) * 16 + (i & 2 ? gate.F : 0);
+    else return (t_first + i * G) * 16;
+  };
   auto issue = [&](int i, int slot) {          // this wave's share of local tile i
-    const int tile = t_first + i * G;
+    const int row = row_of(i);
     lds_u8* const base = smem + slot * Cf::SLOT;
     issue_tile_dma2<SPW, ONCE>(d.W, wbytes, d.Ws, sbytes, base + q * (16 * Cf::SLB) + mh * Cf::WIW * 1024,
                          base + Cf::W_BYTES + wave * 1024, row_off, chunk_off, mh * Cf::WIW * Cf::RPI, soff,
-                         tile * 16 * (int)d.ldw, (int)d.ldw, tile * 16 * (int)d.ldws, with_scales, (uint32_t)(d.K / 2));
+                         row * (int)d.ldw, (int)d.ldw, row * (int)d.ldws, with_scales, (uint32_t)(d.K / 2));
   };
 
   if (t_count == 0) return;                    // uniform per workgroup
@@ -238,6 +245,18 @@ __global__ __launch_bounds__(kWaves * 64) void decode_kernel(const DecodeArgs d)
     for (int w = 1; w < 4; ++w) sum += red[(h * 4 + w) * 64 + l];
     // lane (c, g) holds C[16 h + c][16 tile + 4 g + e], e = 0..3
     const int row = 16 * h + (l & 15);
+    if constexpr (GATED) {
+      lds_v4f* const sums = (lds_v4f*)(smem + Cf::SUMS_OFF) + tid;
+      if ((k & 3) < 3) {                       // uniform
+        sums[(k & 3) * 128] = sum;
+        return;
+      }
+      const v4f acc[4] = {sums[0], sums[128], sums[256], sum};
+      saturate_conversions(true);              // (only here: see gemm_pp_gated_kernel)
+      gated_store<true>(gate, acc, row, row_of(k - 3) + 4 * (l >> 4), row < d.M, (l >> 4) == 0);
+      saturate_conversions(false);
+      return;
+    }
     if (row >= d.M) return;
     OutT* c = (OutT*)d.C + (int64_t)row * d.ldc + (t_first + k * G) * 16 + 4 * (l >> 4);
     if constexpr (sizeof(OutT) == 4) {
@@ -311,7 +330,7 @@ __global__ __launch_bounds__(kWaves * 64) void decode_kernel(const DecodeArgs d)
     __builtin_amdgcn_sched_barrier(0);
     if (i + 2 < t_count) issue(i + 2, (i + 1) & 1);
     __builtin_amdgcn_sched_barrier(0);
-    if (i > 0 && wave < 2) reduce_store(i - 1);   // uniform per wave
+    if (!GATED && i > 0 && wave < 2) reduce_store(i - 1);   // uniform per wave
     v4f acc[2] = {(v4f){0.f, 0.f, 0.f, 0.f}, (v4f){0.f, 0.f, 0.f, 0.f}};   // even / odd K-steps: two MFMA chains
     {
 #pragma unroll
@@ -329,9 +348,39 @@ __global__ __launch_bounds__(kWaves * 64) void decode_kernel(const DecodeArgs d)
       }
     }
     ((lds_v4f*)(smem + Cf::RING + (i & 1) * Cf::RED))[wave * 64 + lane] = acc[0] + acc[1];
+    // (gated: here, where the tile's fragments are gone; beside them it spills)
+    if (GATED && i > 0 && wave < 2) reduce_store(i - 1);
   }
   __syncthreads();
   if (wave < 2) reduce_store(t_count - 1);
+}
+
+template <int XF, int SPW, typename OutT, bool ONCE>
+__global__ __launch_bounds__(kWaves * 64) void decode_kernel(const DecodeArgs d) {
+  decode_body<XF, SPW, OutT, ONCE>(d, Ungated{});
+}
+template <int XF, int SPW, bool ONCE>
+__global__ __launch_bounds__(kWaves * 64) void decode_gated_kernel(const DecodeArgs d, const GateOut gate) {
+  decode_body<XF, SPW, uint16_t, ONCE>(d, gate);
+}
+
+template <int XF, int SPW, bool ONCE>
+int launch_decode_gated_k(const DecodeArgs& d, const GateOut& o, int grid, hipStream_t stream) {
+  using Cf = DecodeCfg<SPW>;
+  auto kern = decode_gated_kernel<XF, SPW, ONCE>;
+  static int attr_done = 0;   // (as below)
+  if (!attr_done) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, Cf::GATED_LDS_BYTES);
+    if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "hipFuncSetAttribute(%d bytes LDS): %s", Cf::GATED_LDS_BYTES, hipGetErrorString(e));
+    attr_done = 1;
+  }
+  const hipError_t e = launch_kernel(kern, dim3(grid), dim3(kWaves * 64), Cf::GATED_LDS_BYTES, stream, d, o);
+  if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "decode_gated_kernel launch: %s", hipGetErrorString(e));
+  return MX_OK;
+}
+template <int XF, bool ONCE>
+int launch_decode_gated_x(const DecodeArgs& d, const GateOut& o, int grid, hipStream_t stream) {
+  return d.K > 4096 ? launch_decode_gated_k<XF, 16, ONCE>(d, o, grid, stream) : launch_decode_gated_k<XF, 8, ONCE>(d, o, grid, stream);
 }
 
 template <int XF, int SPW, typename OutT, bool ONCE>
@@ -361,8 +410,7 @@ int launch_decode_x(const DecodeArgs& d, int grid, hipStream_t stream) {
 
 }  // namespace
 
-
-int launch_gemm_decode(const DecodeArgs& d, hipStream_t stream) {
+static int check_decode(const DecodeArgs& d) {
   if (d.w_fmt != MX_E2M1) return set_error(MX_ERR_DTYPE, "decode kernel: weights must be MX_E2M1");
   if (d.x_fmt != MX_E4M3 && d.x_fmt != MX_E5M2) return set_error(MX_ERR_DTYPE, "decode kernel: activations must be 8-bit");
   if (d.M < 1 || d.M > 32) return set_error(MX_ERR_SHAPE, "decode kernel: M must be in 1..32");
@@ -374,6 +422,20 @@ int launch_gemm_decode(const DecodeArgs& d, hipStream_t stream) {
     return set_error(MX_ERR_LAYOUT, "decode kernel: operands, scales and their row pitches must be 16-byte aligned");
   if ((int64_t)d.N * d.ldw >= ((int64_t)1 << 31) || (int64_t)d.N * d.ldws >= ((int64_t)1 << 31))
     return set_error(MX_ERR_LAYOUT, "decode kernel: W spans 2 GiB or more");
+  return MX_OK;
+}
+
+int launch_gemm_decode_gated(const DecodeArgs& d, const GateOut& o, hipStream_t stream) {
+  if (const int rc = check_decode(d)) return rc;
+  if (d.N != 2 * (int64_t)o.F || o.F % 32 != 0) return set_error(MX_ERR_SHAPE, "gated decode kernel: N must be 2 F, F a multiple of 32");
+  const int units = o.F / 32, grid = units < 256 ? units : 256;
+  if (weights_load_once(d.N, d.K / 2, d.ldw))
+    return d.x_fmt == MX_E4M3 ? launch_decode_gated_x<MX_E4M3, true>(d, o, grid, stream) : launch_decode_gated_x<MX_E5M2, true>(d, o, grid, stream);
+  return d.x_fmt == MX_E4M3 ? launch_decode_gated_x<MX_E4M3, false>(d, o, grid, stream) : launch_decode_gated_x<MX_E5M2, false>(d, o, grid, stream);
+}
+
+int launch_gemm_decode(const DecodeArgs& d, hipStream_t stream) {
+  if (const int rc = check_decode(d)) return rc;
   if (d.c_dtype != MX_F32 && d.c_dtype != MX_BF16) return set_error(MX_ERR_DTYPE, "decode kernel: bad output dtype");
   const int tiles = d.N / 16;
   const int grid = tiles < 256 ? tiles : 256;

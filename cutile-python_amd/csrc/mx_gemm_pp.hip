@@ -48,7 +48,6 @@ namespace {
 // hold the 32 columns of an MX block.  The epilogue is some 1200 vector instructions a wave and tile, which stand in the
 // memory phase; the other team has but one MFMA phase to put beside them.  8192 x 28672 x 4096 MXFP8, bf16 out: 678 us (2.84 PFLOP/s),
 // where a bf16 product and a pass over it take 831; 1531 rows, E4M3 out: 139 against 159 (with the scales re-laid 150 against 168).
-struct Ungated {};
 // KTAIL: K is not a whole number of stages (or there is a single stage): the 16-byte chunks beyond the end of K are
 // masked lane by lane at issue time.  Without it the loads take their precomputed offsets as they are, which keeps a
 // compare and a select per DMA instruction out of the memory phase.

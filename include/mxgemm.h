@@ -355,8 +355,8 @@ MX_API int mx_quantize_both(const mx_tensor* x, mx_tensor* xq, mx_tensor* scale,
  *   E4M3 out) by the hardware's 2^x and reciprocal, a few units in the last place from mx_silu_mul_quantize's
  *   gate_up [M,2F] MX_E4M3 with gate_up_scale [M,2F/32], optional (both NULL): [G|U] quantised, which is what
  *   mx_silu_mul_backward_quantize takes (8.25 bits an element from the forward to the backward pass)
- * Kernels: opts->kernel MX_KERNEL_STREAM (M <= 32) or MX_KERNEL_MFMA_PINGPONG do all in one launch where they can, any
- * other the product into the workspace and a pass over it; MX_KERNEL_AUTO takes what is faster.
+ * Kernels: opts->kernel MX_KERNEL_STREAM, MX_KERNEL_DECODE (M <= 32) and MX_KERNEL_MFMA_PINGPONG do all in one launch where
+ * they can, any other the product into the workspace and a pass over it; MX_KERNEL_AUTO takes what is faster.
  * Workspace: mx_gated_gemm_workspace_bytes(), which holds every form; it is asked for whichever is taken.
  */
 MX_API int64_t mx_gated_gemm_workspace_bytes(int64_t M, int64_t F, int64_t K, const mx_gemm_opts* opts);

@@ -106,9 +106,44 @@ def test_gated_product_streamed_nan(ct, dev):
     assert bool(cq[:, [70, F + 131]].float().isnan().all())
 
 
+@pytest.mark.parametrize("a_fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("M,K,F", [(1, 512, 32), (5, 1024, 96), (17, 4096, 224), (32, 8192, 512), (16, 4608, 64), (20, 5120, 9216)])
+def test_gated_product_decode(ct, dev, M, K, F, a_fmt):
+    """The decode kernel: one and both halves of its rows, both lengths of a K slice, fewer units of 32 columns than workgroups and more."""
+    a, w = randn_operand(M, K, O.E4M3 if a_fmt == "e4m3" else O.E5M2, M + K, dev), randn_operand(2 * F, K, O.E2M1, F, dev, std=K ** -0.5)
+    gu = R.bf16(O.dequantize(a.codes, a.scales, a.fmt).double() @ O.dequantize(w.codes, w.scales, w.fmt).double().T)
+    kw = dict(a_format=a.fmt_kw, w_format="e2m1", kernel="decode")
+    h, cq, cs = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, checkpoint=True, **kw)
+    q, s, cq2, cs2 = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, out_dtype="e4m3", checkpoint=True, **kw)
+    assert R.rel(h, R.silu_mul(gu)) <= R.HALF_BF16 + 2 * BF16_FLIPS
+    assert R.rel(R.value(q, s), R.rows(R.silu_mul(gu))) <= 2 * E4M3_FLIPS
+    assert R.rel(R.value(cq, cs), R.rows(gu)) <= 2 * E4M3_FLIPS
+    assert torch.equal(u8(cq2), u8(cq)) and torch.equal(u8(cs2), u8(cs))
+
+
+def test_gated_product_decode_nan(ct, dev):
+    """NaN elements and scales reach their rows and columns, in a workgroup's first unit and in its second, and nothing else."""
+    M, K, F = 20, 1024, 9216                           # 288 units for 256 workgroups
+    a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(2 * F, K, O.E2M1, 2, dev, std=K ** -0.5)
+    kw = dict(w_format="e2m1", kernel="decode", checkpoint=True)
+    want, wcq, _ = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, **kw)
+    u8(a.storage)[4, 1000] = 0x7F
+    u8(a.scale_t)[18, 3] = 0xFF
+    bad = [5, 70, 8200, 9215]
+    for n, j in enumerate(bad):
+        u8(w.scale_t)[j + F * (n % 2), 7 * n] = 0xFF   # gate rows and up rows
+    h, cq, cs = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, **kw)
+    rows, cols = [i for i in range(M) if i not in (4, 18)], [j for j in range(F) if j not in bad]
+    assert bool(h[[4, 18]].isnan().all()) and bool(h[:, bad].isnan().all()) and bool(cq[[4, 18]].float().isnan().all())
+    assert torch.equal(h[rows][:, cols], want[rows][:, cols]) and not bool(h[rows][:, cols].isnan().any())
+    clean = [j for j in range(2 * F) if j % F // 32 not in [b // 32 for b in bad]]
+    assert torch.equal(u8(cq)[rows][:, clean], u8(wcq)[rows][:, clean])
+
+
 def test_gated_product_is_chosen_by_size(ct, dev):
     """Where the streaming kernel is taken by default, its bits; explicit kernels and the others agree to their bounds."""
-    for M, K, F, w_fmt in ((1, 2048, 4096, O.E4M3), (32, 8192, 2048, O.E4M3), (32, 8192, 1024, O.E2M1), (33, 1024, 512, O.E4M3)):
+    for M, K, F, w_fmt in ((1, 2048, 4096, O.E4M3), (32, 8192, 2048, O.E4M3), (32, 8192, 1024, O.E2M1), (33, 1024, 512, O.E4M3),
+                          (24, 4096, 512, O.E2M1), (12, 4608, 16384, O.E2M1)):
         a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(2 * F, K, w_fmt, 2, dev, std=K ** -0.5)
         got = ct.gated_block_scaled_matmul(a.storage, a.scale_t, w.storage, w.scale_t, w_format=w.fmt_kw)
         for kernel in ("stream", "pingpong", "mfma128"):
