@@ -129,7 +129,8 @@ def gated_block_scaled_matmul(A: torch.Tensor, A_scale, W: torch.Tensor, W_scale
 
     A (M, K) and W (2F, K), gate rows first, hold MX elements as in :func:`block_scaled_matmul` (FP4 packed along K,
     ``"e2m1"`` formats for uint8 storage); A_scale (M, K/32) and W_scale (2F, K/32) are E8M0 tensors or :class:`PackedScales`
-    (operand "a" / "b"); F is a multiple of 32.  From one row (weights streamed) to many.
+    (operand "a" / "b"); F is a multiple of 32.  From one row (weights streamed) to many; of the kernels "stream", "decode" (up
+    to 32 rows) and "pingpong" finish the result in the launch of the product where they can, and "auto" takes what is fastest.
 
     Returns (M, F) in ``torch.bfloat16``, or with ``out_dtype`` an 8-bit format ``(h_q, h_scale)``, ready for the down
     projection.  With ``checkpoint`` also ``(gate_up_q, gate_up_scale)``, [G | U] in MXFP8 E4M3, which is all that
