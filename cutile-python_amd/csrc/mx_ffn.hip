@@ -98,8 +98,15 @@ int run_gated(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const
 struct FfnShape {
   int64_t T, H, F, Ho, Tp;
 };
+// Few tokens: gate and up, and the activation's gradient, are summed in 32-bit precision (mx_gemm_few.hip).  Where a result differs from its
+// definition by more than its own rounding it is by single large elements that took the other neighbour, and the fewer elements the more
+// they weigh.  The largest difference of y, dx, dw1 or dw2 in 12 draws, of its norm (rounding to bf16 alone: 0.0017), without that, T x F: 17 x 512
+// 0.0097, 33 x 512 0.0068, 64 x 512 0.0051, 100 x 512 0.0044, 40 x 2048 0.0037, 300 x 512 0.0034, 200 x 1024 0.0028, 1000 x 512 0.0026; with it 0.0018.
+// us a step, without and with it: 1 and 64 tokens, H x F 4096 x 14336 328 | 349, 389 | 423; 1024 x 2048 49 | 50, 65 | 63; 4096 x 1024
+// 57 | 61, 70 | 71; 73 x 4096 x 7168 211 | 224; 256 x 4096 x 512 78 | 72; 512 x 4096 x 1024 96 | 99; 1024 x 1024 x 512 66 | 69.
+inline bool few_tokens(const FfnShape& s) { return s.T <= 64 || s.T * s.F <= 524288; }
 // scales of an operand whose rows go with the tokens: few rows are multiplied by kernels that read them plain
-inline bool native_rows(int64_t T) { return T > 64; }
+inline bool native_rows(const FfnShape& s) { return !few_tokens(s); }
 inline int64_t scale_bytes(int64_t rows, int64_t K, bool native) { return native ? mx_packed_scale_bytes(rows, K) : rows * (K / 32); }
 
 // what the forward pass leaves for the backward pass
@@ -134,7 +141,7 @@ struct FfnForward {
 FfnForward ffn_forward(uint8_t* base, const FfnShape& s) {
   Deal d = {base};
   FfnForward r;
-  const bool nat = native_rows(s.T);
+  const bool nat = native_rows(s);
   r.xq = d.take(s.T * s.H);
   r.xs = d.take(scale_bytes(s.T, s.H, nat));
   r.w1 = d.take(2 * s.F * s.H);
@@ -158,7 +165,7 @@ struct FfnBackward {
 FfnBackward ffn_backward(uint8_t* base, const FfnShape& s) {
   Deal d = {base};
   FfnBackward r;
-  const bool nat = native_rows(s.T), act = s.F % 64 == 0;   // (launch_silu_backward)
+  const bool nat = native_rows(s), act = s.F % 64 == 0;   // (launch_silu_backward)
   r.native_rows = nat;
   r.native_act = act;
   r.dy = d.take(s.T * s.Ho);
@@ -369,7 +376,7 @@ int mx_ffn_forward(const mx_tensor* x, const mx_tensor* w1, const mx_tensor* w2,
     if (int rc = check_room("saved", saved, saved_bytes, k.bytes)) return rc;
   }
   hipStream_t st = (hipStream_t)stream;
-  const bool nat = native_rows(s.T);
+  const bool nat = native_rows(s);
   const BothTensor list[3] = {both(x, f.xq, f.xs, nat ? kScaleNativeA : kScalePlain, k.xt, k.xts, kScaleNativeB),
                               both(w1, f.w1, f.w1s, kScaleNativeB, k.w1t, k.w1ts, kScaleNativeB),
                               both(w2, f.w2, f.w2s, kScaleNativeB, k.w2t, k.w2ts, kScaleNativeB)};
@@ -379,10 +386,19 @@ int mx_ffn_forward(const mx_tensor* x, const mx_tensor* w1, const mx_tensor* w2,
   g.c = k.gu; g.c_ld = 2 * s.F; g.cs = k.gus; g.cs_ld = 2 * s.F / 32;
   g.F = (int32_t)s.F; g.scale_mode = scale_mode;
   const mx_gemm_opts up = layouts(nat, true), down = layouts(false, true);
-  if (int rc = run_gated(tensor2d(f.xq, MX_E4M3, s.T, s.H, s.H), tensor2d(f.xs, MX_E8M0, s.T, s.H / 32, s.H / 32),
-                         tensor2d(f.w1, MX_E4M3, 2 * s.F, s.H, s.H), tensor2d(f.w1s, MX_E8M0, 2 * s.F, s.H / 32, s.H / 32), g, up, f.work,
-                         f.work_bytes, st))
+  if (few_tokens(s)) {
+    FewArgs few = {f.xq, f.xs, f.w1, f.w1s, (uint16_t*)f.work, (int32_t)s.T, (int32_t)(2 * s.F), (int32_t)s.H};
+    if (scale_mode) {
+      if (int rc = launch_gemm_few_gated(few, g, st)) return rc;
+    } else {
+      if (int rc = launch_gemm_few(few, st)) return rc;
+      if (int rc = launch_gate_up(GateUpArgs{(const uint16_t*)f.work, 2 * s.F, s.T, g}, st)) return rc;
+    }
+  } else if (int rc = run_gated(tensor2d(f.xq, MX_E4M3, s.T, s.H, s.H), tensor2d(f.xs, MX_E8M0, s.T, s.H / 32, s.H / 32),
+                                tensor2d(f.w1, MX_E4M3, 2 * s.F, s.H, s.H), tensor2d(f.w1s, MX_E8M0, 2 * s.F, s.H / 32, s.H / 32), g, up, f.work,
+                                f.work_bytes, st)) {
     return rc;
+  }
   return product(f.h, f.hs, f.w2, f.w2s, *y, s.T, s.Ho, s.F, down, f.work, f.work_bytes, stream);
 }
 
@@ -413,7 +429,11 @@ int mx_ffn_backward(const mx_tensor* dy, const void* saved, int64_t saved_bytes,
   const BothTensor t = both(dy, b.dy, b.dys, b.native_rows ? kScaleNativeA : kScalePlain, dw2 ? b.dyt : nullptr, b.dyts, kScaleNativeA);
   if (int rc = launch_quantize_both(&t, 1, MX_E4M3, scale_mode, st)) return rc;
   const mx_tensor dh = tensor2d(b.dh, MX_BF16, s.T, s.F, s.F);
-  if (int rc = product(b.dy, b.dys, k.w2t, k.w2ts, dh, s.T, s.F, s.Ho, b.o_dh, b.work, b.work_bytes, stream)) return rc;
+  if (few_tokens(s)) {
+    if (int rc = launch_gemm_few(FewArgs{b.dy, b.dys, k.w2t, k.w2ts, (uint16_t*)b.dh, (int32_t)s.T, (int32_t)s.F, (int32_t)s.Ho}, st)) return rc;
+  } else if (int rc = product(b.dy, b.dys, k.w2t, k.w2ts, dh, s.T, s.F, s.Ho, b.o_dh, b.work, b.work_bytes, stream)) {
+    return rc;
+  }
   SiluBackwardArgs a = {};
   a.dh = (const uint16_t*)b.dh; a.dh_ld = s.F;
   a.gu = k.gu; a.gu_ld = 2 * s.F; a.gus = k.gus; a.gus_ld = 2 * s.F / 32;

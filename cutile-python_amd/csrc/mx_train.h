@@ -34,6 +34,15 @@ struct GateUpArgs {
 };
 int launch_gate_up(const GateUpArgs& a, hipStream_t stream);
 
+// E4M3 products of few rows in 32-bit precision (mx_gemm_few.hip): rows without gaps, X's scales plain, W's native (operand B)
+struct FewArgs {
+  const uint8_t *X, *Xs, *W, *Ws;
+  uint16_t* C;                       // bf16 [M, N]; gated: not used
+  int32_t M, N, K;                   // N and K multiples of 32
+};
+int launch_gemm_few(const FewArgs& a, hipStream_t stream);
+int launch_gemm_few_gated(const FewArgs& a, const GateOut& o, hipStream_t stream);   // N = 2 F; the floor rule, E4M3 out
+
 // dh and the checkpoint [g|u] -> d[g|u] quantised along rows and columns, silu(g) * u along columns (all E4M3)
 struct SiluBackwardArgs {
   const uint16_t* dh;                // bf16

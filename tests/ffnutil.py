@@ -68,13 +68,14 @@ def silu_mul_backward(dh, gu):
     return torch.cat((dh * u * s * (1 + g * (1 - s)), dh * g * s), -1), g * s * u
 
 
-def block(x, w1, w2, dy):
-    """y, dx, dw1, dw2 of the block with every quantisation and bf16 rounding that belongs to its definition."""
-    gu = bf16(rows(x) @ rows(w1).T)
-    y = rows(silu_mul(gu)) @ rows(w2).T
-    dh = bf16(rows(dy) @ columns(w2).T)
-    d, a = silu_mul_backward(dh, rows(gu))
-    return y, rows(d) @ columns(w1).T, columns(d) @ columns(x).T, columns(dy) @ columns(a).T
+def block(x, w1, w2, dy, *how):
+    """y, dx, dw1, dw2 of the block with every quantisation (`how`: format, rule) and bf16 rounding that belongs to its definition."""
+    gu = bf16(rows(x, *how) @ rows(w1, *how).T)
+    y = rows(silu_mul(gu), *how) @ rows(w2, *how).T
+    dh = bf16(rows(dy, *how) @ columns(w2, *how).T)
+    d, a = silu_mul_backward(dh, rows(gu, *how))
+    return (y, rows(d, *how) @ columns(w1, *how).T, columns(d, *how) @ columns(x, *how).T,
+            columns(dy, *how) @ columns(a, *how).T)
 
 
 def block_unquantized(x, w1, w2):

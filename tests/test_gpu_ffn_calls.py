@@ -191,6 +191,50 @@ def test_one_tensor_for_several_arguments(ct, dev):
     assert torch.equal(g, dx + dw1)
 
 
+# Few tokens: gate, up and dh are sums in 32 bits, off by 2^-22 of a norm at most; the shares of their elements that flip at a rounding to bf16 and on
+# to E4M3 follow as in test_gpu_ffn.py, on three operands of a path, two flips each.  The last product is the scaled MFMA's (2^-14).
+FEW = 3 * 2 * (2.0 ** -22 * 2.0 ** -3) ** 0.5 + 2.0 ** -14
+
+
+@pytest.mark.parametrize("mode", ["floor", "ceil"])
+@pytest.mark.parametrize("T,H,F,Ho", [(1, 1024, 2048, 1024), (1, 32, 32, 32), (2, 160, 96, 64), (16, 2080, 224, 96), (17, 1024, 512, 1024), (32, 96, 1056, 4128),
+                                      (33, 1024, 512, 256), (64, 544, 1504, 320), (65, 512, 512, 512), (100, 1024, 544, 1024), (513, 288, 992, 96)])
+def test_few_tokens_are_exact(ct, dev, T, H, F, Ho, mode):
+    """Every result of a step with few tokens is its definition's, but for the few elements that lie that close to a border."""
+    x, w1, w2, dy = make(T, H, F, Ho, T + F, dev, torch.float32)
+    y, st = ct.gated_feed_forward_forward(x, w1, w2, scale_mode=mode)
+    got = (y, *ct.gated_feed_forward_backward(dy, st))
+    for g, w in zip(got, R.block(*(t.cpu().double() for t in (x, w1, w2, dy)), "e4m3", mode)):
+        assert R.rel(g, w) <= FEW + 2.0 ** -24
+
+
+def test_few_tokens_powers_of_two(ct, dev):
+    """Scales far from one: the input up and the weight down by 2^60 give the same bits, a gradient of 2^-100 bits scaled by it."""
+    x, w1, w2, dy = make(9, 288, 160, 96, 11, dev, torch.float32)
+    y, st = ct.gated_feed_forward_forward(x, w1, w2)
+    dx, dw1, dw2 = ct.gated_feed_forward_backward(dy, st)
+    y2, st2 = ct.gated_feed_forward_forward(x * 2.0 ** 60, w1 * 2.0 ** -60, w2)
+    dx2, dw12, dw22 = ct.gated_feed_forward_backward(dy * 2.0 ** -40, st2)
+    assert torch.equal(y, y2) and torch.equal(dx2, dx * 2.0 ** -100) and torch.equal(dw12, dw1 * 2.0 ** 20) and torch.equal(dw22, dw2 * 2.0 ** -40)
+
+
+def test_few_tokens_nan(ct, dev):
+    """A NaN in a token reaches its row of y and dx; one in a weight what is multiplied by it."""
+    x, w1, w2, dy = make(20, 128, 96, 64, 12, dev, torch.float32)
+    y, st = ct.gated_feed_forward_forward(x, w1, w2)
+    dx = ct.gated_feed_forward_backward(dy, st)[0]
+    bad = x.clone()
+    bad[7, 100] = float("nan")
+    y2, st2 = ct.gated_feed_forward_forward(bad, w1, w2)
+    dx2, dw1, _ = ct.gated_feed_forward_backward(dy, st2)
+    keep = [i for i in range(20) if i != 7]
+    assert bool(y2[7].isnan().all()) and bool(dx2[7].isnan().all()) and torch.equal(y2[keep], y[keep]) and torch.equal(dx2[keep], dx[keep])
+    assert bool(dw1.isnan().any())
+    worse = w1.clone()
+    worse[3, 5] = float("nan")
+    assert bool(ct.gated_feed_forward_forward(x, worse, w2)[0].isnan().all())
+
+
 @pytest.mark.parametrize("T", [31, 32, 33, 63, 64, 65, 480, 512, 513])
 def test_a_padded_batch(ct, dev, T):
     """Tokens of zeros behind a batch, and a gradient of zeros for them, change no result of the others and no weight's gradient."""
