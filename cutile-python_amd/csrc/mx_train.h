@@ -16,7 +16,7 @@ struct BothTensor {
   int32_t rows, K, x_dtype;
   int32_t s_kind, st_kind;           // kScale*
   // filled in by the launcher
-  int32_t first, tiles, tiles_k, once;
+  int32_t first, tiles, tiles_k, once, near;
 };
 constexpr int kBothMax = 3;
 struct BothArgs {

@@ -68,7 +68,7 @@ __device__ __forceinline__ void store_scales(const uint32_t* lds, uint8_t* s, in
 // PLAIN: aligned rows of whole blocks that do not overlap, tiles of less than 2 GiB.  Loads and stores then go through buffer
 // descriptors of the tile, whose range takes the place of every comparison with the matrix's ends, and magnitudes of 16-bit input
 // are compared two at a time as they lie in memory.  The vector ALUs are what the rest of the time is spent on otherwise: with
-// the comparisons, 64-bit addresses and the scale rule decided per block 8192 x 8192 bf16 took 56 us, now 50 (5.4 TB/s); a copy of
+// the comparisons, 64-bit addresses and the scale rule decided per block 8192 x 8192 bf16 took 56 us, now 48 (5.6 TB/s); a copy of
 // 2 GiB reaches 5.1 TB/s, where what was just written is in no cache, and this kernel 4.4 of 32768 x 14336.
 template <int SRC>
 __device__ __forceinline__ float load_one(const void* x, int64_t at) {
@@ -105,7 +105,8 @@ __global__ __launch_bounds__(256) void quantize_both_kernel(const BothArgs a) {
   const BothTensor t = a.t[which];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rg = lane >> 4, cg = lane & 15;
   uint32_t tr, tk;
-  tile_of<1, false>(blockIdx.x - t.first, t.tiles, t.tiles_k, tr, tk);
+  if (t.near) tile_of<2, true>(blockIdx.x - t.first, t.tiles, t.tiles_k, tr, tk);
+  else tile_of<1, false>(blockIdx.x - t.first, t.tiles, t.tiles_k, tr, tk);
   const int64_t r0 = (int64_t)tr * 128, k0 = (int64_t)tk * 128;
   const int64_t rows = t.rows, K = t.K, Kpad = (K + 31) / 32 * 32, Rpad = (rows + 31) / 32 * 32;
   uint8_t* const srow_b = (uint8_t*)srow;
@@ -640,6 +641,10 @@ int launch_quantize_both(const BothTensor* list, int n, int fmt, int scale_mode,
       if (blocks > 0x7FFFFFFF) return set_error(MX_ERR_SHAPE, "quantize_both: tensor too large");
       t.tiles = (int32_t)tiles;
       t.once = quantize_loads_once((int64_t)t.rows * t.K);
+      // An XCD takes neighbouring tiles, by two rows of tiles, so that lines of scales meet in its L2.  us, row by row over all XCDs and so: bf16
+      // 4096 x 14336 46.4 | 43.6, 8192 x 8192 50.2 | 48.7, 28672 x 4096 97 | 94, 16384 x 8192 123 | 109, 16384 x 14336 221 | 199;
+      // fp32 4096 x 4096 20.7 | 19.4, 8192 x 8192 76 | 78; but 32768 x 14336 437 | 469, 32768 x 14464 428 | 501 (32896 x 14336 502 | 443)
+      t.near = (int64_t)t.rows * t.K < (int64_t)1 << 28;
       a.t[a.n++] = t;
     }
     if (blocks == 0) continue;
