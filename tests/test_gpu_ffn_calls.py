@@ -9,7 +9,7 @@ import ffnutil as R
 from cutile_amd import _lib as L
 from mxutil import randn_operand
 from oracle import mx_oracle as O
-from test_gpu_ffn import BF16_FLIPS, make, u8
+from test_gpu_ffn import BF16_FLIPS, BLOCK, make, u8
 
 pytestmark = pytest.mark.gpu
 
@@ -248,3 +248,42 @@ def test_a_padded_batch(ct, dev, T):
     # (other kernels may be chosen: elements that lie at a rounding's border)
     for a, b in ((py[:T], y), (got[0][:T], want[0]), (got[1], want[1]), (got[2], want[2])):
         assert R.rel(a, b.cpu().double()) <= R.HALF_BF16 + 8 * (2.0 ** -14 * 2.0 ** -3) ** 0.5
+
+
+@pytest.mark.parametrize("mode", ["floor", "ceil"])
+@pytest.mark.parametrize("T,H,F,Ho", [(70, 256, 8224, 64), (600, 160, 992, 96), (1100, 544, 1056, 288), (1531, 256, 416, 128), (2100, 96, 320, 64),
+                                      (520, 1024, 1088, 544), (129, 512, 4160, 256)])
+def test_block_beyond_few_tokens(ct, dev, T, H, F, Ho, mode):
+    """More than 2^19 elements of the activation: F of odd and even multiples of 32, tokens of no and of whole groups of 64 and 512."""
+    assert T > 64 and T * F > 2 ** 19
+    x, w1, w2, dy = make(T, H, F, Ho, T + F, dev, torch.float32)
+    y, st = ct.gated_feed_forward_forward(x, w1, w2, scale_mode=mode)
+    got = (y, *ct.gated_feed_forward_backward(dy, st))
+    for g, w in zip(got, R.block(*(t.cpu().double() for t in (x, w1, w2, dy)), "e4m3", mode)):
+        assert R.rel(g, w) <= 2.0 ** -24 + BLOCK
+    for g, w in zip(ct.gated_feed_forward_backward(dy, st, need_dx=False), (None, *got[2:])):
+        assert g is None if w is None else torch.equal(g, w)
+
+
+@pytest.mark.parametrize("T,H,F,Ho", [(1100, 256, 1056, 128), (1100, 256, 1024, 128)])
+def test_block_beyond_few_tokens_in_graphs(ct, dev, T, H, F, Ho):
+    x, w1, w2, dy = make(T, H, F, Ho, 5, dev)
+    sx, sdy = x.clone(), dy.clone()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            gy, gst = ct.gated_feed_forward_forward(sx, w1, w2)
+            gd = ct.gated_feed_forward_backward(sdy, gst)
+        graphs.append((g, (gy, *gd)))
+    for k in range(4):
+        nx, _, _, ndy = make(T, H, F, Ho, 30 + k, dev)
+        sx.copy_(nx)
+        sdy.copy_(ndy)
+        ey, est = ct.gated_feed_forward_forward(nx, w1, w2)
+        eager = (ey, *ct.gated_feed_forward_backward(ndy, est))
+        for g, out in graphs:
+            g.replay()
+            again = ct.gated_feed_forward_backward(ndy, est)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, eager)) and all(torch.equal(a, b) for a, b in zip(again, eager[1:]))
