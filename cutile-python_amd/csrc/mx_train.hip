@@ -349,12 +349,14 @@ __global__ __launch_bounds__(256) void gate_up_kernel(const GateUpArgs a) {
 // numbers that stay in registers until their rows' and columns' maxima are known, beside g s, which the second and the third are
 // made of.  4096 x 14336: 109 us where every call writes the same memory, 123 (4.4 TB/s) where it is another; a copy of 2 GiB reaches
 // 5.1 TB/s, and the difference goes into eight streams of one line a row each.
-// g -> g s and s (1 + g (1 - s)) = s + g s - g s s; exp through the hardware's 2^x and a reciprocal: a few units in the last
-// place, against the 2^-4 of what follows
+// g -> g s and s (1 + g (1 - s)) = s + g s (1 - s); exp through the hardware's 2^x and a reciprocal: within 2^-18 of the value, of the terms where
+// they cancel (g near -1.28), against the 2^-4 of what follows.  1 - s, not s + g s - g s s: that is 1 + g - g for a large g, 0 in place of 1
+// from 2^24 on.  s is 0 or 1 far out, and g ends at numbers that such an s multiplies without a NaN (-126, below which s is 0; the largest float for
+// a code and scale beyond it); a NaN comes back through s.
 __device__ __forceinline__ void silu_slope(float g, float& gs, float& slope) {
   const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
-  gs = g * s;
-  slope = __builtin_fmaf(-gs, s, s + gs);
+  gs = __builtin_amdgcn_fmed3f(g, -126.0f, 3.4028234664e38f) * s;
+  slope = __builtin_fmaf(gs, 1.0f - s, s);
 }
 
 // Loads and stores through descriptors of the tile, as in quantize_both_kernel (the launcher's rule; PLAIN false: any pitch).

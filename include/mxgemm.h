@@ -371,7 +371,8 @@ MX_API int mx_gated_gemm(const mx_tensor* A, const mx_tensor* A_scale, const mx_
  *   d  [rows,2F], d_scale:  [dg|du] quantised along the rows, for dx = d @ w1
  *   dt [2F,Rpad], dt_scale: its transposed form quantised along the tokens, for dw1 = d.T @ x
  *   at [F,Rpad],  at_scale: the activation, recomputed and quantised along the tokens, for dw2 = dy.T @ a
- * all MX_E4M3, layouts as in mx_quantize_both.
+ * all MX_E4M3, layouts as in mx_quantize_both.  In 32 bits: within 2^-18 of the value before it is quantised, or of the terms of
+ * 1 + g (1 - s) where they cancel, for any gate; sigmoids below 2^-126 are zero, and a gate beyond the largest float counts as that.
  */
 MX_API int mx_silu_mul_backward_quantize(const mx_tensor* dh, const mx_tensor* gate_up, const mx_tensor* gate_up_scale,
                                   mx_tensor* d, mx_tensor* d_scale, mx_tensor* dt, mx_tensor* dt_scale, mx_tensor* at,
