@@ -204,8 +204,8 @@ int product(uint8_t* a, uint8_t* as, uint8_t* b, uint8_t* bs, const mx_tensor& C
 }
 BothTensor both(const mx_tensor* x, uint8_t* q, uint8_t* s, int s_kind, uint8_t* qt, uint8_t* st, int st_kind) {
   BothTensor t = {};
-  t.x = x->ptr; t.x_ld = x->stride[0]; t.x_dtype = x->dtype;
   t.rows = (int32_t)x->shape[0]; t.K = (int32_t)x->shape[1];
+  t.x = x->ptr; t.x_ld = t.rows > 1 ? x->stride[0] : t.K; t.x_dtype = x->dtype;   // (the pitch of one row is anything)
   const int64_t Kp = round32(t.K), Rp = round32(t.rows);
   t.q = q; t.s = s; t.q_ld = Kp; t.s_ld = Kp / 32; t.s_kind = s_kind;
   t.qt = qt; t.st = st; t.qt_ld = Rp; t.st_ld = Rp / 32; t.st_kind = st_kind;
@@ -251,7 +251,8 @@ int mx_quantize_both(const mx_tensor* x, mx_tensor* xq, mx_tensor* scale, mx_ten
     return set_error(MX_ERR_DTYPE, "xq and xt must both be MX_E4M3 or both MX_E5M2 (got %d, %d)", xq->dtype, xt->dtype);
   if (int rc = check_mode(scale_mode)) return rc;
   BothTensor t = both(x, (uint8_t*)xq->ptr, (uint8_t*)scale->ptr, kScalePlain, (uint8_t*)xt->ptr, (uint8_t*)scale_t->ptr, kScalePlain);
-  t.q_ld = xq->stride[0]; t.s_ld = scale->stride[0]; t.qt_ld = xt->stride[0]; t.st_ld = scale_t->stride[0];
+  t.s_ld = scale->stride[0]; t.qt_ld = xt->stride[0]; t.st_ld = scale_t->stride[0];
+  if (rows > 1) t.q_ld = xq->stride[0];   // (the kernel tells rows that are not there by their offsets: no row may lie within the first)
   return launch_quantize_both(&t, 1, xq->dtype, scale_mode, (hipStream_t)stream);
 }
 
