@@ -257,7 +257,7 @@ int mx_quantize_both(const mx_tensor* x, mx_tensor* xq, mx_tensor* scale, mx_ten
 }
 
 int64_t mx_gated_gemm_workspace_bytes(int64_t M, int64_t F, int64_t K, const mx_gemm_opts* opts) {
-  if (M <= 0 || F <= 0 || K <= 0) return 0;
+  if (M <= 0 || F <= 0 || K < 0) return 0;   // (an empty sum is a result too, by way of memory)
   return gated_workspace(M, F, K, opts ? *opts : kPlainOpts);
 }
 
