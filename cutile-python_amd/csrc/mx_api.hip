@@ -1653,6 +1653,7 @@ int gemm_gated_fused(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W
   for (const int32_t l : {o.a_scale_layout, o.b_scale_layout})
     if (l != MX_SCALE_2D && l != MX_SCALE_NATIVE && l != MX_SCALE_SWIZZLE_32_4_4) return kGatedNotFused;
   const bool fp4 = A.dtype == MX_E2M1, pack_a = o.a_scale_layout != MX_SCALE_NATIVE, pack_w = o.b_scale_layout != MX_SCALE_NATIVE;
+  if ((!pack_a && (uintptr_t)As.ptr % 16 != 0) || (!pack_w && (uintptr_t)Ws.ptr % 16 != 0)) return kGatedNotFused;   // (refused by the other form)
   const PpRows pp = pp_rows(M, N, K, fp4, pack_a || pack_w, false);
   if (o.kernel == MX_KERNEL_AUTO) {
     if (M <= kStreamAutoM) return kGatedNotFused;

@@ -1,4 +1,4 @@
-"""Operands of the gated product at the ends of what it takes: an empty sum."""
+"""Operands of the gated product at the ends of what it takes: an empty sum, packed scales that are not where they have to be."""
 import ctypes
 
 import pytest
@@ -21,6 +21,20 @@ def test_workspace_of_an_empty_sum():
     good = dict(A=d(L.MX_E4M3, M, 0), As=d(L.MX_E8M0, M, 0), W=d(L.MX_E4M3, 2 * F, 0), Ws=d(L.MX_E8M0, 2 * F, 0),
                 out=d(L.MX_E4M3, M, F), out_s=d(L.MX_E8M0, M, F // 32), gu=None, gus=None, mode=1, opts=None, ws=P, ws_bytes=need - 1)
     assert lib.mx_gated_gemm(*refs(good.values()), None) == L.MX_ERR_WORKSPACE and f"workspace of {need} bytes" in L.last_error()
+
+
+@pytest.mark.parametrize("operand", ["A_scale", "W_scale"])
+@pytest.mark.parametrize("kernel,M", [(L.MX_KERNEL_MFMA_PINGPONG, 300), (L.MX_KERNEL_AUTO, 4000), (L.MX_KERNEL_MFMA_128x128, 300)])
+def test_packed_scales_that_are_not_aligned(kernel, M, operand):
+    """Refused by every kernel that reads them, before anything is enqueued."""
+    K, F = 512, 2048
+    o = L.MxGemmOpts(struct_size=32, kernel=kernel, block_size=32, a_scale_layout=L.MX_SCALE_NATIVE, b_scale_layout=L.MX_SCALE_NATIVE)
+    lib = L.lib()
+    need = lib.mx_gated_gemm_workspace_bytes(M, F, K, ctypes.byref(o))
+    at = {"A_scale": 0, "W_scale": 0, operand: 4}
+    args = [d(L.MX_E4M3, M, K), d(L.MX_E8M0, M, K // 32, ptr=P + at["A_scale"]), d(L.MX_E4M3, 2 * F, K), d(L.MX_E8M0, 2 * F, K // 32, ptr=P + at["W_scale"]),
+            d(L.MX_BF16, M, F), None, None, None, 1, ctypes.byref(o), P, need]
+    assert lib.mx_gated_gemm(*refs(args), None) == L.MX_ERR_LAYOUT and "16-byte aligned" in L.last_error()
 
 
 @pytest.mark.gpu
