@@ -41,8 +41,8 @@ __device__ __forceinline__ void gated_store(const GateOut& o, const v4f (&acc)[4
     u[2 * k + 1] = __builtin_bit_cast(float, pu & 0xFFFF0000u);
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e)   // (the hardware's 2^x and reciprocal: a few units in the last place)
-    h[e] = g[e] * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g[e])) * u[e];
+  for (int e = 0; e < 8; ++e)   // (the hardware's 2^x and reciprocal: a few units in the last place.  Below -126 the reciprocal is 0, which -inf is no factor for)
+    h[e] = fmaxf(g[e], -126.0f) * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g[e])) * u[e];
   if (o.h_fmt == MX_BF16) {
     uint16_t* const p = (uint16_t*)o.h + row * o.h_ld + col;
     if constexpr (HALVES) {
