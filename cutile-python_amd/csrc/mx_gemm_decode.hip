@@ -252,9 +252,7 @@ __device__ __forceinline__ void decode_body(const DecodeArgs& d, const Gate& gat
         return;
       }
       const v4f acc[4] = {sums[0], sums[128], sums[256], sum};
-      saturate_conversions(true);              // (only here: see gemm_pp_gated_kernel)
       gated_store<true>(gate, acc, row, row_of(k - 3) + 4 * (l >> 4), row < d.M, (l >> 4) == 0);
-      saturate_conversions(false);
       return;
     }
     if (row >= d.M) return;

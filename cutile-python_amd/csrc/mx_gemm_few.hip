@@ -133,7 +133,6 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, co
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] += red[((k * MT + wave) * 4 + j) * 64 + lane];
   if constexpr (GATED) {
-    saturate_conversions(true);
     gated_store(o, v, row, 32 * u + 8 * gq, row < a.M, gq == 0);
   } else {
 #pragma unroll

@@ -70,7 +70,6 @@ __global__ __launch_bounds__(C::WAVES * 64, 2) void stream_gated_kernel(const St
 #pragma unroll
     for (int j = 0; j < NT; ++j) red[((nw * a.kw + kq) * (MT * NT) + i * NT + j) * 64 + lane] = acc[i][j];
   __syncthreads();
-  saturate_conversions(true);
   for (int it = wave; it < nwv * MT; it += C::WAVES) {   // uniform per wave
     const int i = it % MT, wv = it / MT;
     v4f v[4] = {};

@@ -57,3 +57,25 @@ def test_gates_without_bound(ct, dev, kernel, w_fmt, M):
     every = torch.ones((M, 2 * F), dtype=torch.bool)
     same_values(got[3:5], want[3:5], every)
     same_values(got[1:3], want[1:3], every[:, :F])
+
+
+@pytest.mark.parametrize("kernel,M", [("stream", 20), ("pingpong", 20), ("pingpong", 300)])
+def test_gates_that_round_up_to_infinity(ct, dev, kernel, M):
+    """Sums of 32 bits between bf16's largest number and 2^128: infinite in bf16 whichever kernel rounds them."""
+    K, F = 512, 128
+    a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(2 * F, K, O.E4M3, 2, dev)
+    u8(a.storage).zero_()
+    u8(a.scale_t)[:] = 127
+    u8(a.storage)[:, :3] = torch.tensor([0x3F, 0x1F, 0x03], dtype=torch.uint8, device=dev)     # 1.875, 2^-3 15/16, 3 2^-9: 1.998 in all
+    u8(a.scale_t)[:, 0] = 254
+    u8(w.storage).zero_()
+    u8(w.storage)[:, :3] = 0x38
+    u8(w.storage)[1:F:2, :3] = 0xB8
+    u8(w.scale_t)[:] = 127
+    u8(w.scale_t)[F:, 0] = 27                                                                  # up: 2^-100 of it
+    got, want = both(ct, a, w, kernel=kernel)
+    assert bool(want[0][:, ::2].isinf().all()) and bool((want[0][:, 1::2] == 0).all())
+    assert torch.equal(got[0], want[0])
+    every = torch.ones((M, 2 * F), dtype=torch.bool)
+    same_values(got[3:5], want[3:5], every)
+    same_values(got[1:3], want[1:3], every[:, :F])
