@@ -5,12 +5,13 @@
 
 namespace mx {
 
-// one MX block's eight values of this lane: codes (E4M3, the floor rule) and scale byte; NaN is NaN among its block's other values
+// one MX block's eight values of this lane: codes (E4M3, the floor rule) and scale byte.  NaN counts as more than infinity, as in encode_block: the
+// scale is 2^120 and what is finite beside it zero.
 __device__ __forceinline__ u2 gated_encode(const float (&v)[8], uint32_t& byte) {
   float m = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) m = fmax_abs(m, v[e]);
-  const BlockScale b = block_scale<MX_E4M3, true>(max_xor_16_32(__builtin_bit_cast(uint32_t, m)));
+  for (int e = 0; e < 8; ++e) m = __builtin_elementwise_maximum(m, __builtin_fabsf(v[e]));   // (keeps NaN; two of them are one instruction)
+  const BlockScale b = block_scale<MX_E4M3, true>(max_xor_16_32(magnitude(m)));
   byte = b.byte;
   return (u2){encode4<MX_E4M3>(v[0], v[1], v[2], v[3], b.scale), encode4<MX_E4M3>(v[4], v[5], v[6], v[7], b.scale)};
 }

@@ -33,6 +33,33 @@ def same_values(got, want, sure):
 
 
 @pytest.mark.parametrize("kernel,w_fmt,M", KERNELS)
+def test_a_block_with_nan(ct, dev, kernel, w_fmt, M):
+    """NaN is the largest of its block under the floor rule: the scale is that of an infinity, and the finite numbers beside it are zeros."""
+    K, F = 1024, 256
+    a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(2 * F, K, w_fmt, 2, dev, std=K ** -0.5)
+    for row, block in ((70, 3), (F + 131, 31), (F + 64, 0)):       # a gate row and two up rows: NaN scales
+        u8(w.scale_t)[row, block] = 0xFF
+    got, want = both(ct, a, w, kernel=kernel)
+    nan = [70, 131, 64]
+    assert bool(got[0][:, nan].isnan().all()) and bool(want[0][:, nan].isnan().all())
+    assert int(got[0].isnan().sum()) == M * 3
+    odd = torch.zeros((M, 2 * F), dtype=torch.bool)               # blocks that hold a NaN (others: sums' last bits may differ)
+    for c in (70, F + 131, F + 64):
+        odd[:, c // 32 * 32:c // 32 * 32 + 32] = True
+    same_values(got[3:5], want[3:5], odd)
+    oddh = odd[:, :F] | odd[:, F:]
+    same_values(got[1:3], want[1:3], oddh)
+    assert bool((u8(got[4]).cpu()[:, 70 // 32] == 247).all()) and bool((u8(got[2]).cpu()[:, 70 // 32] == 247).all())
+    # a NaN in a row of A: every block of the row
+    u8(a.scale_t)[M // 2, 5] = 0xFF
+    got, want = both(ct, a, w, kernel=kernel)
+    row = torch.zeros((M, 2 * F), dtype=torch.bool)
+    row[M // 2] = True
+    same_values(got[3:5], want[3:5], row)
+    same_values(got[1:3], want[1:3], row[:, :F])
+
+
+@pytest.mark.parametrize("kernel,w_fmt,M", KERNELS)
 def test_gates_without_bound(ct, dev, kernel, w_fmt, M):
     """Sums beyond bf16's and beyond 32-bit numbers: silu(-inf) u is zero, silu(inf) u infinite, and what bf16 rounds up to infinity is that."""
     K, F = 512, 128
