@@ -1587,7 +1587,7 @@ namespace mx {
 // The streaming kernel with the gate in its epilogue against the product through memory and a pass over it.  A workgroup of the fused
 // kernel owns 32 columns of the result and all of K, so what grows is each wave's share of a row of W; the separate kernels split K
 // over workgroups as well.  Measured, fused and through memory, us (K x F, rows; FP8 unless noted):
-//   2048 x 7168 1: 7.8 and 10.0; 4096 x 14336 1: 21.4 and 24.1, 32: 24.9 and 27.8; 8192 x 4096 1: 13.2 and 18.8; 8192 x 14336 32: 45.7 and 48.8
+//   2048 x 7168 1: 7.2 and 9.9; 4096 x 14336 1: 21.4 and 24.1, 32: 24.9 and 27.8; 8192 x 4096 1: 13.2 and 18.8; 8192 x 14336 32: 45.7 and 48.8
 //   rows of W over 8192 bytes:                      16384 x 4096 1: 34.3 and 31.5, 16384 x 7168 16: 50.2 and 43.8 (FP4, 8192 bytes: 25.8 and 29.0)
 //   fewer than 128 workgroups, rows over 4096:      8192 x 2048 1: 11.2 and 10.5, 32: 14.5 and 12.0; 4096 x 2048 32: 9.5 and 10.2
 //   FP4, 17 to 32 rows, K over 4096: X is twice as long as W's rows; 8192 x 2048 12.3 and 11.4, 8192 x 7168 14.6 and 18.9, and for

@@ -3,8 +3,8 @@
 // The scaled MFMA aligns the products of an instruction with some 18 bits below the largest: 1.5e-5 of a sum's norm, whatever K.  With
 // many tokens that is far below the roundings around it.  With few, a result that is rounded to bf16 and to E4M3 behind it (gate,
 // up, the activation's gradient) may be one of the large ones that carry a norm, and its other neighbour is 2^-4 of it away: a step of one token,
-// 1024 x 2048, was 0.0055 of dw1's norm off now and then.  Here elements and scales become bf16 numbers, which is exact (but beyond bf16's
-// range: quantised numbers of a float are within it), and v_mfma_f32_16x16x32_bf16 sums them to 1e-7.
+// 1024 x 2048, was 0.0055 of dw1's norm off now and then.  Here elements and scales become bf16 numbers, which is exact but for quantised
+// numbers below bf16's smallest (the least code and scale are 2^-136) and for 2^128, to which the ceiling rule rounds floats just below it, and v_mfma_f32_16x16x32_bf16 sums them to 1e-7.
 //
 // Bound: reading W once.  A load instruction takes 128 bytes, a K-step of four MX blocks, of eight rows; the wave's corner of LDS hands lane
 // (c, g) the 32 bytes of row c's block g, whose scale in the native layout is its own (without that, 16 rows x 16 bytes an instruction,

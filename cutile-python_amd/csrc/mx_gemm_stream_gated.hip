@@ -5,7 +5,7 @@
 // ranges of a workgroup's waves meet in LDS, where a lane then finds gate and up of eight columns, and the four lanes l ^ 16, l ^ 32
 // an MX block.  Workgroups of four waves: two of them fit on a CU, one's start and output beside the other's stream; with eight
 // waves 4096 x 4096 (K x F) FP8 takes 10.5 us in place of 8.8, 8192 x 14336 48 in place of 38.
-// One row: 2048 x 7168 FP8 7.8 us (29 MB of W, 3.8 TB/s; a launch alone is about 3), 8192 x 14336 38 us (235 MB, 6.2 TB/s).
+// One row: 2048 x 7168 FP8 7.2 us (29 MB of W and 1 of scales, 4.2 TB/s; a launch alone is about 3), 8192 x 14336 38 us (235 MB, 6.2 TB/s).
 #include "mx_gated.h"
 #include "mx_gemm_stream.h"
 

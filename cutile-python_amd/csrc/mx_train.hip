@@ -1,6 +1,6 @@
 // Kernels of the gated feed-forward block that is trained in 8 bits: quantisation along both axes of a matrix, the activation
 // between the projections with its checkpoint, and the activation's backward pass.  What they quantise follows encode_block
-// (mx_quant.h) to the bit.
+// (mx_quant.h) to the bit, but for blocks with a NaN or, under the ceiling rule, an infinity in silu_backward_kernel.
 #include <type_traits>
 
 #include "mx_encode.h"
@@ -349,8 +349,8 @@ __global__ __launch_bounds__(256) void gate_up_kernel(const GateUpArgs a) {
 // numbers that stay in registers until their rows' and columns' maxima are known, beside g s, which the second and the third are
 // made of.  4096 x 14336: 109 us where every call writes the same memory, 123 (4.4 TB/s) where it is another; a copy of 2 GiB reaches
 // 5.1 TB/s, and the difference goes into eight streams of one line a row each.
-// g -> g s and s (1 + g (1 - s)) = s + g s (1 - s); exp through the hardware's 2^x and a reciprocal: within 2^-18 of the value, of the terms where
-// they cancel (g near -1.28), against the 2^-4 of what follows.  1 - s, not s + g s - g s s: that is 1 + g - g for a large g, 0 in place of 1
+// g -> g s and s (1 + g (1 - s)) = s + g s (1 - s); exp through the hardware's 2^x and a reciprocal: within 2^-18 of the value (2^-17 for g below -32,
+// where rounding -1.44 g counts), of the terms where they cancel (g near -1.28), against the 2^-4 of what follows.  1 - s, not s + g s - g s s: that is 1 + g - g for a large g, 0 in place of 1
 // from 2^24 on.  s is 0 or 1 far out, and g ends at numbers that such an s multiplies without a NaN (-126, below which s is 0; the largest float for
 // a code and scale beyond it); a NaN comes back through s.
 __device__ __forceinline__ void silu_slope(float g, float& gs, float& slope) {
@@ -462,7 +462,8 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
     if (lr - 4 * rg < n_rows) {                        // (waves without rows have nothing to do)
       auto scale_in = [&](int o, int i) { return (uint32_t)((const uint8_t*)sin[o])[(lr + i) * 4 + lc / 32]; };
       const __amdgpu_buffer_rsrc_t rd = make_rsrc(a.d + r0 * a.d_ld + k0, PLAIN ? (uint32_t)((n_rows - 1) * a.d_ld + F + n_cols) : 0u);
-      // (The maxima pass over NaN: it is NaN among codes of its block's other values.)
+      // (The maxima pass over NaN: it is NaN among codes of its block's other values, where encode_block gives zeros under the floor rule and NaN
+      // under the ceiling rule.  An infinity under the ceiling rule has the scale NaN as there, and other codes.)
       // one result at a time, 32 numbers of a lane: out along the rows (dg, du), then along the columns
       auto row_out = [&](int o, const float (&v)[4][8]) {
 #pragma unroll
@@ -645,7 +646,8 @@ int launch_quantize_both(const BothTensor* list, int n, int fmt, int scale_mode,
       t.once = quantize_loads_once((int64_t)t.rows * t.K);
       // An XCD takes neighbouring tiles, by two rows of tiles, so that lines of scales meet in its L2.  us, row by row over all XCDs and so: bf16
       // 4096 x 14336 46.4 | 43.6, 8192 x 8192 50.2 | 48.7, 28672 x 4096 97 | 94, 16384 x 8192 123 | 109, 16384 x 14336 221 | 199;
-      // fp32 4096 x 4096 20.7 | 19.4, 8192 x 8192 76 | 78; but 32768 x 14336 437 | 469, 32768 x 14464 428 | 501 (32896 x 14336 502 | 443)
+      // fp32 4096 x 4096 20.7 | 19.4, 8192 x 8192 76 | 78; but 32768 x 14336 437 | 469, 32768 x 14464 428 | 501.  Not of a number of elements alone:
+      // 32896 x 14336 502 | 443, 13 % lost here.
       t.near = (int64_t)t.rows * t.K < (int64_t)1 << 28;
       a.t[a.n++] = t;
     }

@@ -352,11 +352,17 @@ MX_API int mx_quantize_both(const mx_tensor* x, mx_tensor* xq, mx_tensor* scale,
  *   [2F,K/32]; opts->a_scale_layout / b_scale_layout are As's / Ws's); F % 32 == 0
  *   out [M,F] MX_BF16 (out_scale NULL), or MX_E4M3 / MX_E5M2 with out_scale [M,F/32], in the format that
  *   mx_silu_mul_quantize leaves.  SiLU is in 32 bits; where the product's own kernel finishes it (the floor rule, bf16 or
- *   E4M3 out) by the hardware's 2^x and reciprocal, a few units in the last place from mx_silu_mul_quantize's
+ *   E4M3 out) by the hardware's 2^x and reciprocal, for gates above -32 a few units in the last place from
+ *   mx_silu_mul_quantize's, 2^-17 of the value at -87, zero for less (mx_silu_mul_quantize: for less than -87.5)
  *   gate_up [M,2F] MX_E4M3 with gate_up_scale [M,2F/32], optional (both NULL): [G|U] quantised, which is what
  *   mx_silu_mul_backward_quantize takes (8.25 bits an element from the forward to the backward pass)
  * Kernels: opts->kernel MX_KERNEL_STREAM, MX_KERNEL_DECODE (M <= 32) and MX_KERNEL_MFMA_PINGPONG do all in one launch where
  * they can, any other the product into the workspace and a pass over it; MX_KERNEL_AUTO takes what is faster.
+ * Precision: every kernel sums on the scaled matrix instructions, which align an instruction's products with some 18 bits below
+ * the largest: G and U are within 1.5e-5 of their norm before they are rounded, and where they are rounded again, a result
+ * that lies that close to a border is its other neighbour (quantised results 0.0004 to 0.004 of their norm from the definition).
+ * What is not finite does not depend on the kernel: a block with a NaN has mx_quantize's scale, silu(-inf) is zero.  K may be
+ * zero: an empty sum is zero.  Of tensors with one row the row stride may be anything.
  * Workspace: mx_gated_gemm_workspace_bytes(), which holds every form; it is asked for whichever is taken.
  */
 MX_API int64_t mx_gated_gemm_workspace_bytes(int64_t M, int64_t F, int64_t K, const mx_gemm_opts* opts);
@@ -371,8 +377,10 @@ MX_API int mx_gated_gemm(const mx_tensor* A, const mx_tensor* A_scale, const mx_
  *   d  [rows,2F], d_scale:  [dg|du] quantised along the rows, for dx = d @ w1
  *   dt [2F,Rpad], dt_scale: its transposed form quantised along the tokens, for dw1 = d.T @ x
  *   at [F,Rpad],  at_scale: the activation, recomputed and quantised along the tokens, for dw2 = dy.T @ a
- * all MX_E4M3, layouts as in mx_quantize_both.  In 32 bits: within 2^-18 of the value before it is quantised, or of the terms of
- * 1 + g (1 - s) where they cancel, for any gate; sigmoids below 2^-126 are zero, and a gate beyond the largest float counts as that.
+ * all MX_E4M3, layouts as in mx_quantize_both.  In 32 bits: before it is quantised a result is within 2^-18 of its value (2^-17 for
+ * gates below -32), or of the terms of 1 + g (1 - s) where they cancel; sigmoids below 2^-126 are zero, and a gate beyond the
+ * largest float counts as that.  A NaN is NaN itself and leaves its block's scale to the other elements (mx_quantize: zeros
+ * beside a NaN under the floor rule, all NaN under the ceiling rule).
  */
 MX_API int mx_silu_mul_backward_quantize(const mx_tensor* dh, const mx_tensor* gate_up, const mx_tensor* gate_up_scale,
                                   mx_tensor* d, mx_tensor* d_scale, mx_tensor* dt, mx_tensor* dt_scale, mx_tensor* at,
@@ -385,7 +393,14 @@ MX_API int mx_silu_mul_backward_quantize(const mx_tensor* dh, const mx_tensor* g
  *   backward  dh = bf16(Q_r(dy) Q_c(w2));  d[G|U] and a as mx_silu_mul_backward_quantize, from Q_r([G|U])
  *             dx = Q_r(d) Q_c(w1);  dw1 = Q_c(d)^T Q_c(x);  dw2 = Q_c(dy)^T Q_c(a)
  *   x [T,H], w1 [2F,H] (gate rows first), w2 [H_out,F], dy [T,H_out]: MX_F32, MX_BF16 or MX_F16; y, dx, dw1, dw2 MX_F32 or
- *   MX_BF16; rows contiguous; H, F and H_out multiples of 32
+ *   MX_BF16; rows contiguous; H, F and H_out multiples of 32; no operand (T x H, T x 2F, T x H_out, 2F x H, H_out x F)
+ *   of 2^31 elements or more
+ * Precision: with few tokens (up to 64, or T F up to 2^19) G, U and dh are summed in 32 bits and results are their definition's to
+ * their rounding; with more, and for the last product of every result, as in mx_gated_gemm (results 0.0017 to 0.0026 of their norm
+ * from the definition, of which rounding to bf16 is 0.0017).  With few tokens operands become bf16 numbers: quantised numbers
+ * below bf16's smallest may be lost there, and 2^128, to which the ceiling rule rounds floats just below it, is infinite.
+ * Infinities: under the floor rule one counts as 1.75 x 2^128, so that what comes of it may be finite; under the ceiling rule
+ * its block is NaN.
  * `saved` (mx_ffn_saved_bytes(), NULL where no backward pass will follow) is what the forward pass leaves for the backward
  * pass: Q_c(x), Q_r([G|U]), Q_c(w1), Q_c(w2).  The backward pass reads it only, and neither x nor the weights.  Of dx,
  * dw1 and dw2 those that are not wanted may be NULL.  A T of zero is a valid forward pass and no valid backward pass.
