@@ -315,9 +315,12 @@ def _round_up_or_down(x, bits):
 
 
 def _store(value, bits, root):
-    """An optimizer state as E4M3 elements and E8M0 scales; roots above zero are never stored as zero."""
+    """An optimizer state as E4M3 elements and E8M0 scales; roots above zero are never stored as zero.  The scale is the least power of
+    two that the block's largest element is at most 448 times of: one that ended at 448 could not grow from step to step."""
     b = value.view(-1, 32)
-    e = _exponent(b.abs().amax(-1))
+    amax = b.abs().amax(-1)
+    f, e = torch.frexp(amax)
+    e = torch.where(amax == 0, -127, e - 9 + (f > 0.875)).clamp(-127, 127)
     v = _round_up_or_down(_down(b, e), bits.view(-1, 32))
     if root:
         v = torch.where(b > 0, v.clamp(min=0.001953125), v)
@@ -471,7 +474,9 @@ def _hash64(x):
 
 def _state64(value, chance, root):
     b = value.reshape(-1, 32)
-    scale = _scale64(b)
+    top = torch.amax(torch.abs(b), -1)
+    scale = _two_to(torch.clamp(torch.where(top > 0, torch.ceil(torch.log2(top / 448)), torch.full_like(top, -127.0)), -127.0, 127.0))
+    scale = torch.where(top > 448 * scale, 2 * scale, scale)   # (a logarithm rounded down to a whole number)
     v = torch.abs(b) / scale[:, None]
     step = _steps(v, 4, -9)
     v = torch.clamp(torch.floor(v / step + chance.reshape(-1, 32) / 65536) * step, max=448.0)
