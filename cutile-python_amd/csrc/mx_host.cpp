@@ -52,6 +52,11 @@ struct Lib {
   MX_FN(mx_ffn_forward_workspace_bytes);
   MX_FN(mx_ffn_backward);
   MX_FN(mx_ffn_backward_workspace_bytes);
+  MX_FN(mx_layer_norm);
+  MX_FN(mx_layer_norm_quantize);
+  MX_FN(mx_layer_norm_backward_workspace_bytes);
+  MX_FN(mx_layer_norm_backward);
+  MX_FN(mx_adamw_step);
 } lib;
 #undef MX_FN
 PyObject* packed_type = nullptr;   // ops.PackedScales
@@ -718,6 +723,309 @@ PyObject* py_feed_forward_backward(PyObject*, PyObject* const* a, Py_ssize_t n) 
   return tuple_of({r[0], r[1], r[2]});
 }
 
+// ---- layer norm ---------------------------------------------------------------------------------------------------------------------
+// a weight or bias: undefined, or a contiguous vector of H on the device
+bool norm_vector(const at::Tensor& t, int64_t H, const at::Device& dev, mx_tensor* d) {
+  if (!t.defined()) return true;
+  if (t.dim() != 1 || t.size(0) != H || !t.is_contiguous() || t.device() != dev || float_code(t.scalar_type()) < 0) return false;
+  *d = desc(t, float_code(t.scalar_type()));
+  return true;
+}
+// an argument that is a tensor or None; false: neither
+bool optional_tensor(PyObject* o, at::Tensor* t) {
+  if (o == Py_None) return true;
+  if (!THPVariable_Check(o)) return false;
+  *t = THPVariable_Unpack(o);
+  return true;
+}
+bool norm_operands(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, mx_tensor* dx, mx_tensor* dw, mx_tensor* db) {
+  return on_current_device(x) && matrix(x, float_code(x.scalar_type()), dx) && norm_vector(w, dx->shape[1], x.device(), dw) &&
+         norm_vector(b, dx->shape[1], x.device(), db);
+}
+mx_tensor rows_of(const at::Tensor& t, int dtype, const mx_tensor& like) {   // a dense tensor as like's matrix
+  return mx_tensor{t.data_ptr(), dtype, 2, {like.shape[0], like.shape[1], 0, 0}, {like.shape[1], 1, 0, 0}, -1, 0};
+}
+at::Tensor norm_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, double eps, at::Tensor* mean, at::Tensor* rstd) {
+  mx_tensor dx, dw, db, dm, dr;
+  if (!norm_operands(x, w, b, &dx, &dw, &db)) throw Refused{0};
+  const at::Device dev = x.device();
+  at::Tensor y = device_empty(x.sizes(), x.scalar_type(), dev);
+  mx_tensor dy = rows_of(y, dx.dtype, dx);
+  if (mean) {
+    *mean = device_empty({dx.shape[0]}, at::kFloat, dev);
+    *rstd = device_empty({dx.shape[0]}, at::kFloat, dev);
+    dm = desc(*mean, MX_F32);
+    dr = desc(*rstd, MX_F32);
+  }
+  const int rc = lib.p_mx_layer_norm(&dx, w.defined() ? &dw : nullptr, b.defined() ? &db : nullptr, eps, &dy, mean ? &dm : nullptr, mean ? &dr : nullptr,
+                                     stream_of(dev));
+  if (rc != MX_OK) throw Refused{rc};
+  return y;
+}
+// dx, dweight, dbias (undefined where not asked for)
+std::vector<at::Tensor> norm_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& mean, const at::Tensor& rstd, const at::Tensor& w,
+                                      const bool (&want)[3], at::ScalarType b_type) {
+  mx_tensor dx, dw, db, ddy, o[3];
+  if (!norm_operands(x, w, at::Tensor(), &dx, &dw, &db) || dy.device() != x.device() || dy.scalar_type() != x.scalar_type() || !matrix(dy, dx.dtype, &ddy) ||
+      ddy.shape[0] != dx.shape[0] || ddy.shape[1] != dx.shape[1])
+    throw Refused{0};
+  const at::Device dev = x.device();
+  for (const at::Tensor* t : {&mean, &rstd})
+    if (t->dim() != 1 || t->size(0) != dx.shape[0] || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->device() != dev) throw Refused{0};
+  std::vector<at::Tensor> out(3);
+  if (want[0]) {
+    out[0] = device_empty(x.sizes(), x.scalar_type(), dev);
+    o[0] = rows_of(out[0], dx.dtype, dx);
+  }
+  for (int i = 1; i < 3; ++i)
+    if (want[i]) {
+      out[i] = device_empty({dx.shape[1]}, i == 2 ? b_type : w.defined() ? w.scalar_type() : at::kFloat, dev);
+      o[i] = desc(out[i], float_code(out[i].scalar_type()));
+    }
+  const int64_t need = want[1] || want[2] ? lib.p_mx_layer_norm_backward_workspace_bytes(dx.shape[0], dx.shape[1]) : 0;
+  at::Tensor ws;
+  if (need > 0) ws = device_empty({need}, at::kByte, dev);
+  mx_tensor dm = desc(mean, MX_F32), dr = desc(rstd, MX_F32);
+  const int rc = lib.p_mx_layer_norm_backward(&ddy, &dx, &dm, &dr, w.defined() ? &dw : nullptr, want[0] ? &o[0] : nullptr, want[1] ? &o[1] : nullptr,
+                                              want[2] ? &o[2] : nullptr, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(dev));
+  if (rc != MX_OK) throw Refused{rc};
+  return out;
+}
+// gradients of a call that was asked for their graph: there is none, and whoever differentiates them is to be told
+std::vector<at::Tensor> without_graph(std::vector<at::Tensor> r, const char* what) {
+  for (at::Tensor& t : r)
+    if (t.defined()) t.set_requires_grad(true);
+  const int n = (int)r.size();
+  return torch::autograd::DelayedError(what, n)(std::move(r));
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const std::optional<at::Tensor>& ow,
+                            const std::optional<at::Tensor>& ob, double eps) {
+    const at::Tensor w = ow.value_or(at::Tensor()), b = ob.value_or(at::Tensor());
+    at::Tensor mean, rstd, y = norm_forward(x, w, b, eps, &mean, &rstd);
+    ctx->save_for_backward({x, w, mean, rstd});
+    ctx->saved_data["bias"] = (int64_t)(b.defined() ? b.scalar_type() : at::ScalarType::Undefined);
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const bool again = at::GradMode::is_enabled();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto s = ctx->get_saved_variables();
+    const auto b_type = (at::ScalarType)ctx->saved_data["bias"].toInt();
+    // (edges are counted over the tensors that there are)
+    const bool has_w = s[1].defined(), has_b = b_type != at::ScalarType::Undefined;
+    const bool want[3] = {ctx->needs_input_grad(0), has_w && ctx->needs_input_grad(1), has_b && ctx->needs_input_grad(has_w ? 2 : 1)};
+    at::Tensor dy = grads[0], x = s[0];
+    mx_tensor d;
+    if (dy.scalar_type() != x.scalar_type()) dy = dy.to(x.scalar_type());
+    if (!matrix(dy, float_code(dy.scalar_type()), &d)) dy = dy.contiguous();
+    std::vector<at::Tensor> r;
+    try {
+      r = norm_backward(dy, x, s[2], s[3], s[1], want, b_type);
+    } catch (const Refused& e) {
+      TORCH_CHECK(false, "layer_norm, backward pass: ", e.rc ? lib.p_mx_last_error() : "unexpected gradient");
+    }
+    if (again) r = without_graph(std::move(r), "layer_norm: its gradients cannot be differentiated");
+    r.emplace_back();
+    return r;
+  }
+};
+
+// layer_norm(x, weight, bias, eps, form) -> result, error code, or None.  form 0: y; 1: (y, mean, rstd); 2: y that autograd
+// differentiates, not under graph capture
+PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 5) { PyErr_SetString(PyExc_TypeError, "layer_norm takes 5 arguments"); return nullptr; }
+  at::Tensor w, b;
+  if (!THPVariable_Check(a[0]) || !optional_tensor(a[1], &w) || !optional_tensor(a[2], &b)) Py_RETURN_NONE;
+  const at::Tensor& x = THPVariable_Unpack(a[0]);
+  const double eps = PyFloat_AsDouble(a[3]);
+  const int form = (int)PyLong_AsLong(a[4]);
+  if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  mx_tensor dx, dw, db;
+  if (!norm_operands(x, w, b, &dx, &dw, &db)) Py_RETURN_NONE;
+  if (form == 2 && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) Py_RETURN_NONE;
+  at::Tensor y, mean, rstd;
+  int rc = MX_OK;
+  {
+    NoGil nogil;
+    try {
+      if (form == 2) {
+        const auto optional = [](const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
+        y = LayerNorm::apply(x, optional(w), optional(b), eps);
+      } else {
+        at::AutoDispatchBelowADInplaceOrView below;
+        y = norm_forward(x, w, b, eps, form == 1 ? &mean : nullptr, &rstd);
+      }
+    } catch (const Refused& e) {
+      rc = e.rc;
+    }
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  return form == 1 ? tuple_of({y, mean, rstd}) : THPVariable_Wrap(y);
+}
+
+// layer_norm_backward(dy, x, mean, rstd, weight, need_dx, need_dweight, need_dbias) -> (dx, dweight, dbias) with None where not asked for,
+// error code, or None; dweight and dbias have weight's type (float32 without a weight)
+PyObject* py_layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8) { PyErr_SetString(PyExc_TypeError, "layer_norm_backward takes 8 arguments"); return nullptr; }
+  for (int i = 0; i < 4; ++i)
+    if (!THPVariable_Check(a[i])) Py_RETURN_NONE;
+  at::Tensor w;
+  if (!optional_tensor(a[4], &w)) Py_RETURN_NONE;
+  const at::Tensor &dy = THPVariable_Unpack(a[0]), &x = THPVariable_Unpack(a[1]), &mean = THPVariable_Unpack(a[2]), &rstd = THPVariable_Unpack(a[3]);
+  const bool want[3] = {PyObject_IsTrue(a[5]) == 1, PyObject_IsTrue(a[6]) == 1, PyObject_IsTrue(a[7]) == 1};
+  std::vector<at::Tensor> r;
+  int rc = MX_OK;
+  {
+    NoGil nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    try {
+      r = norm_backward(dy, x, mean, rstd, w, want, w.defined() ? w.scalar_type() : at::kFloat);
+    } catch (const Refused& e) {
+      rc = e.rc ? e.rc : 1;
+    }
+  }
+  if (rc == 1) Py_RETURN_NONE;
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  return tuple_of({r[0], r[1], r[2]});
+}
+
+// layer_norm_quantize(x, weight, bias, dtype | str, eps, mode) -> (elements, scales), error code, or None
+PyObject* py_layer_norm_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) { PyErr_SetString(PyExc_TypeError, "layer_norm_quantize takes 6 arguments"); return nullptr; }
+  at::Tensor w, b;
+  if (!THPVariable_Check(a[0]) || !optional_tensor(a[1], &w) || !optional_tensor(a[2], &b)) Py_RETURN_NONE;
+  const at::Tensor& x = THPVariable_Unpack(a[0]);
+  const int fmt = format_of(a[3]);                     // (8-bit formats)
+  const double eps = PyFloat_AsDouble(a[4]);
+  const int mode = (int)PyLong_AsLong(a[5]);
+  if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  mx_tensor dx, dw, db;
+  if (fmt < 0 || !norm_operands(x, w, b, &dx, &dw, &db) || dx.shape[1] < 32) Py_RETURN_NONE;
+  const at::Device dev = x.device();
+  Codes c(dx.shape[0], up32(dx.shape[1]), fmt, dev);
+  int rc;
+  {
+    NoGil nogil;
+    rc = lib.p_mx_layer_norm_quantize(&dx, w.defined() ? &dw : nullptr, b.defined() ? &db : nullptr, eps, &c.dq, &c.ds, mode, stream_of(dev));
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  if (x.dim() != 2) {
+    auto shape = x.sizes().vec();
+    shape.back() = up32(dx.shape[1]);
+    c.q = c.q.view(shape);
+    shape.back() /= 32;
+    c.s = c.s.view(shape);
+  }
+  return tuple_of({c.q, c.s});
+}
+
+// ---- AdamW --------------------------------------------------------------------------------------------------------------------------
+// a number, or a tensor of one element of type `t` on the device; false: neither
+bool number_or_tensor(PyObject* o, at::ScalarType t, const at::Device& dev, double* v, const void** at) {
+  if (THPVariable_Check(o)) {
+    const at::Tensor& x = THPVariable_Unpack(o);
+    if (x.scalar_type() != t || x.numel() != 1 || x.device() != dev) return false;
+    *at = x.data_ptr();
+    return true;
+  }
+  *v = PyFloat_AsDouble(o);
+  if (PyErr_Occurred()) { PyErr_Clear(); return false; }
+  return true;
+}
+inline void written(const at::Tensor& t) {   // behind torch's back: whoever saved it for a backward pass is to be told
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+// adamw(params, grads, states, copies | None, step, lr, beta1, beta2, eps, weight_decay, grad_scale, seed) -> True, error code, or None
+PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 12) { PyErr_SetString(PyExc_TypeError, "adamw takes 12 arguments"); return nullptr; }
+  auto seq = [](PyObject* o) { return PyList_Check(o) || PyTuple_Check(o); };
+  if (!seq(a[0]) || !seq(a[1]) || !seq(a[2]) || (a[3] != Py_None && !seq(a[3]))) Py_RETURN_NONE;
+  const Py_ssize_t cnt = PySequence_Fast_GET_SIZE(a[0]);
+  if (cnt == 0 || cnt > 1 << 24) Py_RETURN_NONE;
+  for (int i = 1; i < 4; ++i)
+    if (a[i] != Py_None && PySequence_Fast_GET_SIZE(a[i]) != cnt) Py_RETURN_NONE;
+  std::vector<mx_adamw_tensor> list(cnt);
+  std::vector<at::Tensor> keep;   // written to; the lists may change while the GIL is released
+  keep.reserve(6 * cnt);
+  at::Device dev(at::kCUDA);
+  int bits = 0;
+  for (Py_ssize_t i = 0; i < cnt; ++i) {
+    auto item = [&](int k) { return PySequence_Fast_GET_ITEM(a[k], i); };
+    PyObject* const state = item(2);
+    if (!THPVariable_Check(item(0)) || !PyTuple_Check(state) || PyTuple_GET_SIZE(state) != 4) Py_RETURN_NONE;
+    const at::Tensor& p = THPVariable_Unpack(item(0));
+    if (i == 0) {
+      if (!on_current_device(p)) Py_RETURN_NONE;
+      dev = p.device();
+    }
+    mx_adamw_tensor& t = list[i];
+    t = mx_adamw_tensor{};
+    t.n = p.numel();
+    t.param_dtype = out_code(p.scalar_type());
+    if (t.param_dtype < 0 || p.device() != dev || !p.is_contiguous()) Py_RETURN_NONE;
+    t.grad_dtype = MX_F32;
+    if (item(1) == Py_None) { t.n = 0; continue; }      // no gradient: nothing to do
+    if (!THPVariable_Check(item(1))) Py_RETURN_NONE;
+    const at::Tensor& g = THPVariable_Unpack(item(1));
+    if (g.layout() != at::kStrided || g.device() != dev || g.sizes() != p.sizes() || !g.is_contiguous()) Py_RETURN_NONE;
+    t.grad_dtype = out_code(g.scalar_type());
+    if (t.grad_dtype < 0) Py_RETURN_NONE;
+    PyObject* s[4];
+    for (int k = 0; k < 4; ++k) s[k] = PyTuple_GET_ITEM(state, k);
+    if (!THPVariable_Check(s[0]) || !THPVariable_Check(s[1])) Py_RETURN_NONE;
+    const int b = THPVariable_Unpack(s[0]).scalar_type() == at::kFloat ? 32 : 8;
+    if (bits != 0 && b != bits) Py_RETURN_NONE;
+    bits = b;
+    void* at[4] = {};
+    for (int k = 0; k < (b == 8 ? 4 : 2); ++k) {
+      if (!THPVariable_Check(s[k])) Py_RETURN_NONE;
+      const at::Tensor& x = THPVariable_Unpack(s[k]);
+      const int64_t want = b == 32 ? t.n : k < 2 ? up32(t.n) : up32(t.n) / 32;
+      const auto type = b == 32 ? at::kFloat : k < 2 ? at::kFloat8_e4m3fn : at::kFloat8_e8m0fnu;
+      if (x.scalar_type() != type || x.numel() != want || x.device() != dev || !x.is_contiguous()) Py_RETURN_NONE;
+      at[k] = x.data_ptr();
+      keep.push_back(x);
+    }
+    if (b == 32 && (s[2] != Py_None || s[3] != Py_None)) Py_RETURN_NONE;
+    t.param = p.data_ptr(); t.grad = g.data_ptr();
+    t.exp_avg = at[0]; t.exp_avg_sq = at[1]; t.exp_avg_scale = at[2]; t.exp_avg_sq_scale = at[3];
+    keep.push_back(p);
+    if (a[3] != Py_None && item(3) != Py_None) {
+      if (!THPVariable_Check(item(3))) Py_RETURN_NONE;
+      const at::Tensor& c = THPVariable_Unpack(item(3));
+      if (c.scalar_type() != at::kBFloat16 || c.sizes() != p.sizes() || c.device() != dev || !c.is_contiguous()) Py_RETURN_NONE;
+      t.copy = c.data_ptr();
+      keep.push_back(c);
+    }
+  }
+  mx_adamw_opts o = {};
+  o.struct_size = sizeof(o);
+  o.state_bits = bits ? bits : 32;
+  const void *step_at = nullptr, *lr_at = nullptr, *scale_at = nullptr;
+  if (THPVariable_Check(a[4])) {
+    double unused;
+    if (!number_or_tensor(a[4], at::kLong, dev, &unused, &step_at)) Py_RETURN_NONE;
+  } else {
+    o.step = PyLong_AsLongLong(a[4]);
+  }
+  if (!number_or_tensor(a[5], at::kFloat, dev, &o.lr, &lr_at) || !number_or_tensor(a[10], at::kFloat, dev, &o.grad_scale, &scale_at)) Py_RETURN_NONE;
+  o.beta1 = PyFloat_AsDouble(a[6]); o.beta2 = PyFloat_AsDouble(a[7]); o.eps = PyFloat_AsDouble(a[8]); o.weight_decay = PyFloat_AsDouble(a[9]);
+  o.seed = (uint32_t)PyLong_AsUnsignedLongMask(a[11]);
+  if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  o.step_at = (const int64_t*)step_at; o.lr_at = (const float*)lr_at; o.scale_at = (const float*)scale_at;
+  int rc;
+  {
+    NoGil nogil;
+    rc = lib.p_mx_adamw_step((int32_t)cnt, list.data(), &o, stream_of(dev));
+    if (rc == MX_OK)
+      for (const at::Tensor& t : keep) written(t);
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  Py_RETURN_TRUE;
+}
+
 // bind(handle of the loaded libmxgemm.so, PackedScales class)
 PyObject* py_bind(PyObject*, PyObject* args) {
   unsigned long long h;
@@ -748,6 +1056,11 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   MX_FN(mx_ffn_forward_workspace_bytes)
   MX_FN(mx_ffn_backward)
   MX_FN(mx_ffn_backward_workspace_bytes)
+  MX_FN(mx_layer_norm)
+  MX_FN(mx_layer_norm_quantize)
+  MX_FN(mx_layer_norm_backward_workspace_bytes)
+  MX_FN(mx_layer_norm_backward)
+  MX_FN(mx_adamw_step)
 #undef MX_FN
   Py_INCREF(cls);
   Py_XDECREF(packed_type);
@@ -775,6 +1088,10 @@ PyMethodDef methods[] = {
     {"silu_backward", (PyCFunction)(void (*)(void))guarded<py_silu_backward>, METH_FASTCALL, nullptr},
     {"feed_forward", (PyCFunction)(void (*)(void))guarded<py_feed_forward>, METH_FASTCALL, nullptr},
     {"feed_forward_backward", (PyCFunction)(void (*)(void))guarded<py_feed_forward_backward>, METH_FASTCALL, nullptr},
+    {"layer_norm", (PyCFunction)(void (*)(void))guarded<py_layer_norm>, METH_FASTCALL, nullptr},
+    {"layer_norm_backward", (PyCFunction)(void (*)(void))guarded<py_layer_norm_backward>, METH_FASTCALL, nullptr},
+    {"layer_norm_quantize", (PyCFunction)(void (*)(void))guarded<py_layer_norm_quantize>, METH_FASTCALL, nullptr},
+    {"adamw", (PyCFunction)(void (*)(void))guarded<py_adamw>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mxhost", nullptr, -1, methods};
 

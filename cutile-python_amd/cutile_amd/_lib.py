@@ -53,6 +53,18 @@ class MxGemmOpts(ctypes.Structure):
                 ("split_k", ctypes.c_int32), ("tile_m", ctypes.c_int32)]
 
 
+class MxAdamwTensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "copy")] + [
+        ("n", ctypes.c_int64), ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32)]
+
+
+class MxAdamwOpts(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_int32), ("state_bits", ctypes.c_int32)] + [
+        (n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "grad_scale")] + [
+        ("step", ctypes.c_int64), ("seed", ctypes.c_uint32), ("reserved", ctypes.c_uint32)] + [
+        (n, ctypes.c_void_p) for n in ("lr_at", "step_at", "scale_at")]
+
+
 # every symbol include/mxgemm.h declares: name -> (restype, argtypes)
 _P = ctypes.POINTER
 SYMBOLS = {
@@ -100,6 +112,11 @@ SYMBOLS = {
                                                           ctypes.c_int64, ctypes.c_void_p]),
     "mx_ffn_backward": (ctypes.c_int, [_P(MxTensor), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]
                         + [_P(MxTensor)] * 3 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "mx_layer_norm": (ctypes.c_int, [_P(MxTensor)] * 3 + [ctypes.c_double] + [_P(MxTensor)] * 3 + [ctypes.c_void_p]),
+    "mx_layer_norm_quantize": (ctypes.c_int, [_P(MxTensor)] * 3 + [ctypes.c_double] + [_P(MxTensor)] * 2 + [ctypes.c_int32, ctypes.c_void_p]),
+    "mx_layer_norm_backward_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64] * 2),
+    "mx_layer_norm_backward": (ctypes.c_int, [_P(MxTensor)] * 8 + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "mx_adamw_step": (ctypes.c_int, [ctypes.c_int32, _P(MxAdamwTensor), _P(MxAdamwOpts), ctypes.c_void_p]),
     "mx_probe_mfma_rate": (ctypes.c_int, [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
                                           ctypes.c_void_p, ctypes.c_void_p]),
     "mx_probe_rcp": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]),

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define MXGEMM_VERSION 106
+#define MXGEMM_VERSION 107
 
 /* Exported symbols (the library is built with hidden default visibility). */
 #if defined(__GNUC__)
@@ -414,6 +414,72 @@ MX_API int mx_ffn_forward(const mx_tensor* x, const mx_tensor* w1, const mx_tens
 MX_API int mx_ffn_backward(const mx_tensor* dy, const void* saved, int64_t saved_bytes, int64_t H, int64_t F, mx_tensor* dx,
                     mx_tensor* dw1, mx_tensor* dw2, int32_t scale_mode, void* workspace, int64_t workspace_bytes,
                     void* stream);
+
+/*
+ * Layer norm of the rows of a matrix (no reference counterpart among the ported paths; in front of the projections of a model):
+ *   mean = sum x / H,  rstd = 1 / sqrt(sum (x - mean)^2 / H + eps),  y = (x - mean) rstd weight + bias
+ *   x [rows,H] MX_F32 | MX_BF16 | MX_F16, rows contiguous, of any alignment and pitch; H at least 1
+ *   weight, bias [H] of any of these types, each may be NULL (ones, zeros)
+ *   y [rows,H] of x's type; mean, rstd [rows] MX_F32, each may be NULL
+ * In 32 bits, one rounding at the end; a row with a NaN or an infinity is NaN.
+ */
+MX_API int mx_layer_norm(const mx_tensor* x, const mx_tensor* weight, const mx_tensor* bias, double eps, mx_tensor* y, mx_tensor* mean,
+                  mx_tensor* rstd, void* stream);
+
+/*
+ * The same with y MX-quantised instead of rounded, in one pass: xq, scale and scale_mode as in mx_quantize (H at least 32, the tail
+ * zero); rows of xq start at multiples of 8 bytes (MX_E2M1: of 4).
+ */
+MX_API int mx_layer_norm_quantize(const mx_tensor* x, const mx_tensor* weight, const mx_tensor* bias, double eps, mx_tensor* xq,
+                           mx_tensor* scale, int32_t scale_mode, void* stream);
+
+/*
+ * Backward pass of mx_layer_norm: with h = dy weight, xhat = (x - mean) rstd
+ *   dx = rstd (h - mean(h) - xhat mean(h xhat)),  dweight = sum over rows of dy xhat,  dbias = sum over rows of dy
+ *   dy, x, dx [rows,H] of one type; mean, rstd as the forward pass leaves them; weight may be NULL
+ *   dweight, dbias [H] of any float type.  Of dx, dweight and dbias those that are not wanted may be NULL.
+ * Sums are in 32 bits and in a fixed order.  Workspace, for dweight and dbias only: mx_layer_norm_backward_workspace_bytes().
+ */
+MX_API int64_t mx_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H);
+MX_API int mx_layer_norm_backward(const mx_tensor* dy, const mx_tensor* x, const mx_tensor* mean, const mx_tensor* rstd, const mx_tensor* weight,
+                           mx_tensor* dx, mx_tensor* dweight, mx_tensor* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * One AdamW step over many tensors (no reference counterpart: the reference trains nothing), 54 of them to a launch:
+ *   g = grad * grad_scale,  m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * in 32 bits, param rounded to its type; `copy`, where given, receives the new parameter in MX_BF16 (the copy that a product takes of
+ * an fp32 master).  Tensors are n contiguous elements each; n may be zero.
+ *   state_bits 32: exp_avg = m and exp_avg_sq = v, fp32 [n]; the scales are not used
+ *   state_bits 8:  exp_avg holds m and exp_avg_sq holds sqrt(v) as MX_E4M3 [n rounded up to 32, aligned to 8 bytes], the scales are
+ *     MX_E8M0 [of 32 elements each], the least power of two that keeps the largest of them within 448.  Elements are rounded up or down at random, up with the chance that their place between
+ *     the two neighbours gives: the random bits are a hash of seed, step, place in the list and element, so that a call can be
+ *     repeated.  A root above zero is never stored as zero.  Zeros (elements and scales) are the state to begin with.
+ * lr_at, step_at, scale_at: device addresses of lr, step and grad_scale, or NULL; what is given there is read by the kernel, so that a
+ * captured graph can go on counting.  Parameters, states and copies must not overlap one another, nor a gradient.
+ */
+typedef struct mx_adamw_tensor {
+  void* param;                 /* MX_F32 | MX_BF16 */
+  const void* grad;            /* MX_F32 | MX_BF16 */
+  void* exp_avg;
+  void* exp_avg_sq;
+  void* exp_avg_scale;
+  void* exp_avg_sq_scale;
+  void* copy;
+  int64_t n;
+  int32_t param_dtype, grad_dtype;
+} mx_adamw_tensor;
+typedef struct mx_adamw_opts {
+  int32_t struct_size;         /* sizeof(mx_adamw_opts) */
+  int32_t state_bits;
+  double lr, beta1, beta2, eps, weight_decay, grad_scale;
+  int64_t step;                /* of this step, from 1 on */
+  uint32_t seed, reserved;
+  const float* lr_at;
+  const int64_t* step_at;
+  const float* scale_at;
+} mx_adamw_opts;
+MX_API int mx_adamw_step(int32_t count, const mx_adamw_tensor* tensors, const mx_adamw_opts* opts, void* stream);
 
 /*
  * Re-lays a scale tensor into an MFMA-ready native layout consumed by the MFMA kernels
