@@ -169,9 +169,12 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = g[e] * gs;
-      // (rounded one by one, like the formula in separate operations: a state on the border of two scales is then on the same side)
-      m[e] = __fadd_rn(__fmul_rn(a.b1, m[e]), __fmul_rn(a.c1, x));
-      v[e] = __fadd_rn(__fmul_rn(a.b2, v[e]), __fmul_rn(__fmul_rn(a.c2, x), x));
+      {
+        // (rounded one by one, like the formula in separate operations: what lies on the border of two codes is then on the same side)
+#pragma clang fp contract(off)
+        m[e] = a.b1 * m[e] + a.c1 * x;
+        v[e] = a.b2 * v[e] + a.c2 * x * x;
+      }
       r[e] = __builtin_sqrtf(v[e]);
       p[e] = __builtin_fmaf(p[e], keep, -(rate * m[e] / __builtin_fmaf(r[e], root, a.eps)));
     }

@@ -10,7 +10,7 @@
 // (c, g) the 32 bytes of row c's block g, whose scale in the native layout is its own (without that, 16 rows x 16 bytes an instruction,
 // a step of one token through 4096 x 1024 took 68 us in place of 61).  A bf16 instruction takes eight elements of each of the four
 // blocks.  Two K-steps are in flight in registers, eight waves split K and add up in LDS.  Any K % 32 == 0.
-#include "mx_gated.h"
+#include "mx_linear.h"
 #include "mx_train.h"
 
 namespace mx {
@@ -29,13 +29,17 @@ __device__ __forceinline__ bf8 to_bf16(int lo, int hi, float scale) {
 
 // A workgroup: up to 32 rows of X and four 16-row tiles of W, the 64 rows of group u, or with GATED 32 gate rows and the 32 up rows of the
 // same columns.  Beyond 32 rows workgroups share W: ids 8 apart, which are on one XCD.
-template <int MT, bool GATED>
-__global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, const GateOut o) {
+// Out: Ungated (C), GateOut or LinearOut.
+template <int MT, class Out>
+__global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, const Out o) {
+  constexpr bool GATED = std::is_same<Out, GateOut>::value;
   __shared__ v4f red[kFewWaves * MT * 4 * 64];         // [wave][row tile][tile][lane]; before, 4 KiB a wave to sort operands in
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, gq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), id = blockIdx.x;
   const int slabs = (a.M + 31) / 32, u = slabs > 1 ? id / (8 * slabs) * 8 + id % 8 : id, m0 = slabs > 1 ? id / 8 % slabs * 32 : 0;
-  if (GATED ? 32 * u >= o.F : 64 * u >= a.N) return;   // uniform: the grid is rounded up
+  int F = 0;                                           // of GateOut
+  if constexpr (GATED) F = o.F;
+  if (GATED ? 32 * u >= F : 64 * u >= a.N) return;     // uniform: the grid is rounded up
   const int K = a.K, steps = (K + 127) / 128, KQ = (steps + 3) / 4;
   const int s0 = wave * steps / kFewWaves, s1 = (wave + 1) * steps / kFewWaves;
   const __amdgpu_buffer_rsrc_t rsX = make_rsrc(a.X, (uint32_t)(a.M * K)), rsXs = make_rsrc(a.Xs, (uint32_t)(a.M * (K / 32)));
@@ -51,7 +55,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, co
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int first = GATED ? 32 * u + (j / 2) * o.F : 64 * u + 32 * (j / 2);   // of the 32 rows that tiles j & ~1, j | 1 are
+    const int first = GATED ? 32 * u + (j / 2) * F : 64 * u + 32 * (j / 2);   // of the 32 rows that tiles j & ~1, j | 1 are
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int n = first + 4 * (j % 2) + bperm_lane_off(8 * h + lrow);
@@ -134,6 +138,18 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, co
     for (int j = 0; j < 4; ++j) v[j] += red[((k * MT + wave) * 4 + j) * 64 + lane];
   if constexpr (GATED) {
     gated_store(o, v, row, 32 * u + 8 * gq, row < a.M, gq == 0);
+  } else if constexpr (std::is_same<Out, LinearOut>::value) {
+#pragma unroll 1
+    for (int p = 0; p < 2; ++p) {
+      const int n = 64 * u + 32 * p + 8 * gq;
+      float bias[8];
+      linear_bias(o, n, bias);
+      // (one copy of the activation for each kind: the constants of the others are a branch away)
+      const v4f lo = p ? v[2] : v[0], hi = p ? v[3] : v[1];
+      if (o.act == MX_ACT_GELU) linear_finish<kActErf, true>(o, lo, hi, bias, row, n, a.N - n, row < a.M, gq == 0);
+      else if (o.act == MX_ACT_SILU || o.act == MX_ACT_GELU_TANH) linear_finish<kActSigmoid, true>(o, lo, hi, bias, row, n, a.N - n, row < a.M, gq == 0);
+      else linear_finish<kActPlain, true>(o, lo, hi, bias, row, n, a.N - n, row < a.M, gq == 0);
+    }
   } else {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
@@ -143,11 +159,11 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, co
   }
 }
 
-template <bool GATED>
-int launch(const FewArgs& a, const GateOut& o, int units, hipStream_t stream) {
+template <class Out>
+int launch(const FewArgs& a, const Out& o, int units, hipStream_t stream) {
   const int slabs = (a.M + 31) / 32, blocks = slabs > 1 ? (units + 7) / 8 * 8 * slabs : units;
-  const hipError_t e = a.M <= 16 ? launch_kernel(few_kernel<1, GATED>, dim3((unsigned)blocks), dim3(kFewWaves * 64), 0, stream, a, o)
-                                 : launch_kernel(few_kernel<2, GATED>, dim3((unsigned)blocks), dim3(kFewWaves * 64), 0, stream, a, o);
+  const hipError_t e = a.M <= 16 ? launch_kernel(few_kernel<1, Out>, dim3((unsigned)blocks), dim3(kFewWaves * 64), 0, stream, a, o)
+                                 : launch_kernel(few_kernel<2, Out>, dim3((unsigned)blocks), dim3(kFewWaves * 64), 0, stream, a, o);
   if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "few_kernel launch: %s", hipGetErrorString(e));
   return MX_OK;
 }
@@ -155,7 +171,8 @@ int launch(const FewArgs& a, const GateOut& o, int units, hipStream_t stream) {
 }  // namespace
 
 // (operands of less than 2 GiB, checked by the callers)
-int launch_gemm_few(const FewArgs& a, hipStream_t stream) { return launch<false>(a, GateOut{}, (a.N + 63) / 64, stream); }
-int launch_gemm_few_gated(const FewArgs& a, const GateOut& o, hipStream_t stream) { return launch<true>(a, o, o.F / 32, stream); }
+int launch_gemm_few(const FewArgs& a, hipStream_t stream) { return launch(a, Ungated{}, (a.N + 63) / 64, stream); }
+int launch_gemm_few_gated(const FewArgs& a, const GateOut& o, hipStream_t stream) { return launch(a, o, o.F / 32, stream); }
+int launch_gemm_few_linear(const FewArgs& a, const LinearOut& o, hipStream_t stream) { return launch(a, o, (a.N + 63) / 64, stream); }
 
 }  // namespace mx

@@ -57,6 +57,13 @@ struct Lib {
   MX_FN(mx_layer_norm_backward_workspace_bytes);
   MX_FN(mx_layer_norm_backward);
   MX_FN(mx_adamw_step);
+  MX_FN(mx_linear_gemm);
+  MX_FN(mx_linear_gemm_workspace_bytes);
+  MX_FN(mx_linear_saved_bytes);
+  MX_FN(mx_linear_forward);
+  MX_FN(mx_linear_forward_workspace_bytes);
+  MX_FN(mx_linear_backward);
+  MX_FN(mx_linear_backward_workspace_bytes);
 } lib;
 #undef MX_FN
 PyObject* packed_type = nullptr;   // ops.PackedScales
@@ -921,6 +928,213 @@ PyObject* py_layer_norm_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return tuple_of({c.q, c.s});
 }
 
+// ---- the linear layer -----------------------------------------------------------------------------------------------------------------
+// bias and residual of a result with the sizes `shape` (last: N); false: not for the native path
+bool around(const at::Tensor& bias, const at::Tensor& res, at::IntArrayRef shape, const at::Device& dev, mx_tensor* db, mx_tensor* dr) {
+  if (!norm_vector(bias, shape.back(), dev, db)) return false;
+  return !res.defined() || (res.device() == dev && res.sizes() == shape && matrix(res, float_code(res.scalar_type()), dr));
+}
+
+// linear_gemm(A, A_scale, W, W_scale, bias, residual, a_format, w_format, out_dtype, act, kernel) -> result or tuple, error code, or None
+PyObject* py_linear_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 11) { PyErr_SetString(PyExc_TypeError, "linear_gemm takes 11 arguments"); return nullptr; }
+  at::Tensor bias, res;
+  if (!THPVariable_Check(a[0]) || !THPVariable_Check(a[2]) || !optional_tensor(a[4], &bias) || !optional_tensor(a[5], &res)) Py_RETURN_NONE;
+  const at::Tensor &A = THPVariable_Unpack(a[0]), &W = THPVariable_Unpack(a[2]);
+  if (A.dim() != 2 || W.dim() != 2 || !on_current_device(A) || W.device() != A.device()) Py_RETURN_NONE;
+  const int fa = elem_format(A, a[6]), fw = elem_format(W, a[7]);
+  if (fa < 0 || fw < 0 || A.stride(1) != 1 || W.stride(1) != 1) Py_RETURN_NONE;
+  const at::Device dev = A.device();
+  const mx_tensor dA = desc(A, fa, fa == MX_E2M1 ? 1 : -1), dW = desc(W, fw, fw == MX_E2M1 ? 1 : -1);
+  const int64_t M = dA.shape[0], K = dA.shape[1], N = dW.shape[0], shape[2] = {M, N};
+  if (M == 0 || K == 0 || N == 0 || dW.shape[1] != K) Py_RETURN_NONE;
+  mx_tensor dAs, dWs, db, dr;
+  mx_gemm_opts o = {sizeof(mx_gemm_opts), 0, 0, 0, (int32_t)PyLong_AsLong(a[10]), 32, 0, 0};
+  if (!scale_desc(a[1], M, K, false, dev, &dAs, &o.a_scale_layout) || !scale_desc(a[3], N, K, true, dev, &dWs, &o.b_scale_layout) ||
+      !around(bias, res, shape, dev, &db, &dr))
+    Py_RETURN_NONE;
+  int fo = THPDtype_Check(a[8]) ? out_code(((THPDtype*)a[8])->scalar_type) : -1;
+  if (fo < 0) fo = format_of(a[8]);
+  const int act = (int)PyLong_AsLong(a[9]);
+  if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  if (fo < 0 || fo == MX_E5M2 || (fo == MX_E4M3 && N % 32 != 0)) Py_RETURN_NONE;
+  Codes c;
+  if (fo == MX_E4M3) {
+    c = Codes(M, N, MX_E4M3, dev);
+  } else {
+    c.q = device_empty({M, N}, fo == MX_F32 ? at::kFloat : at::kBFloat16, dev);
+    c.dq = desc(c.q, fo);
+  }
+  const int64_t need = lib.p_mx_linear_gemm_workspace_bytes(M, N, K, &o);
+  at::Tensor ws;
+  if (need > 0) ws = device_empty({need}, at::kByte, dev);
+  int rc;
+  {
+    NoGil nogil;
+    rc = lib.p_mx_linear_gemm(&dA, &dAs, &dW, &dWs, bias.defined() ? &db : nullptr, res.defined() ? &dr : nullptr, act, &c.dq, fo == MX_E4M3 ? &c.ds : nullptr,
+                              nullptr, &o, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(dev));
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  return fo == MX_E4M3 ? tuple_of({c.q, c.s}) : THPVariable_Wrap(c.q);
+}
+
+struct LinearSizes { int64_t T, K, N; };
+bool linear_operands(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, const at::Tensor& res, mx_tensor* dx, mx_tensor* dw, mx_tensor* db,
+                     mx_tensor* dr, LinearSizes* s) {
+  if (!on_current_device(x) || w.device() != x.device() || x.dim() < 2 || w.dim() != 2 || out_code(x.scalar_type()) < 0 || out_code(w.scalar_type()) < 0 ||
+      !matrix(x, out_code(x.scalar_type()), dx) || !matrix(w, out_code(w.scalar_type()), dw))
+    return false;
+  *s = {dx->shape[0], dx->shape[1], dw->shape[0]};
+  if (dw->shape[1] != s->K || s->K % 32 != 0 || s->N % 32 != 0) return false;
+  auto shape = x.sizes().vec();
+  shape.back() = s->N;
+  return around(bias, res, shape, x.device(), db, dr);
+}
+at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, const at::Tensor& res, int act, int mode, at::Tensor* saved) {
+  mx_tensor dx, dw, db, dr;
+  LinearSizes s;
+  if (!linear_operands(x, w, bias, res, &dx, &dw, &db, &dr, &s)) throw Refused{0};
+  const at::Device dev = x.device();
+  auto shape = x.sizes().vec();
+  shape.back() = s.N;
+  at::Tensor y = device_empty(shape, x.scalar_type(), dev);
+  mx_tensor dy{y.data_ptr(), dx.dtype, 2, {s.T, s.N, 0, 0}, {s.N, 1, 0, 0}, -1, 0};
+  const int64_t kept = saved ? lib.p_mx_linear_saved_bytes(s.T, s.K, s.N, act) : 0, need = lib.p_mx_linear_forward_workspace_bytes(s.T, s.K, s.N);
+  if (saved) *saved = device_empty({kept}, at::kByte, dev);
+  at::Tensor ws = device_empty({need}, at::kByte, dev);
+  const int rc = lib.p_mx_linear_forward(&dx, &dw, bias.defined() ? &db : nullptr, res.defined() ? &dr : nullptr, act, &dy, mode,
+                                         saved ? saved->data_ptr() : nullptr, kept, ws.data_ptr(), need, stream_of(dev));
+  if (rc != MX_OK) throw Refused{rc};
+  return y;
+}
+// dx, dw, dbias (undefined where not asked for) from dy [T, N]
+std::vector<at::Tensor> linear_backward(const at::Tensor& dy, const at::Tensor& saved, const LinearSizes& s, const at::ScalarType (&types)[3],
+                                        const bool (&want)[3], int act, int mode) {
+  const at::Device dev = dy.device();
+  mx_tensor d{};
+  if (!matrix(dy, float_code(dy.scalar_type()), &d)) throw Refused{0};
+  std::vector<at::Tensor> out(3);
+  mx_tensor od[3];
+  for (int i = 0; i < 3; ++i)
+    if (want[i]) {
+      out[i] = i == 2 ? device_empty({s.N}, types[i], dev) : device_empty({i == 0 ? s.T : s.N, s.K}, types[i], dev);
+      od[i] = desc(out[i], float_code(types[i]));
+    }
+  const int64_t need = lib.p_mx_linear_backward_workspace_bytes(s.T, s.K, s.N);
+  at::Tensor ws = device_empty({need}, at::kByte, dev);
+  const int rc = lib.p_mx_linear_backward(&d, saved.data_ptr(), saved.numel(), s.K, act, want[0] ? &od[0] : nullptr, want[1] ? &od[1] : nullptr,
+                                          want[2] ? &od[2] : nullptr, mode, ws.data_ptr(), need, stream_of(dev));
+  if (rc != MX_OK) throw Refused{rc};
+  return out;
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias,
+                            const std::optional<at::Tensor>& res, int64_t act, int64_t mode) {
+    at::Tensor saved, y = linear_forward(x, w, bias.value_or(at::Tensor()), res.value_or(at::Tensor()), (int)act, (int)mode, &saved);
+    ctx->save_for_backward({saved});
+    ctx->saved_data["x"] = x.sizes().vec();
+    ctx->saved_data["sizes"] = std::vector<int64_t>{x.numel() / x.size(-1), x.size(-1), w.size(0), act, mode, (int64_t)x.scalar_type(), (int64_t)w.scalar_type(),
+                                                    bias ? (int64_t)bias->scalar_type() : -1, res ? (int64_t)res->scalar_type() : -1};
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const bool again = at::GradMode::is_enabled();
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto v = ctx->saved_data["sizes"].toIntVector();
+    const bool has_b = v[7] >= 0, has_r = v[8] >= 0;
+    const at::ScalarType types[3] = {(at::ScalarType)v[5], (at::ScalarType)v[6], has_b ? (at::ScalarType)v[7] : at::kFloat};
+    // (edges are counted over the tensors that there are)
+    const bool want[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), has_b && ctx->needs_input_grad(2)};
+    const bool want_r = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
+    at::Tensor dy = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({v[0], v[2]});
+    if (dy.stride(1) != 1 || dy.stride(0) < 0) dy = dy.contiguous();
+    std::vector<at::Tensor> r(3);
+    if (want[0] || want[1] || want[2]) {
+      try {
+        r = linear_backward(dy, ctx->get_saved_variables()[0], {v[0], v[1], v[2]}, types, want, (int)v[3], (int)v[4]);
+      } catch (const Refused& e) {
+        TORCH_CHECK(false, "linear, backward pass: ", e.rc ? lib.p_mx_last_error() : "unexpected gradient");
+      }
+    }
+    const auto shape = ctx->saved_data["x"].toIntVector();
+    if (want[0] && shape.size() != 2) r[0] = r[0].view(shape);
+    if (again) r = without_graph(std::move(r), "linear: its gradients cannot be differentiated");
+    r.push_back(want_r ? grads[0].to((at::ScalarType)v[8]) : at::Tensor());
+    r.emplace_back();
+    r.emplace_back();
+    return r;
+  }
+};
+
+// linear(x, w, bias, residual, act, mode, form) -> result, error code, or None.  form 0: y without a backward pass; 1: (y, state for
+// linear_backward); 2: y that autograd differentiates, not under graph capture
+PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 7) { PyErr_SetString(PyExc_TypeError, "linear takes 7 arguments"); return nullptr; }
+  at::Tensor bias, res;
+  if (!THPVariable_Check(a[0]) || !THPVariable_Check(a[1]) || !optional_tensor(a[2], &bias) || !optional_tensor(a[3], &res)) Py_RETURN_NONE;
+  const at::Tensor &x = THPVariable_Unpack(a[0]), &w = THPVariable_Unpack(a[1]);
+  mx_tensor dx, dw, db, dr;
+  LinearSizes s;
+  if (!linear_operands(x, w, bias, res, &dx, &dw, &db, &dr, &s)) Py_RETURN_NONE;
+  const int act = (int)PyLong_AsLong(a[4]), mode = (int)PyLong_AsLong(a[5]), form = (int)PyLong_AsLong(a[6]);
+  if (form == 2 && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) Py_RETURN_NONE;
+  at::Tensor y, saved;
+  int rc = MX_OK;
+  {
+    NoGil nogil;
+    try {
+      if (form == 2) {
+        const auto optional = [](const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
+        y = Linear::apply(x, w, optional(bias), optional(res), (int64_t)act, (int64_t)mode);
+      } else {
+        at::AutoDispatchBelowADInplaceOrView below;
+        y = linear_forward(x, w, bias, res, act, mode, form == 1 ? &saved : nullptr);
+      }
+    } catch (const Refused& e) {
+      rc = e.rc;
+    }
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  return form == 1 ? tuple_of({y, saved}) : THPVariable_Wrap(y);
+}
+
+// linear_backward(dy, saved, T, K, N, x_dtype, w_dtype, bias_dtype, need_dx, need_dw, need_dbias, act, mode)
+//   -> (dx [T, K], dw, dbias) with None where not asked for, error code, or None
+PyObject* py_linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 13) { PyErr_SetString(PyExc_TypeError, "linear_backward takes 13 arguments"); return nullptr; }
+  if (!THPVariable_Check(a[0]) || !THPVariable_Check(a[1])) Py_RETURN_NONE;
+  const at::Tensor &dy = THPVariable_Unpack(a[0]), &saved = THPVariable_Unpack(a[1]);
+  const LinearSizes s = {PyLong_AsLongLong(a[2]), PyLong_AsLongLong(a[3]), PyLong_AsLongLong(a[4])};
+  at::ScalarType types[3];
+  bool want[3];
+  for (int i = 0; i < 3; ++i) {
+    if (!THPDtype_Check(a[5 + i])) Py_RETURN_NONE;
+    types[i] = ((THPDtype*)a[5 + i])->scalar_type;
+    want[i] = PyObject_IsTrue(a[8 + i]) == 1;
+    if ((i < 2 ? out_code(types[i]) : float_code(types[i])) < 0) Py_RETURN_NONE;
+  }
+  const int act = (int)PyLong_AsLong(a[11]), mode = (int)PyLong_AsLong(a[12]);
+  if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  mx_tensor d;
+  if (dy.dim() < 2 || !on_current_device(dy) || saved.device() != dy.device() || !matrix(dy, float_code(dy.scalar_type()), &d) || d.shape[0] != s.T ||
+      d.shape[1] != s.N || !saved.is_contiguous() || saved.scalar_type() != at::kByte)
+    Py_RETURN_NONE;
+  std::vector<at::Tensor> r;
+  int rc = MX_OK;
+  {
+    NoGil nogil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    try {
+      r = linear_backward(dy, saved, s, types, want, act, mode);
+    } catch (const Refused& e) {
+      rc = e.rc;
+    }
+  }
+  if (rc != MX_OK) return PyLong_FromLong(rc);
+  return tuple_of({r[0], r[1], r[2]});
+}
+
 // ---- AdamW --------------------------------------------------------------------------------------------------------------------------
 // a number, or a tensor of one element of type `t` on the device; false: neither
 bool number_or_tensor(PyObject* o, at::ScalarType t, const at::Device& dev, double* v, const void** at) {
@@ -1061,6 +1275,13 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   MX_FN(mx_layer_norm_backward_workspace_bytes)
   MX_FN(mx_layer_norm_backward)
   MX_FN(mx_adamw_step)
+  MX_FN(mx_linear_gemm)
+  MX_FN(mx_linear_gemm_workspace_bytes)
+  MX_FN(mx_linear_saved_bytes)
+  MX_FN(mx_linear_forward)
+  MX_FN(mx_linear_forward_workspace_bytes)
+  MX_FN(mx_linear_backward)
+  MX_FN(mx_linear_backward_workspace_bytes)
 #undef MX_FN
   Py_INCREF(cls);
   Py_XDECREF(packed_type);
@@ -1091,6 +1312,9 @@ PyMethodDef methods[] = {
     {"layer_norm", (PyCFunction)(void (*)(void))guarded<py_layer_norm>, METH_FASTCALL, nullptr},
     {"layer_norm_backward", (PyCFunction)(void (*)(void))guarded<py_layer_norm_backward>, METH_FASTCALL, nullptr},
     {"layer_norm_quantize", (PyCFunction)(void (*)(void))guarded<py_layer_norm_quantize>, METH_FASTCALL, nullptr},
+    {"linear_gemm", (PyCFunction)(void (*)(void))guarded<py_linear_gemm>, METH_FASTCALL, nullptr},
+    {"linear", (PyCFunction)(void (*)(void))guarded<py_linear>, METH_FASTCALL, nullptr},
+    {"linear_backward", (PyCFunction)(void (*)(void))guarded<py_linear_backward>, METH_FASTCALL, nullptr},
     {"adamw", (PyCFunction)(void (*)(void))guarded<py_adamw>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mxhost", nullptr, -1, methods};

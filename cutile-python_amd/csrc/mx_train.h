@@ -43,6 +43,9 @@ struct FewArgs {
 int launch_gemm_few(const FewArgs& a, hipStream_t stream);
 int launch_gemm_few_gated(const FewArgs& a, const GateOut& o, hipStream_t stream);   // N = 2 F; the floor rule, E4M3 out
 
+struct LinearOut;
+int launch_gemm_few_linear(const FewArgs& a, const LinearOut& o, hipStream_t stream);
+
 // dh and the checkpoint [g|u] -> d[g|u] quantised along rows and columns, silu(g) * u along columns (all E4M3)
 struct SiluBackwardArgs {
   const uint16_t* dh;                // bf16

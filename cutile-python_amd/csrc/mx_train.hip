@@ -5,13 +5,13 @@
 
 #include "mx_encode.h"
 #include "mx_gemm_tile.h"   // make_rsrc, kOobOffset
+#include "mx_linear.h"
 #include "mx_load_once.h"
 #include "mx_train.h"
 
 namespace mx {
 namespace {
 
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 
 // Tile (tr, tk) of a workgroup: groups of ROWS tile rows, walked column by column.  Workgroup ids are dealt round-robin to the 8 XCDs,
@@ -609,6 +609,147 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
   }
 }
 
+// ================================================================================================================================
+// A linear layer's gradient through its activation
+// ================================================================================================================================
+// d = dy act'(P), quantised along the rows (for the product with w) and along the columns (for the gradient of w), and its sums over the
+// rows (the bias's gradient).  Bound: memory, 4 bytes read and 2.06 written an element.  Tiles, exchanges and layouts are those of
+// quantize_both_kernel; a column's sum is the lane's eight rows, then lanes l ^ 16, l ^ 32, the four waves, and the tiles by a second launch,
+// always in this order.
+template <int SRC, bool PRE, bool FLOOR>
+__global__ __launch_bounds__(256) void act_backward_kernel(const ActBackwardArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
+  __shared__ uint32_t srow[128], scol[128];
+  __shared__ float sums[4][128];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rg = lane >> 4, cg = lane & 15;
+  uint32_t tr, tk;
+  tile_of<2, true>(blockIdx.x, a.tiles, a.tiles_k, tr, tk);
+  const int64_t r0 = (int64_t)tr * 128, k0 = (int64_t)tk * 128, rows = a.rows, N = a.N, Rpad = (rows + 31) / 32 * 32;
+  const bool inside = r0 < rows && k0 < N;             // (else: padding of native scales only)
+  if constexpr (FLOOR) saturate_conversions();
+  if (a.partial) {
+    for (int i = tid; i < 512; i += 256) sums[i >> 7][i & 127] = 0.f;
+    __syncthreads();
+  }
+  if (inside && r0 + 32 * wave < rows) {               // (waves without rows have nothing to do)
+    const int64_t row = r0 + 32 * wave + 8 * rg, col = k0 + 8 * cg;   // of the lane's first element
+    const bool col_in = col < N;
+    float v[8][8];
+    u4 raw[8][SRC == MX_F32 ? 2 : 1], rp[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool in = col_in && row + i < rows;
+      const uint8_t* const dy = (const uint8_t*)a.dy + (row + i) * a.dy_ld * kSize<SRC>;
+      raw[i][0] = load_piece<SRC>(dy, col, in ? 8 : 0);
+      if constexpr (SRC == MX_F32) raw[i][1] = load_piece<SRC>(dy, col + 4, in ? 4 : 0);
+      if constexpr (PRE) rp[i] = load_piece<MX_BF16>(a.pre + (row + i) * a.pre_ld, col, in ? 8 : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (SRC == MX_F32) {
+        float x[4], y[4];
+        unpack_piece<MX_F32>(raw[i][0], x);
+        unpack_piece<MX_F32>(raw[i][1], y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[i][e] = x[e]; v[i][4 + e] = y[e]; }
+      } else {
+        unpack_piece<SRC>(raw[i][0], v[i]);
+      }
+      if constexpr (PRE) {
+        float p[8];
+        unpack_piece<MX_BF16>(rp[i], p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] *= act_slope(p[e], a.act);
+      }
+    }
+    uint32_t most = 0;
+    if (a.d) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t am = 0, c[2], byte;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) am = umax(am, magnitude(v[i][e]));
+        am = max_quad(am);
+        most = umax(most, am);
+        const BlockScale b = block_scale<MX_E4M3, FLOOR>(am);
+        c[0] = encode4<MX_E4M3>(v[i][0], v[i][1], v[i][2], v[i][3], b.scale);
+        c[1] = encode4<MX_E4M3>(v[i][4], v[i][5], v[i][6], v[i][7], b.scale);
+        byte = b.byte;
+        if (odd_block<FLOOR>(am)) encode_slow<8>(v[i], am, MX_E4M3, FLOOR, c, byte);
+        if (col_in && row + i < rows) *(u2*)(a.d + (row + i) * a.d_ld + col) = (u2){c[0], c[1]};
+        ((uint8_t*)srow)[(32 * wave + 8 * rg + i) * 4 + (cg >> 2)] = (uint8_t)byte;
+      }
+    }
+    auto place = [&](int e, u2 c) {
+      *(u2*)(tile + (8 * cg + e) * 128 + (((2 * wave + (rg >> 1)) ^ (cg & 7)) << 4) + (rg & 1) * 8) = c;
+    };
+    if (a.dt) {
+      uint32_t m[8], own[2];
+      float scale[2], s[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m[e] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[e] = umax(m[e], magnitude(v[i][e]));
+      }
+      max_columns(m, own);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        most = umax(most, own[e]);
+        const BlockScale b = block_scale<MX_E4M3, FLOOR>(own[e]);
+        scale[e] = b.scale;
+        ((uint8_t*)scol)[(8 * cg + own_column(lane) + e) * 4 + wave] = (uint8_t)b.byte;
+      }
+      spread_columns(scale, s);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        place(e, (u2){encode4<MX_E4M3>(v[0][e], v[1][e], v[2][e], v[3][e], s[e]), encode4<MX_E4M3>(v[4][e], v[5][e], v[6][e], v[7][e], s[e])});
+      if (__builtin_amdgcn_ballot_w64(odd_block<FLOOR>(most))) {   // a wave with such a block does its columns again
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float w[8];
+          uint32_t c[2], byte;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = v[i][e];
+          encode_slow<8>(w, max_xor_16_32(m[e]), MX_E4M3, FLOOR, c, byte);
+          place(e, (u2){c[0], c[1]});
+          if (rg == 0) ((uint8_t*)scol)[(8 * cg + e) * 4 + wave] = (uint8_t)byte;
+        }
+      }
+    }
+    if (a.partial) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float s = v[0][e];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += v[i][e];
+        const auto x = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, s), __builtin_bit_cast(uint32_t, s), false, false);
+        s = __builtin_bit_cast(float, (uint32_t)x[0]) + __builtin_bit_cast(float, (uint32_t)x[1]);
+        const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, s), __builtin_bit_cast(uint32_t, s), false, false);
+        s = __builtin_bit_cast(float, (uint32_t)y[0]) + __builtin_bit_cast(float, (uint32_t)y[1]);
+        if (rg == 0) sums[wave][8 * cg + e] = s;
+      }
+    }
+  }
+  __syncthreads();
+  if (inside && a.dt) {
+    const int m_cols = N - k0 < 128 ? (int)(N - k0) : 128, m_rows = Rpad - r0 < 128 ? (int)(Rpad - r0) : 128;   // of the transposed tile
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int c = n * 32 + (tid >> 3), j = tid & 7;
+      if (c < m_cols && 16 * j < m_rows)
+        *(u4*)(a.dt + (k0 + c) * a.dt_ld + r0 + 16 * j) = *(const u4*)(tile + c * 128 + ((j ^ (c >> 3 & 7)) << 4));
+    }
+  }
+  if (inside && a.partial && tid < 128 && k0 + tid < N)
+    a.partial[(int64_t)tr * N + k0 + tid] = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
+  if (tid >= 128) {
+    if (a.d) store_scales(srow, a.ds, a.ds_ld, a.ds_kind, tid - 128, r0, rows, k0 / 32, N / 32);
+  } else if (a.dt) {
+    store_scales(scol, a.dts, a.dts_ld, a.dts_kind, tid, k0, N, r0 / 32, Rpad / 32);
+  }
+}
+
 template <int SRC, int FMT, bool PLAIN>
 hipError_t launch_both(const BothArgs& a, int64_t blocks, hipStream_t stream) {
   const dim3 grid((unsigned)blocks);
@@ -709,6 +850,37 @@ int launch_silu_backward(const SiluBackwardArgs& args, hipStream_t stream) {
   MX_CASE(false, false, false)
 #undef MX_CASE
   if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "silu_backward_kernel launch: %s", hipGetErrorString(e));
+  return MX_OK;
+}
+
+// (N a multiple of 32; rows of d at 8 bytes, of dt at 16: the caller's own)
+int launch_act_backward(const ActBackwardArgs& args, hipStream_t stream) {
+  ActBackwardArgs a = args;
+  if (a.rows <= 0 || a.N <= 0) return MX_OK;
+  const int64_t rows = a.dt && a.dts_kind != kScalePlain ? (a.rows + 511ll) / 512 * 512 : a.rows;
+  const int64_t cols = a.d && a.ds_kind != kScalePlain ? (a.N + 511ll) / 512 * 512 : a.N;
+  a.tiles_k = (int32_t)((cols + 127) / 128);
+  const int64_t blocks = (rows + 127) / 128 * a.tiles_k;
+  if (blocks > 0x7FFFFFFF) return set_error(MX_ERR_SHAPE, "act_backward: tensor too large");
+  a.tiles = (int32_t)blocks;
+  hipError_t e = hipSuccess;
+#define MX_CASE(SRC, PRE, FLOOR) \
+  if (a.dy_dtype == SRC && (a.pre != nullptr) == PRE && (a.scale_mode != 0) == FLOOR) \
+    e = launch_kernel(act_backward_kernel<SRC, PRE, FLOOR>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  MX_CASE(MX_BF16, true, true)
+  MX_CASE(MX_BF16, true, false)
+  MX_CASE(MX_BF16, false, true)
+  MX_CASE(MX_BF16, false, false)
+  MX_CASE(MX_F32, true, true)
+  MX_CASE(MX_F32, true, false)
+  MX_CASE(MX_F32, false, true)
+  MX_CASE(MX_F32, false, false)
+  MX_CASE(MX_F16, true, true)
+  MX_CASE(MX_F16, true, false)
+  MX_CASE(MX_F16, false, true)
+  MX_CASE(MX_F16, false, false)
+#undef MX_CASE
+  if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "act_backward_kernel launch: %s", hipGetErrorString(e));
   return MX_OK;
 }
 

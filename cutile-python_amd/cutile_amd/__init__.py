@@ -15,6 +15,7 @@ from .ops import (PackedScales, bench_block_scaled_matmul, block_quantize, clear
                   silu_and_mul_quantize, swizzle_32_4_4, unswizzle_32_4_4)
 from .ffn import (FeedForwardState, block_quantize_both, gated_block_scaled_matmul, gated_feed_forward,
                   gated_feed_forward_backward, gated_feed_forward_forward, silu_and_mul_backward_quantize)
+from .linear import LinearState, block_scaled_linear, linear, linear_backward, linear_forward
 from .norm import layer_norm, layer_norm_backward, layer_norm_forward, layer_norm_quantize
 from .optim import AdamWState, adamw_state, adamw_step
 
@@ -25,6 +26,7 @@ __all__ = [
     "silu_and_mul_quantize", "cutile_moe_scaled", "grouped_block_scaled_matmul", "bench_block_scaled_matmul",
     "clear_scale_cache", "block_quantize_both", "gated_block_scaled_matmul", "silu_and_mul_backward_quantize",
     "gated_feed_forward", "gated_feed_forward_forward", "gated_feed_forward_backward", "FeedForwardState",
+    "block_scaled_linear", "linear", "linear_forward", "linear_backward", "LinearState",
     "layer_norm", "layer_norm_forward", "layer_norm_backward", "layer_norm_quantize",
     "AdamWState", "adamw_state", "adamw_step",
 ]

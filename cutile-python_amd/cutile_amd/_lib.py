@@ -31,6 +31,7 @@ MX_KERNEL_MFMA_PINGPONG = 6
 MX_KERNEL_MFMA_PINGPONG32 = 7
 MX_KERNEL_MFMA_W4_PERSISTENT = 8
 MX_KERNEL_STREAM = 9
+MX_ACT_NONE, MX_ACT_RELU, MX_ACT_GELU, MX_ACT_GELU_TANH, MX_ACT_SILU = 0, 1, 2, 3, 4
 
 KERNELS = {
     "auto": MX_KERNEL_AUTO, "generic": MX_KERNEL_GENERIC, "mfma128": MX_KERNEL_MFMA_128x128,
@@ -112,6 +113,16 @@ SYMBOLS = {
                                                           ctypes.c_int64, ctypes.c_void_p]),
     "mx_ffn_backward": (ctypes.c_int, [_P(MxTensor), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]
                         + [_P(MxTensor)] * 3 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "mx_linear_gemm_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64] * 3 + [_P(MxGemmOpts)]),
+    "mx_linear_gemm": (ctypes.c_int, [_P(MxTensor)] * 6 + [ctypes.c_int32] + [_P(MxTensor)] * 3 + [
+        _P(MxGemmOpts), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "mx_linear_saved_bytes": (ctypes.c_int64, [ctypes.c_int64] * 3 + [ctypes.c_int32]),
+    "mx_linear_forward_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64] * 3),
+    "mx_linear_backward_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64] * 3),
+    "mx_linear_forward": (ctypes.c_int, [_P(MxTensor)] * 4 + [ctypes.c_int32, _P(MxTensor), ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
+                                                             ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "mx_linear_backward": (ctypes.c_int, [_P(MxTensor), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]
+                           + [_P(MxTensor)] * 3 + [ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
     "mx_layer_norm": (ctypes.c_int, [_P(MxTensor)] * 3 + [ctypes.c_double] + [_P(MxTensor)] * 3 + [ctypes.c_void_p]),
     "mx_layer_norm_quantize": (ctypes.c_int, [_P(MxTensor)] * 3 + [ctypes.c_double] + [_P(MxTensor)] * 2 + [ctypes.c_int32, ctypes.c_void_p]),
     "mx_layer_norm_backward_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64] * 2),

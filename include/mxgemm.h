@@ -119,6 +119,16 @@ enum {
                                  2-D scales, 8-bit or FP4 B with plain or MX_SCALE_NATIVE scales, K % 128 == 0 */
 };
 
+/* Activations of mx_linear_gemm and of the trained layer: x s(x) with s(z) = 1 / (1 + exp(-z)) (MX_ACT_SILU), x P(X < x) of a normal X
+ * (MX_ACT_GELU), x s(2 sqrt(2 / pi) (x + 0.044715 x^3)) (MX_ACT_GELU_TANH). */
+enum {
+  MX_ACT_NONE = 0,
+  MX_ACT_RELU = 1,
+  MX_ACT_GELU = 2,
+  MX_ACT_GELU_TANH = 3,
+  MX_ACT_SILU = 4
+};
+
 typedef struct mx_gemm_opts {
   int32_t struct_size;    /* sizeof(mx_gemm_opts), for forward compatibility                    */
   int32_t accumulate;     /* 0: C = A@B ; 1: C = A@B + C  (the `acc` operand of ct.mma_scaled)   */
@@ -414,6 +424,46 @@ MX_API int mx_ffn_forward(const mx_tensor* x, const mx_tensor* w1, const mx_tens
 MX_API int mx_ffn_backward(const mx_tensor* dy, const void* saved, int64_t saved_bytes, int64_t H, int64_t F, mx_tensor* dx,
                     mx_tensor* dw1, mx_tensor* dw2, int32_t scale_mode, void* workspace, int64_t workspace_bytes,
                     void* stream);
+
+/*
+ * A linear layer on block-scaled operands, in the product's epilogue where its kernel can:
+ *   out = act((A * As) @ (W * Ws).T + bias) + residual
+ * (no reference counterpart: the reference's sample stops at the product.)
+ *   A [M,K], W [N,K] (K contiguous), element formats, scales and layouts as in mx_gemm (Ws is [N,K/32]; opts->a_scale_layout /
+ *   b_scale_layout are As's / Ws's); block size 32; K may be zero
+ *   bias [N] MX_F32 | MX_BF16 | MX_F16 or NULL; residual [M,N] of any of these, rows contiguous, or NULL; activation MX_ACT_*
+ *   out [M,N] MX_F32 | MX_BF16 (out_scale NULL), rows contiguous, of any alignment; or MX_E4M3 with out_scale [M,N/32], N % 32 == 0, rows
+ *   at multiples of 8 bytes: quantised by the floor rule from the unrounded result, the left operand of the next product
+ *   pre [M,N] MX_BF16 or NULL: product + bias, for a backward pass
+ * Sums as in mx_gemm (the scaled matrix instructions align an instruction's products with some 18 bits below the largest: 1.5e-5 of the
+ * result's norm), everything behind them in 32 bits; the activation is within 2e-6 of its value.  act(-inf) is zero for gelu and silu;
+ * a block of out with a NaN has mx_quantize's scale and zeros.
+ * Operands that only the general kernel takes are refused unless opts->kernel is MX_KERNEL_GENERIC; the product then goes through the
+ * workspace.  Workspace: mx_linear_gemm_workspace_bytes(); what mx_gemm_workspace_bytes calls optional is optional here.
+ */
+MX_API int64_t mx_linear_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, const mx_gemm_opts* opts);
+MX_API int mx_linear_gemm(const mx_tensor* A, const mx_tensor* A_scale, const mx_tensor* W, const mx_tensor* W_scale, const mx_tensor* bias,
+                   const mx_tensor* residual, int32_t activation, mx_tensor* out, mx_tensor* out_scale, mx_tensor* pre,
+                   const mx_gemm_opts* opts, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The same layer trained, every product block-scaled (MXFP8 E4M3).  Q_r, Q_c: quantised along the rows, along the columns:
+ *   forward   P = Q_r(x) Q_r(w)^T + bias;  y = act(P) + residual
+ *   backward  d = dy act'(bf16(P));  dx = Q_r(d) Q_c(w);  dw = Q_c(d)^T Q_c(x);  dbias = sum over rows of d  (residual's gradient is dy)
+ *   x [T,K], w [N,K], dy [T,N]: MX_F32, MX_BF16 or MX_F16; bias and residual as in mx_linear_gemm; y, dx, dw MX_F32 or MX_BF16; dbias
+ *   [N] of any float type; rows contiguous; K and N multiples of 32; no operand (T x K, T x N, N x K) of 2^31 elements or more
+ * Precision: with few tokens (up to 64, or T N up to 2^19) P is summed in 32 bits; with more, and in the other products, as in mx_linear_gemm.
+ * `saved` (mx_linear_saved_bytes(), NULL where no backward pass will follow): Q_c(x), Q_c(w) and, with an activation, bf16(P).  The
+ * backward pass reads it only, and neither x nor w.  Of dx, dw and dbias those that are not wanted may be NULL.  A T of zero is a valid
+ * forward pass and no valid backward pass.  saved and workspace are aligned to 256 bytes.
+ */
+MX_API int64_t mx_linear_saved_bytes(int64_t T, int64_t K, int64_t N, int32_t activation);
+MX_API int64_t mx_linear_forward_workspace_bytes(int64_t T, int64_t K, int64_t N);
+MX_API int64_t mx_linear_backward_workspace_bytes(int64_t T, int64_t K, int64_t N);
+MX_API int mx_linear_forward(const mx_tensor* x, const mx_tensor* w, const mx_tensor* bias, const mx_tensor* residual, int32_t activation, mx_tensor* y,
+                      int32_t scale_mode, void* saved, int64_t saved_bytes, void* workspace, int64_t workspace_bytes, void* stream);
+MX_API int mx_linear_backward(const mx_tensor* dy, const void* saved, int64_t saved_bytes, int64_t K, int32_t activation, mx_tensor* dx, mx_tensor* dw,
+                       mx_tensor* dbias, int32_t scale_mode, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Layer norm of the rows of a matrix (no reference counterpart among the ported paths; in front of the projections of a model):
