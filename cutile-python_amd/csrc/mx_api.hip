@@ -11,6 +11,7 @@
 #include "mx_common.h"
 #include "mx_gemm_pp.h"
 #include "mx_gemm_t128.h"
+#include "mx_linear.h"
 #include "mx_moe_rules.h"
 #include "mx_moe_tile.h"
 #include "mx_stream.h"
@@ -394,7 +395,7 @@ constexpr int kAccNeedsCopy = 2;    // gemm_impl with an addend: the kernel can 
 
 int gemm_impl(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const mx_tensor* Bs, mx_tensor* C,
               const mx_gemm_opts* opts, void* workspace, int64_t workspace_bytes, void* stream, GemmPlan* plan,
-              const float* acc = nullptr);
+              const float* acc = nullptr, const LinearOut* lin = nullptr);
 }  // namespace
 
 int mx_gemm(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const mx_tensor* Bs, mx_tensor* C,
@@ -430,10 +431,11 @@ int mx_gemm_add(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, con
 
 namespace {
 // mx_gemm; with `plan` nothing is launched: a problem of the simple kind is described in *plan (return MX_OK),
-// any other valid problem returns kPlanNotSimple.  acc: fp32 addend laid out like C (contiguous)
+// any other valid problem returns kPlanNotSimple.  acc: fp32 addend laid out like C (contiguous).  lin: what becomes of the product
+// in the place of C (its extents and type only are looked at); kLinearNotFused where no kernel that can do it is taken, with nothing enqueued
 int gemm_impl(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const mx_tensor* Bs, mx_tensor* C,
               const mx_gemm_opts* opts, void* workspace, int64_t workspace_bytes, void* stream, GemmPlan* plan,
-              const float* acc) {
+              const float* acc, const LinearOut* lin) {
   mx_gemm_opts o = opts ? *opts : kDefaultOpts;
   if (int rc = check_tensor(A, "A", 2, 3)) return rc;
   if (int rc = check_tensor(B, "B", 2, 3)) return rc;
@@ -666,6 +668,12 @@ int gemm_impl(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const
       kernel != MX_KERNEL_MFMA_256x256_W4)
     return set_error(MX_ERR_LAYOUT, "split_k = %d is only available on the one-tile MFMA kernels (kernel %d chosen)",
                      o.split_k, kernel);
+  if (lin) {
+    if (kernel == MX_KERNEL_DECODE && o.kernel == MX_KERNEL_AUTO && !why_stream) kernel = MX_KERNEL_STREAM;
+    const bool fused = kernel == MX_KERNEL_STREAM || kernel == MX_KERNEL_MFMA_128x128 ||
+                       (kernel == MX_KERNEL_MFMA_PINGPONG && A->dtype == MX_E4M3 && (B->dtype == MX_E4M3 || B->dtype == MX_E2M1) && linear_is_plain(*lin, M));
+    if (!fused) return kLinearNotFused;
+  }
   if (plan && kernel != MX_KERNEL_MFMA_128x128) return kPlanNotSimple;
   if (acc && kernel != MX_KERNEL_MFMA_128x128) return kAccNeedsCopy;
   if (kernel == MX_KERNEL_GENERIC) {
@@ -714,7 +722,7 @@ int gemm_impl(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const
     if (B->dtype != MX_E2M1 && ws_min > 0 && (!workspace || workspace_bytes < ws_min))
       return set_error(MX_ERR_WORKSPACE, "workspace of %lld bytes required, %lld given", (long long)ws_min,
                        (long long)workspace_bytes);
-    return launch_gemm_stream(sa, (hipStream_t)stream);
+    return lin ? launch_gemm_stream_linear(sa, *lin, (hipStream_t)stream) : launch_gemm_stream(sa, (hipStream_t)stream);
   }
 
   if (kernel == MX_KERNEL_DECODE) {
@@ -778,7 +786,7 @@ int gemm_impl(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const
                        t128_plain_scales(Bs->ptr, Bs->stride[1], Bs->stride[0], N, K, A->dtype, B->dtype);
     g.a_plain = a_can; g.b_plain = a_can && b_can;
     // (in place however the rows lie, where that pays: the re-layout launch costs a small product a third of its time)
-    if (!g.b_plain && o.a_scale_layout == MX_SCALE_2D && o.b_scale_layout == MX_SCALE_2D &&
+    if (!g.b_plain && !(lin && S == 1) && o.a_scale_layout == MX_SCALE_2D && o.b_scale_layout == MX_SCALE_2D &&
         t128_any_pays(M, N, K, 1, A->dtype == MX_E2M1 && B->dtype == MX_E2M1) &&
         t128_any_scales(As->stride[0], As->stride[1], M, K) && t128_any_scales(Bs->stride[1], Bs->stride[0], N, K))
       g.a_plain = g.b_plain = kT128ScalesAny;
@@ -822,9 +830,10 @@ int gemm_impl(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const
     }
     if (pack_a || pack_b)   // one launch for both operands
       if (int rc = launch_pack_scales_pair(pack_a ? &pa : nullptr, pack_b ? &pb : nullptr, (hipStream_t)stream)) return rc;
-    if (S == 1) return launch_gemm_t128(g, (hipStream_t)stream);
+    if (S == 1) return lin ? launch_gemm_t128_linear(g, *lin, (hipStream_t)stream) : launch_gemm_t128(g, (hipStream_t)stream);
     g.partial = (float*)ws;
     if (int rc = launch_gemm_t128(g, (hipStream_t)stream)) return rc;
+    if (lin) return launch_linear_pass(g.partial, S, M, *lin, (hipStream_t)stream);
     return launch_splitk_reduce(g.partial, S, M, N, C->ptr, C->stride[0], C->dtype, o.accumulate, (hipStream_t)stream);
   }
   if (S > 1) {
@@ -896,7 +905,7 @@ int gemm_impl(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const
     const int64_t tail = pp_tail_bytes(M, N, K, A->dtype == MX_E2M1 && B->dtype == MX_E2M1, true);
     if (tail > 0 && tile_rows == 256 && workspace_bytes >= need + tail) g.tail = (float*)((uint8_t*)workspace + need);
   }
-  return launch_gemm_mfma(g, kernel, (hipStream_t)stream);
+  return lin ? launch_gemm_pingpong_linear(g, *lin, (hipStream_t)stream) : launch_gemm_mfma(g, kernel, (hipStream_t)stream);
 }
 }  // namespace
 
@@ -1692,5 +1701,19 @@ int gemm_gated_fused(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W
   g.a_rows = M;
   g.tile_rows = pp.rows;
   return launch_gemm_pingpong_gated(g, out, stream);
+}
+
+// A linear layer's product on the kernel that mx_gemm would take, W [N, K] with the scales of its rows (descriptors have been checked).
+int gemm_linear_fused(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const LinearOut& out, const mx_gemm_opts& o,
+                      void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  auto flipped = [](mx_tensor t) {
+    std::swap(t.shape[0], t.shape[1]);
+    std::swap(t.stride[0], t.stride[1]);
+    if (t.packed_dim >= 0) t.packed_dim = 1 - t.packed_dim;
+    return t;
+  };
+  const mx_tensor B = flipped(W), Bs = o.b_scale_layout == MX_SCALE_2D ? flipped(Ws) : Ws;
+  mx_tensor C = {out.c, MX_BF16, 2, {A.shape[0], W.shape[0], 0, 0}, {W.shape[0], 1, 0, 0}, -1, 0};
+  return gemm_impl(&A, &As, &B, &Bs, &C, &o, workspace, workspace_bytes, stream, nullptr, nullptr, &out);
 }
 }  // namespace mx

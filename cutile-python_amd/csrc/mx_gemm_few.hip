@@ -144,11 +144,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, co
       const int n = 64 * u + 32 * p + 8 * gq;
       float bias[8];
       linear_bias(o, n, bias);
-      // (one copy of the activation for each kind: the constants of the others are a branch away)
-      const v4f lo = p ? v[2] : v[0], hi = p ? v[3] : v[1];
-      if (o.act == MX_ACT_GELU) linear_finish<kActErf, true>(o, lo, hi, bias, row, n, a.N - n, row < a.M, gq == 0);
-      else if (o.act == MX_ACT_SILU || o.act == MX_ACT_GELU_TANH) linear_finish<kActSigmoid, true>(o, lo, hi, bias, row, n, a.N - n, row < a.M, gq == 0);
-      else linear_finish<kActPlain, true>(o, lo, hi, bias, row, n, a.N - n, row < a.M, gq == 0);
+      linear_finish_any<true>(o, p ? v[2] : v[0], p ? v[3] : v[1], bias, row, n, a.N - n, row < a.M, gq == 0);
     }
   } else {
 #pragma unroll

@@ -39,6 +39,7 @@
 
 #include "mx_gated.h"
 #include "mx_gemm_pp.h"
+#include "mx_linear.h"
 
 namespace mx {
 namespace {
@@ -53,13 +54,21 @@ namespace {
 // compare and a select per DMA instruction out of the memory phase.
 // SPLIT: the walk may end with a K range of one more tile, whose sums go to g.tail.  (An instance of its own: the few scalars
 // more cost the whole-round products, MXFP4 8192^3 232.2 -> 234.0 us.)
-// Gate: Ungated or GateOut
+// Gate: Ungated, GateOut or LinearGate: bias, activation and residual of a linear layer (mx_linear.h).  The activation's kind and the output's
+// are instances of their own: a wave has 16 groups of eight columns, each with its own copy of all this, and with the choices made there the
+// 270 KiB of a kernel were more than the instruction cache for either team.
+template <int KIND_, bool CODES_>
+struct LinearGate : LinearOut {
+  static constexpr int KIND = KIND_;
+  static constexpr bool CODES = CODES_;
+};
 template <class C, typename OutT, bool GROUPED, bool SPLIT, int TEAM, bool KTAIL, class Gate>
 __device__ __forceinline__ void pp_body(const GemmArgs& g, const Gate& gate, lds_u8* const smem, const int wn,
                                         const int lane, const TileWalk& walk) {
   using P = PP<C>;
-  constexpr bool GATED = !std::is_same<Gate, Ungated>::value;
-  static_assert(!GATED || (!GROUPED && !SPLIT), "");
+  constexpr bool GATED = std::is_same<Gate, GateOut>::value;
+  constexpr bool LINEAR = std::is_base_of<LinearOut, Gate>::value;
+  static_assert(!(GATED || LINEAR) || (!GROUPED && !(GATED && SPLIT)), "");
   constexpr int AL = P::AL, BL = P::BL;
   // A tiles (of 8) whose fragments are read in the memory phase; the others are read inside the MFMA phase,
   // 8 MFMAs ahead of their use.  Two measured best (four: 1.5 % slower on MXFP8, 5 % on the grouped
@@ -286,6 +295,65 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, const Gate& gate, lds
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+      return;
+    } else if constexpr (LINEAR) {
+      constexpr bool CODES = Gate::CODES;
+      const int col = n0 + wn0 + 8 * gq;
+      const uint32_t row = m0 + wm0 + r;
+      float bias[2][8];
+      uint32_t vc[2], vs[2], vp[2], vr[2];             // offsets of the lane's columns in its first row
+      const uint32_t c_ld = (uint32_t)gate.c_ld * (CODES ? 1 : 2), s_ld = (uint32_t)gate.s_ld, p_ld = (uint32_t)gate.pre_ld * 2, r_ld = (uint32_t)gate.r_ld * 2;
+      const __amdgpu_buffer_rsrc_t rc = make_rsrc(gate.c, g.M * c_ld), rsc = make_rsrc(gate.s, CODES ? g.M * s_ld : 0u), rp = make_rsrc(gate.pre, gate.pre ? g.M * p_ld : 0u),
+                                   rr = make_rsrc(gate.res, gate.res ? (g.M - 1) * r_ld + gate.N * 2 : 0u);   // (its rows may overlap)
+#pragma unroll
+      for (int jp = 0; jp < 2; ++jp) {
+        const uint32_t n = col + 32 * jp, out = (int)n < gate.N ? 0u : kOobOffset;
+        linear_bias(gate, n, bias[jp]);
+        vc[jp] = out | (row * c_ld + n * (CODES ? 1 : 2));
+        vs[jp] = out | (gq == 0 ? row * s_ld + n / 32 : kOobOffset);
+        vp[jp] = out | (row * p_ld + n * 2);
+        vr[jp] = out | (row * r_ld + n * 2);
+      }
+      u4 res[2][2];
+      auto request = [&](int i) {                      // (a row tile ahead)
+#pragma unroll
+        for (int jp = 0; jp < 2; ++jp) res[i & 1][jp] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rr, vr[jp] + 16 * i * r_ld, 0, 0));
+      };
+      if (gate.res) request(0);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if (gate.res && i + 1 < MT) request(i + 1);
+#pragma unroll
+        for (int jp = 0; jp < 2; ++jp) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = acc[i][2 * jp][e] + bias[jp][e];
+            v[4 + e] = acc[i][2 * jp + 1][e] + bias[jp][4 + e];
+          }
+          if (gate.pre) __builtin_amdgcn_raw_buffer_store_b128(pack_piece<MX_BF16>(v), rp, vp[jp] + 16 * i * p_ld, 0, 0);
+          activate<Gate::KIND>(v, gate.act);
+          if (gate.res) {
+            float x[8];
+            unpack_piece<MX_BF16>(res[i & 1][jp], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += x[e];
+          }
+          if constexpr (CODES) {
+            uint32_t byte;
+            const float scale = linear_scale<true>(v, byte);
+            saturate_conversions(true);                // (set back behind the store, as in linear_finish)
+            const u2 c = {encode4<MX_E4M3>(v[0], v[1], v[2], v[3], scale), encode4<MX_E4M3>(v[4], v[5], v[6], v[7], scale)};
+            __builtin_amdgcn_raw_buffer_store_b64(c, rc, vc[jp] + 16 * i * c_ld, 0, 0);
+            saturate_conversions(false);
+            __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, rsc, vs[jp] + 16 * i * s_ld, 0, 0);
+          } else {
+            __builtin_amdgcn_raw_buffer_store_b128(pack_piece<MX_BF16>(v), rc, vc[jp] + 16 * i * c_ld, 0, 0);
+          }
+          acc[i][2 * jp] = (v4f){0.f, 0.f, 0.f, 0.f};
+          acc[i][2 * jp + 1] = (v4f){0.f, 0.f, 0.f, 0.f};
+        }
+      }
       return;
     } else if constexpr (!GROUPED) {
       // interior tile, plain store: one address per lane, everything else immediate offsets
@@ -586,15 +654,15 @@ template <class C, typename OutT, bool GROUPED, bool SPLIT>
 __global__ __launch_bounds__(512) void gemm_pp_kernel(const GemmArgs g) {
   pp_kernel<C, OutT, GROUPED, SPLIT>(g, Ungated{});
 }
-template <class C>
-__global__ __launch_bounds__(512) void gemm_pp_gated_kernel(const GemmArgs g, const GateOut gate) {
-  pp_kernel<C, uint16_t, false, false>(g, gate);
+template <class C, bool SPLIT, class Gate>
+__global__ __launch_bounds__(512) void gemm_pp_gated_kernel(const GemmArgs g, const Gate gate) {
+  pp_kernel<C, uint16_t, false, SPLIT>(g, gate);
 }
 
 // Adds up the partial sums of the tiles that gemm_pp_kernel split along K, in the order of their slices, and writes them.
 // Workgroup: (XCD, one of its split tiles, one wave's 128 x 64 block of it), four waves of two row tiles each.
-template <class C, typename OutT, bool GROUPED>
-__global__ __launch_bounds__(256) void pp_tail_kernel(const GemmArgs g, const int grid) {
+template <class C, typename OutT, bool GROUPED, class Gate>
+__global__ __launch_bounds__(256) void pp_tail_kernel(const GemmArgs g, const Gate gate, const int grid) {
   const int xcd = blockIdx.x & 7, wv = (blockIdx.x >> 3) & 7, at = blockIdx.x >> 6;
   const int lane = threadIdx.x & 63, r = lane & 15, gq = lane >> 4, w4 = threadIdx.x >> 6;
   TileWalk walk = {};
@@ -620,6 +688,18 @@ __global__ __launch_bounds__(256) void pp_tail_kernel(const GemmArgs g, const in
       const v4f* const t = (const v4f*)g.tail + ((int64_t)wg * 8 + wv) * 32 * 64 + i * 4 * 64 + lane;
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += t[j * 64];
+    }
+    if constexpr (std::is_base_of<LinearOut, Gate>::value) {
+#pragma unroll
+      for (int jp = 0; jp < 2; ++jp) {
+        const int col = n + 32 * jp;
+        float bias[8];
+        linear_bias(gate, col, bias);
+        ResidualPiece res = {};
+        linear_request(gate, res, m, col, g.N - col, m < g.M);
+        linear_finish<Gate::KIND, true>(gate, v[2 * jp], v[2 * jp + 1], bias, res, m, col, g.N - col, m < g.M, gq == 0);
+      }
+      continue;
     }
     int64_t row = m;
     bool ok = m < g.M;
@@ -660,25 +740,30 @@ int launch_pp(const GemmArgs& g, hipStream_t stream) {
   hipError_t e = launch_kernel(kern, dim3((unsigned)grid), dim3(512), PP<C>::LDS_BYTES, stream, g);
   if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "gemm_pp_kernel launch: %s", hipGetErrorString(e));
   if constexpr (SPLIT) {
-    e = launch_kernel(pp_tail_kernel<C, OutT, GROUPED>, dim3(8 * 8 * kTailMax), dim3(256), 0, stream, g, (int)grid);
+    e = launch_kernel(pp_tail_kernel<C, OutT, GROUPED, Ungated>, dim3(8 * 8 * kTailMax), dim3(256), 0, stream, g, Ungated{}, (int)grid);
     if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "pp_tail_kernel launch: %s", hipGetErrorString(e));
   }
   return MX_OK;
 }
 
-template <class C>
-int launch_pp_gated(const GemmArgs& g, const GateOut& o, hipStream_t stream) {
-  auto kern = gemm_pp_gated_kernel<C>;
+template <class C, bool SPLIT = false, class Gate>
+int launch_pp_gated(const GemmArgs& g, const Gate& o, hipStream_t stream) {
+  auto kern = gemm_pp_gated_kernel<C, SPLIT, Gate>;
   static int attr_done = 0;   // (as above)
   if (!attr_done) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, PP<C>::LDS_BYTES);
     if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "hipFuncSetAttribute(%d bytes LDS): %s", PP<C>::LDS_BYTES, hipGetErrorString(e));
     attr_done = 1;
   }
-  const int64_t grid = pp_grid(g.M, g.N, g.K, C::KSUB, C::BM);
+  int64_t grid = pp_grid(g.M, g.N, g.K, C::KSUB, C::BM);
   if (grid <= 0) return MX_OK;
-  const hipError_t e = launch_kernel(kern, dim3((unsigned)grid), dim3(512), PP<C>::LDS_BYTES, stream, g, o);
+  if (SPLIT) grid = num_cus();
+  hipError_t e = launch_kernel(kern, dim3((unsigned)grid), dim3(512), PP<C>::LDS_BYTES, stream, g, o);
   if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "gemm_pp_gated_kernel launch: %s", hipGetErrorString(e));
+  if constexpr (SPLIT) {
+    e = launch_kernel(pp_tail_kernel<C, uint16_t, false, Gate>, dim3(8 * 8 * kTailMax), dim3(256), 0, stream, g, o, (int)grid);
+    if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "pp_tail_kernel launch: %s", hipGetErrorString(e));
+  }
   return MX_OK;
 }
 
@@ -689,6 +774,19 @@ template <int AF, int BF>
 int launch_pp_gated_pair(const GemmArgs& g, const GateOut& o, hipStream_t stream) {
   if (g.tile_rows == 192) return launch_pp_gated<Cfg<AF, BF, 192, 256, 2, 4>>(g, o, stream);
   return launch_pp_gated<Cfg<AF, BF, 256, 256, 2, 4>>(g, o, stream);
+}
+
+// A linear layer's, one kind of activation.
+template <int AF, int BF, int KIND>
+int launch_pp_linear_pair(const GemmArgs& g, const LinearOut& o, hipStream_t stream) {
+  auto run = [&](auto codes) {
+    LinearGate<KIND, decltype(codes)::value> gate = {};
+    static_cast<LinearOut&>(gate) = o;
+    if (g.tile_rows == 192) return launch_pp_gated<Cfg<AF, BF, 192, 256, 2, 4>>(g, gate, stream);
+    using C = Cfg<AF, BF, 256, 256, 2, 4>;
+    return g.tail ? launch_pp_gated<C, true>(g, gate, stream) : launch_pp_gated<C>(g, gate, stream);
+  };
+  return o.c_fmt == MX_E4M3 ? run(std::true_type{}) : run(std::false_type{});
 }
 
 // One element-format pair (grouped and plain, fp32 and bf16 output) per compilation of this file, so that the pairs
@@ -709,7 +807,9 @@ int launch_pp_pair(const GemmArgs& g, hipStream_t stream) {
   }
   return g.tail ? run(std::true_type{}) : run(std::false_type{});
 }
-#if MX_PP_PAIR >= 4
+#if MX_PP_PAIR >= 8
+template int launch_pp_linear_pair<MX_E4M3, MX_PP_PAIR < 11 ? MX_E4M3 : MX_E2M1, (MX_PP_PAIR - 8) % 3>(const GemmArgs&, const LinearOut&, hipStream_t);
+#elif MX_PP_PAIR >= 4
 template int launch_pp_gated_pair<MX_PP_PAIR == 4 || MX_PP_PAIR == 7 ? MX_E4M3 : MX_PP_PAIR == 5 ? MX_E5M2 : MX_E2M1,
                                   MX_PP_PAIR == 4 ? MX_E4M3 : MX_PP_PAIR == 5 ? MX_E5M2 : MX_E2M1>(const GemmArgs&, const GateOut&, hipStream_t);
 #elif MX_PP_PAIR == 0
@@ -728,6 +828,27 @@ int launch_gemm_pingpong_gated(const GemmArgs& g, const GateOut& o, hipStream_t 
   MX_CASE(MX_E4M3, MX_E2M1)
 #undef MX_CASE
   return set_error(MX_ERR_DTYPE, "MFMA kernel: unsupported element format pair (%d, %d)", g.a_fmt, g.b_fmt);
+}
+#define MX_EXTERN(BF, KIND) extern template int launch_pp_linear_pair<MX_E4M3, BF, KIND>(const GemmArgs&, const LinearOut&, hipStream_t);
+MX_EXTERN(MX_E4M3, kActPlain)
+MX_EXTERN(MX_E4M3, kActSigmoid)
+MX_EXTERN(MX_E4M3, kActErf)
+MX_EXTERN(MX_E2M1, kActPlain)
+MX_EXTERN(MX_E2M1, kActSigmoid)
+MX_EXTERN(MX_E2M1, kActErf)
+#undef MX_EXTERN
+
+// (E4M3 activations, linear_is_plain())
+int launch_gemm_pingpong_linear(const GemmArgs& g, const LinearOut& o, hipStream_t stream) {
+  const int kind = act_kind(o.act);
+#define MX_CASE(BF) \
+  if (g.a_fmt == MX_E4M3 && g.b_fmt == BF) \
+    return kind == kActErf ? launch_pp_linear_pair<MX_E4M3, BF, kActErf>(g, o, stream) \
+           : kind == kActSigmoid ? launch_pp_linear_pair<MX_E4M3, BF, kActSigmoid>(g, o, stream) : launch_pp_linear_pair<MX_E4M3, BF, kActPlain>(g, o, stream);
+  MX_CASE(MX_E4M3)
+  MX_CASE(MX_E2M1)
+#undef MX_CASE
+  return set_error(MX_ERR_DTYPE, "linear ping-pong kernel: unsupported element format pair (%d, %d)", g.a_fmt, g.b_fmt);
 }
 extern template int launch_pp_pair<MX_E5M2, MX_E5M2>(const GemmArgs&, hipStream_t);
 extern template int launch_pp_pair<MX_E2M1, MX_E2M1>(const GemmArgs&, hipStream_t);

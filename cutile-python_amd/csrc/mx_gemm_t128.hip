@@ -31,6 +31,7 @@
 #include "mx_gemm_pp.h"
 #include "mx_gemm_t128.h"
 #include "mx_gemm_tile.h"
+#include "mx_linear.h"
 #include "mx_t128_schedule.h"
 
 namespace mx {
@@ -49,8 +50,11 @@ constexpr int kScaleNative = 0, kScalePlain = 1, kScaleAny = 2;
 template <class C, int NS, int AS>
 constexpr bool kSpread = NS > 2 && !(AS == kScaleAny && C::BM == 128);
 
-template <class C, int NS, int AS, int BS, bool GROUPED, bool SPREAD = kSpread<C, NS, AS>>
-__device__ __forceinline__ void t128_tile(const T128Args& g, lds_u8* const smem, const int pid, const int split, const int bz) {
+// Out: Ungated (C, or partial sums) or LinearOut: bias, activation and residual of a linear layer (mx_linear.h)
+template <class C, int NS, int AS, int BS, bool GROUPED, bool SPREAD = kSpread<C, NS, AS>, class Out = Ungated>
+__device__ __forceinline__ void t128_tile(const T128Args& g, lds_u8* const smem, const int pid, const int split, const int bz, const Out& out = {}) {
+  constexpr bool LINEAR = std::is_same<Out, LinearOut>::value;
+  static_assert(!(LINEAR && GROUPED), "");
   constexpr int KS = C::KSUB, SPQ = 4 / KS, MT = C::MT, NT = C::NTL;
   constexpr bool AP = AS != kScaleNative, BP = BS != kScaleNative, ANY = AS == kScaleAny;
   static_assert(ANY == (BS == kScaleAny) && !(ANY && GROUPED) && MT == NT && (C::BM == 128 || !GROUPED), "");
@@ -280,7 +284,7 @@ __device__ __forceinline__ void t128_tile(const T128Args& g, lds_u8* const smem,
       }
     }
   };
-  if constexpr (EARLY_ADD) {
+  if constexpr (EARLY_ADD && !LINEAR) {
     if (g.c_dtype == MX_F32 && g.k_splits <= 1) load_addend();
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -371,6 +375,35 @@ __device__ __forceinline__ void t128_tile(const T128Args& g, lds_u8* const smem,
   }
 
   // ---- epilogue: lane (r, gq) of tile pair (2 jp, 2 jp + 1) holds row 16 i + r, columns 32 jp + 8 gq .. + 7 -------------
+  if constexpr (LINEAR) {
+    // one copy of it all in a loop, the row tiles moving up behind it (four copies of three activations would be 40 KiB)
+    float bias[NT / 2][8];
+#pragma unroll
+    for (int jp = 0; jp < NT / 2; ++jp) linear_bias(out, n + 32 * jp, bias[jp]);
+#pragma unroll 1
+    for (int i = 0; i < MT; ++i) {
+      const int64_t row = m0 + wm0 + 16 * i + r;
+#pragma unroll 1
+      for (int jp = 0; jp < NT / 2; ++jp) {
+        v4f lo = acc[0][0], hi = acc[0][1];
+        float b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = bias[0][e];
+        if (NT > 2 && jp) {
+          lo = acc[0][NT - 2];
+          hi = acc[0][NT - 1];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) b[e] = bias[NT / 2 - 1][e];
+        }
+        linear_finish_any<true>(out, lo, hi, b, row, n + 32 * jp, cols - 32 * jp, row < g.M, gq == 0);
+      }
+#pragma unroll
+      for (int k = 0; k + 1 < MT; ++k)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[k][j] = acc[k + 1][j];
+    }
+    return;
+  }
   auto store = [&](auto kind) {        // 0: fp32, 1: bf16, 2: fp32 partial product of a split
     constexpr int kd = decltype(kind)::value;
     using OutT = std::conditional_t<kd == 1, uint16_t, float>;
@@ -408,10 +441,10 @@ __device__ __forceinline__ void t128_tile(const T128Args& g, lds_u8* const smem,
   else store(std::integral_constant<int, 1>{});
 }
 
-template <class C, int NS, int AS, int BS, bool GROUPED, bool SPREAD>
-__global__ __launch_bounds__(256, NS == 2 || (C::BM == 64 && NS == 4) ? 2 : 1) void t128_kernel(const T128Args g) {
+template <class C, int NS, int AS, int BS, bool GROUPED, bool SPREAD, class Out>
+__global__ __launch_bounds__(256, NS == 2 || (C::BM == 64 && NS == 4) ? 2 : 1) void t128_kernel(const T128Args g, const Out out) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem_generic[];
-  t128_tile<C, NS, AS, BS, GROUPED, SPREAD>(g, (lds_u8*)smem_generic, blockIdx.x, blockIdx.y, blockIdx.z);
+  t128_tile<C, NS, AS, BS, GROUPED, SPREAD, Out>(g, (lds_u8*)smem_generic, blockIdx.x, blockIdx.y, blockIdx.z, out);
   __builtin_amdgcn_s_waitcnt(0x0F70);   // the trailing zero-fill DMA has left the queue before the LDS is given back
 }
 
@@ -457,9 +490,9 @@ __global__ __launch_bounds__(256, 2) void t128_list_kernel(const T128List gl) {
   }
 }
 
-template <class C, int NS, int AS, int BS, bool GROUPED, bool SPREAD = kSpread<C, NS, AS>>
-int launch_one(const T128Args& g, hipStream_t stream) {
-  auto kern = t128_kernel<C, NS, AS, BS, GROUPED, SPREAD>;
+template <class C, int NS, int AS, int BS, bool GROUPED, bool SPREAD = kSpread<C, NS, AS>, class Out = Ungated>
+int launch_one(const T128Args& g, hipStream_t stream, const Out& out = {}) {
+  auto kern = t128_kernel<C, NS, AS, BS, GROUPED, SPREAD, Out>;
   constexpr int lds = NS * C::STAGE + ((NS + 4 / C::KSUB - 1) / (4 / C::KSUB) + 1) * 4096;
   static int attr_done = 0;   // benign race: the attribute call is idempotent
   if (!attr_done) {
@@ -469,7 +502,7 @@ int launch_one(const T128Args& g, hipStream_t stream) {
   }
   const int64_t tiles = (int64_t)((g.M + C::BM - 1) / C::BM) * ((g.N + C::BN - 1) / C::BN);
   if (tiles <= 0) return MX_OK;
-  hipError_t e = launch_kernel(kern, dim3((unsigned)tiles, (unsigned)g.k_splits, (unsigned)g.batch), dim3(256), lds, stream, g);
+  hipError_t e = launch_kernel(kern, dim3((unsigned)tiles, (unsigned)g.k_splits, (unsigned)g.batch), dim3(256), lds, stream, g, out);
   if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "t128_kernel launch: %s", hipGetErrorString(e));
   return MX_OK;
 }
@@ -521,6 +554,26 @@ int t128_pair(const T128Args& g, hipStream_t stream) {
   }
   return wgs <= 256 ? depth(C{}, std::integral_constant<int, 4>{}) : depth(C{}, std::integral_constant<int, 2>{});
 }
+// The same with a linear layer's epilogue; scales plain in both operands, plain in A, or native (rows at any byte are re-laid first: the
+// instances for them would be as many again).
+template <int AF, int BF>
+int t128_linear_pair(const T128Args& g, const LinearOut& o, hipStream_t stream) {
+  using C = Cfg<AF, BF, 128, 128, 2, 2>;
+  auto depth = [&](auto cfg, auto ns) {
+    using D = decltype(cfg);
+    constexpr int NS = decltype(ns)::value;
+    return !g.a_plain   ? launch_one<D, NS, kScaleNative, kScaleNative, false, kSpread<D, NS, kScaleNative>, LinearOut>(g, stream, o)
+           : !g.b_plain ? launch_one<D, NS, kScalePlain, kScaleNative, false, kSpread<D, NS, kScalePlain>, LinearOut>(g, stream, o)
+                        : launch_one<D, NS, kScalePlain, kScalePlain, false, kSpread<D, NS, kScalePlain>, LinearOut>(g, stream, o);
+  };
+  const int64_t small = t128_small_tiles(g.M, g.N);
+  if (small <= kT128SmallTiles) {
+    using S = Cfg<AF, BF, 64, 64, 2, 2>;
+    return small <= 256 ? depth(S{}, std::integral_constant<int, 8>{}) : depth(S{}, std::integral_constant<int, 4>{});
+  }
+  const int64_t wgs = (int64_t)((g.M + 127) / 128) * ((g.N + 127) / 128);
+  return wgs <= 256 ? depth(C{}, std::integral_constant<int, 4>{}) : depth(C{}, std::integral_constant<int, 2>{});
+}
 template <int AF, int BF>
 int t128_list_pair(const T128Args* problems, int n, hipStream_t stream) {
   using C = Cfg<AF, BF, 128, 128, 2, 2>;
@@ -547,7 +600,15 @@ int t128_list_pair(const T128Args* problems, int n, hipStream_t stream) {
 #define T128_INSTANCES(AF, BF)                                             \
   template int t128_pair<AF, BF>(const T128Args&, hipStream_t);            \
   template int t128_list_pair<AF, BF>(const T128Args*, int, hipStream_t);
-#if T128_PAIR == 1
+#if T128_PAIR == 4
+template int t128_linear_pair<MX_E4M3, MX_E4M3>(const T128Args&, const LinearOut&, hipStream_t);
+#elif T128_PAIR == 5
+template int t128_linear_pair<MX_E5M2, MX_E5M2>(const T128Args&, const LinearOut&, hipStream_t);
+#elif T128_PAIR == 6
+template int t128_linear_pair<MX_E2M1, MX_E2M1>(const T128Args&, const LinearOut&, hipStream_t);
+#elif T128_PAIR == 7
+template int t128_linear_pair<MX_E4M3, MX_E2M1>(const T128Args&, const LinearOut&, hipStream_t);
+#elif T128_PAIR == 1
 T128_INSTANCES(MX_E5M2, MX_E5M2)
 #elif T128_PAIR == 2
 T128_INSTANCES(MX_E2M1, MX_E2M1)
@@ -561,6 +622,24 @@ T128_INSTANCES(MX_E4M3, MX_E4M3)
 T128_EXTERN(MX_E5M2, MX_E5M2)
 T128_EXTERN(MX_E2M1, MX_E2M1)
 T128_EXTERN(MX_E4M3, MX_E2M1)
+
+#define T128_LINEAR(AF, BF) extern template int t128_linear_pair<AF, BF>(const T128Args&, const LinearOut&, hipStream_t);
+T128_LINEAR(MX_E4M3, MX_E4M3)
+T128_LINEAR(MX_E5M2, MX_E5M2)
+T128_LINEAR(MX_E2M1, MX_E2M1)
+T128_LINEAR(MX_E4M3, MX_E2M1)
+
+// (one product, one range of K)
+int launch_gemm_t128_linear(const T128Args& g, const LinearOut& o, hipStream_t stream) {
+#define MX_CASE(AF, BF) \
+  if (g.a_fmt == AF && g.b_fmt == BF) return t128_linear_pair<AF, BF>(g, o, stream);
+  MX_CASE(MX_E4M3, MX_E4M3)
+  MX_CASE(MX_E5M2, MX_E5M2)
+  MX_CASE(MX_E2M1, MX_E2M1)
+  MX_CASE(MX_E4M3, MX_E2M1)
+#undef MX_CASE
+  return set_error(MX_ERR_DTYPE, "MFMA kernel: unsupported element format pair (%d, %d)", g.a_fmt, g.b_fmt);
+}
 
 int launch_gemm_t128(const T128Args& g, hipStream_t stream) {
 #define MX_CASE(AF, BF) \

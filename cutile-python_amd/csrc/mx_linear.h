@@ -83,11 +83,52 @@ __device__ __forceinline__ float act_slope(float x, int act) {
   return __builtin_fmaf(c * s, (1.0f - s) * slope, s);
 }
 
+// eight numbers of a row of the residual as they lie in memory (fp32: two pieces)
+struct ResidualPiece { u4 lo, hi; };
+__device__ __forceinline__ void linear_request(const LinearOut& o, ResidualPiece& r, int64_t row, int col, int cols, bool live) {
+  if (!o.res) return;
+  const int n = live ? cols : 0;
+  if (o.res_dtype == MX_F32) {
+    const float* const p = (const float*)o.res + row * o.r_ld;
+    r.lo = load_piece<MX_F32>(p, col, n);
+    r.hi = load_piece<MX_F32>(p, col + 4, n - 4);
+  } else {
+    r.lo = load_piece<MX_BF16>((const uint16_t*)o.res + row * o.r_ld, col, n);
+  }
+}
+__device__ __forceinline__ void linear_add(const LinearOut& o, const ResidualPiece& p, float (&v)[8]) {
+  if (!o.res) return;
+  if (o.res_dtype == MX_F32) {
+    float x[4], y[4];
+    unpack_piece<MX_F32>(p.lo, x);
+    unpack_piece<MX_F32>(p.hi, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] += x[e]; v[4 + e] += y[e]; }
+  } else {
+    float r[8];
+    if (o.res_dtype == MX_BF16) unpack_piece<MX_BF16>(p.lo, r);
+    else unpack_piece<MX_F16>(p.lo, r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += r[e];
+  }
+}
+
+// scale of the block that four lanes hold (LANES16: l ^ 16, l ^ 32, else 4 n .. 4 n + 3), and its byte
+template <bool LANES16>
+__device__ __forceinline__ float linear_scale(const float (&v)[8], uint32_t& byte) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = __builtin_elementwise_maximum(m, __builtin_fabsf(v[e]));   // (keeps NaN: block_quantize's scale and zeros)
+  const BlockScale s = block_scale<MX_E4M3, true>(LANES16 ? max_xor_16_32(magnitude(m)) : max_quad(magnitude(m)));
+  byte = s.byte;
+  return s.scale;
+}
+
 // Columns col .. col + 7 of row `row`, of which `cols` (1 to 8; anything less: none) exist; a, b: the product.  live: the row exists.
-// With codes the four lanes l ^ 16, l ^ 32 (LANES16) or 4 n .. 4 n + 3 hold a block's 32 columns, scale_lane one of them.
+// With codes four lanes hold a block's 32 columns, scale_lane one of them.
 template <int KIND, bool LANES16>
-__device__ __forceinline__ void linear_finish(const LinearOut& o, const v4f& a, const v4f& b, const float (&bias)[8], int64_t row, int col, int cols, bool live,
-                                              bool scale_lane) {
+__device__ __forceinline__ void linear_finish(const LinearOut& o, const v4f& a, const v4f& b, const float (&bias)[8], const ResidualPiece& res, int64_t row, int col,
+                                              int cols, bool live, bool scale_lane) {
   const bool in = live && cols > 0;
   float v[8];
 #pragma unroll
@@ -95,36 +136,59 @@ __device__ __forceinline__ void linear_finish(const LinearOut& o, const v4f& a, 
     v[e] = a[e] + bias[e];
     v[4 + e] = b[e] + bias[4 + e];
   }
-  if (o.pre && in)
-    store8_edge<uint16_t>(o.pre + row * o.pre_ld + col, (v4f){v[0], v[1], v[2], v[3]}, (v4f){v[4], v[5], v[6], v[7]}, cols);
+  auto put16 = [&](uint16_t* p) { store8_edge<uint16_t>(p, (v4f){v[0], v[1], v[2], v[3]}, (v4f){v[4], v[5], v[6], v[7]}, cols); };
+  if (o.pre && in) put16(o.pre + row * o.pre_ld + col);
   activate<KIND>(v, o.act);
-  if (o.res && in) {
-    float r[8];
-    load_floats<8>((const uint8_t*)o.res + row * o.r_ld * (o.res_dtype == MX_F32 ? 4 : 2), o.res_dtype, col, cols, 0.f, r);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += r[e];
-  }
-  const v4f lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+  linear_add(o, res, v);
   if (o.c_fmt == MX_BF16) {
-    if (in) store8_edge<uint16_t>((uint16_t*)o.c + row * o.c_ld + col, lo, hi, cols);
+    if (in) put16((uint16_t*)o.c + row * o.c_ld + col);
   } else if (o.c_fmt == MX_F32) {
-    if (in) store8_edge<float>((float*)o.c + row * o.c_ld + col, lo, hi, cols);
+    if (in) store8_edge<float>((float*)o.c + row * o.c_ld + col, (v4f){v[0], v[1], v[2], v[3]}, (v4f){v[4], v[5], v[6], v[7]}, cols);
   } else {
-    float m = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = __builtin_elementwise_maximum(m, __builtin_fabsf(v[e]));   // (keeps NaN: block_quantize's scale and zeros)
-    const uint32_t am = LANES16 ? max_xor_16_32(magnitude(m)) : max_quad(magnitude(m));
-    const BlockScale s = block_scale<MX_E4M3, true>(am);
+    uint32_t byte;
+    const float scale = linear_scale<LANES16>(v, byte);
+    // (the mode is set back behind the store: before it, the compiler takes the conversions down to the store, out of the mode)
     saturate_conversions(true);
-    const u2 c = {encode4<MX_E4M3>(v[0], v[1], v[2], v[3], s.scale), encode4<MX_E4M3>(v[4], v[5], v[6], v[7], s.scale)};
-    saturate_conversions(false);
+    const u2 c = {encode4<MX_E4M3>(v[0], v[1], v[2], v[3], scale), encode4<MX_E4M3>(v[4], v[5], v[6], v[7], scale)};
     if (in) {
       *(u2*)((uint8_t*)o.c + row * o.c_ld + col) = c;
-      if (scale_lane) o.s[row * o.s_ld + col / 32] = (uint8_t)s.byte;
+      if (scale_lane) o.s[row * o.s_ld + col / 32] = (uint8_t)byte;
     }
+    saturate_conversions(false);
   }
 }
+// the same with the kind chosen here, where one place finishes all that a wave has
+template <bool LANES16>
+__device__ __forceinline__ void linear_finish_any(const LinearOut& o, const v4f& a, const v4f& b, const float (&bias)[8], int64_t row, int col, int cols, bool live,
+                                                  bool scale_lane) {
+  ResidualPiece res = {};
+  linear_request(o, res, row, col, cols, live);
+  if (o.act == MX_ACT_GELU) linear_finish<kActErf, LANES16>(o, a, b, bias, res, row, col, cols, live, scale_lane);
+  else if (o.act == MX_ACT_SILU || o.act == MX_ACT_GELU_TANH) linear_finish<kActSigmoid, LANES16>(o, a, b, bias, res, row, col, cols, live, scale_lane);
+  else linear_finish<kActPlain, LANES16>(o, a, b, bias, res, row, col, cols, live, scale_lane);
+}
+
+// What a wave's row tiles of the ping-pong kernel leave by: everything through buffer descriptors, whose range takes the place of comparisons
+// with the last row; columns that are not there have an offset beyond it.  bf16 (CODES false) or E4M3 out, a bf16 residual, rows of
+// whole 16-byte pieces (codes: of 8), each tensor less than 2 GiB: linear_is_plain().
+inline bool linear_is_plain(const LinearOut& o, int64_t M) {
+  const int64_t lim = (int64_t)1 << 31;
+  auto fine = [&](const void* p, int64_t ld, int size, int align) { return !p || ((uintptr_t)p % align == 0 && ld * size % align == 0 && M * ld * size < lim); };
+  return o.N % 8 == 0 && (o.c_fmt == MX_BF16 ? fine(o.c, o.c_ld, 2, 16) : o.c_fmt == MX_E4M3 && fine(o.c, o.c_ld, 1, 8) && fine(o.s, o.s_ld, 1, 1)) &&
+         fine(o.pre, o.pre_ld, 2, 16) && (!o.res || (o.res_dtype == MX_BF16 && fine(o.res, o.r_ld, 2, 16)));
+}
 __device__ __forceinline__ void linear_bias(const LinearOut& o, int col, float (&bias)[8]) { load_floats<8>(o.bias, o.bias_dtype, col, o.N - col, 0.f, bias); }
+
+// the product's kernels with this epilogue: MX_KERNEL_MFMA_PINGPONG, MX_KERNEL_MFMA_128x128 (one K range), MX_KERNEL_STREAM
+int launch_gemm_pingpong_linear(const GemmArgs& g, const LinearOut& o, hipStream_t stream);
+struct T128Args;
+int launch_gemm_t128_linear(const T128Args& g, const LinearOut& o, hipStream_t stream);
+struct StreamArgs;
+int launch_gemm_stream_linear(const StreamArgs& a, const LinearOut& o, hipStream_t stream);
+// a product on the kernel that mx_gemm would take, with its workspace; kLinearNotFused: on none of these (nothing enqueued)
+constexpr int kLinearNotFused = 3;
+int gemm_linear_fused(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const LinearOut& out, const mx_gemm_opts& o,
+                      void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 // fp32 products [splits][M][N], added in their order, to the layer's output (mx_linear.hip); splits may be zero
 int launch_linear_pass(const float* product, int splits, int64_t M, const LinearOut& o, hipStream_t stream);

@@ -26,7 +26,9 @@ __global__ __launch_bounds__(256) void linear_pass_kernel(const float* product, 
     }
   float bias[8];
   linear_bias(o, col, bias);
-  linear_finish<KIND, false>(o, a, b, bias, row, col, cols, row < M, (threadIdx.x & 3) == 0);
+  ResidualPiece res = {};
+  linear_request(o, res, row, col, cols, row < M);
+  linear_finish<KIND, false>(o, a, b, bias, res, row, col, cols, row < M, (threadIdx.x & 3) == 0);
 }
 
 // sums [parts][N] -> out [N]: a workgroup takes 64 columns, its waves every 16th part
@@ -96,18 +98,48 @@ int check_linear(const mx_tensor* bias, const mx_tensor* residual, int32_t act, 
 int check_apart(const mx_tensor* t, const char* name) {
   return t->shape[0] > 1 && t->stride[0] < t->shape[1] ? set_error(MX_ERR_LAYOUT, "%s: rows overlap", name) : MX_OK;
 }
-// the product through the workspace, then the pass
-int64_t pass_workspace(int64_t M, int64_t N, int64_t K, const mx_gemm_opts& o) {
-  return round256(M * N * 4) + round256(mx_gemm_workspace_bytes(M, N, K, &o));
+// What no kernel finishes goes through the workspace, some rows at a time (a multiple of 256, which every scale layout can be entered at): the
+// product, then the pass.
+constexpr int64_t kPassBytes = (int64_t)16 << 20;
+int64_t pass_rows(int64_t M, int64_t N) { return std::min(M, std::max(kPassBytes / (N * 4) / 256 * 256, (int64_t)256)); }
+mx_gemm_opts pass_opts(const mx_gemm_opts& o) {
+  mx_gemm_opts r = o;
+  if (r.split_k == 0) r.split_k = 1;
+  return r;
 }
-int run_pass(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const LinearOut& out, const mx_gemm_opts& o, void* workspace,
-             int64_t workspace_bytes, hipStream_t stream) {
-  const int64_t M = A.shape[0], N = W.shape[0];
-  Deal ws = {(uint8_t*)workspace};
-  mx_tensor c = tensor2d(ws.take(M * N * 4), MX_F32, M, N, N);
+int64_t linear_workspace(int64_t M, int64_t N, int64_t K, const mx_gemm_opts& o) {
+  const mx_gemm_opts po = pass_opts(o);
+  const int64_t rows = pass_rows(M, N);
+  return std::max(round256(rows * N * 4) + round256(mx_gemm_workspace_bytes(rows, N, K, &po)), mx_gemm_workspace_bytes(M, N, K, &o));
+}
+int run_linear(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, const mx_tensor& Ws, const LinearOut& out, const mx_gemm_opts& o, void* workspace,
+               int64_t workspace_bytes, hipStream_t stream) {
+  const int64_t M = A.shape[0], N = W.shape[0], K = A.shape[1], rows = pass_rows(M, N);
+  if (const int rc = gemm_linear_fused(A, As, W, Ws, out, o, workspace, workspace_bytes, stream); rc != kLinearNotFused) return rc;
+  const mx_gemm_opts po = pass_opts(o);
   const mx_tensor B = transposed(W), Bs = o.b_scale_layout == MX_SCALE_2D ? transposed(Ws) : Ws;
-  if (int rc = mx_gemm(&A, &As, &B, &Bs, &c, &o, ws.base + ws.at, workspace_bytes - ws.at, stream)) return rc;
-  return launch_linear_pass((const float*)c.ptr, 1, M, out, stream);
+  for (int64_t m0 = 0; m0 < M; m0 += rows) {
+    const int64_t m = std::min(rows, M - m0);
+    Deal ws = {(uint8_t*)workspace};
+    mx_tensor a = A, as = As, c = tensor2d(ws.take(rows * N * 4), MX_F32, m, N, N);
+    a.shape[0] = m;
+    a.ptr = (uint8_t*)A.ptr + m0 * A.stride[0];
+    if (o.a_scale_layout == MX_SCALE_2D || o.a_scale_layout == MX_SCALE_SWIZZLE_32_4_4) {
+      as.shape[0] = o.a_scale_layout == MX_SCALE_2D ? m : m / 128;
+      as.ptr = (uint8_t*)As.ptr + (o.a_scale_layout == MX_SCALE_2D ? m0 : m0 / 128) * As.stride[0];
+    } else {
+      as.shape[0] = m;
+      as.ptr = (uint8_t*)As.ptr + m0 / 64 * packed_scale_quads(K) * 1024;
+    }
+    if (int rc = mx_gemm(&a, &as, &B, &Bs, &c, &po, ws.base + ws.at, workspace_bytes - ws.at, stream)) return rc;
+    LinearOut l = out;
+    l.c = (uint8_t*)out.c + m0 * out.c_ld * (out.c_fmt == MX_F32 ? 4 : out.c_fmt == MX_BF16 ? 2 : 1);
+    if (out.s) l.s = out.s + m0 * out.s_ld;
+    if (out.pre) l.pre = out.pre + m0 * out.pre_ld;
+    if (out.res) l.res = (const uint8_t*)out.res + m0 * out.r_ld * (out.res_dtype == MX_F32 ? 4 : 2);
+    if (int rc = launch_linear_pass((const float*)c.ptr, 1, m, l, stream)) return rc;
+  }
+  return MX_OK;
 }
 
 // ---- the trained layer ----------------------------------------------------------------------------------------------------------------
@@ -150,7 +182,7 @@ LinearForward linear_forward(uint8_t* base, const LinearShape& s) {
   r.w = d.take(s.N * s.K);
   r.ws = d.take(mx_packed_scale_bytes(s.N, s.K));
   const mx_gemm_opts o = layouts(true, true);
-  r.work_bytes = few_tokens(s) ? 0 : pass_workspace(s.T, s.N, s.K, o);
+  r.work_bytes = few_tokens(s) ? 0 : linear_workspace(s.T, s.N, s.K, o);
   r.work = d.take(r.work_bytes);
   r.bytes = d.at;
   return r;
@@ -211,7 +243,7 @@ extern "C" {
 
 int64_t mx_linear_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, const mx_gemm_opts* opts) {
   if (M <= 0 || N <= 0 || K < 0) return 0;
-  return pass_workspace(M, N, K, opts ? *opts : kPlainOpts);
+  return linear_workspace(M, N, K, opts ? *opts : kPlainOpts);
 }
 
 int mx_linear_gemm(const mx_tensor* A, const mx_tensor* As, const mx_tensor* W, const mx_tensor* Ws, const mx_tensor* bias, const mx_tensor* residual,
@@ -261,8 +293,8 @@ int mx_linear_gemm(const mx_tensor* A, const mx_tensor* As, const mx_tensor* W, 
   }
   if (M == 0 || N == 0) return MX_OK;
   o.accumulate = 0;
-  if (int rc = check_room("workspace", workspace, workspace_bytes, pass_workspace(M, N, K, o))) return rc;
-  return run_pass(*A, *As, *W, *Ws, l, o, workspace, workspace_bytes, (hipStream_t)stream);
+  if (int rc = check_room("workspace", workspace, workspace_bytes, linear_workspace(M, N, K, o))) return rc;
+  return run_linear(*A, *As, *W, *Ws, l, o, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 int64_t mx_linear_saved_bytes(int64_t T, int64_t K, int64_t N, int32_t activation) {
@@ -309,7 +341,7 @@ int mx_linear_forward(const mx_tensor* x, const mx_tensor* w, const mx_tensor* b
   l.c = y->ptr; l.c_ld = y->stride[0]; l.c_fmt = y->dtype;
   if (activation != MX_ACT_NONE) { l.pre = (uint16_t*)k.pre; l.pre_ld = s.N; }
   if (few) return launch_gemm_few_linear(FewArgs{f.xq, f.xs, f.w, f.ws, nullptr, (int32_t)s.T, (int32_t)s.N, (int32_t)s.K}, l, st);
-  return run_pass(tensor2d(f.xq, MX_E4M3, s.T, s.K, s.K), tensor2d(f.xs, MX_E8M0, s.T, s.K / 32, s.K / 32), tensor2d(f.w, MX_E4M3, s.N, s.K, s.K),
+  return run_linear(tensor2d(f.xq, MX_E4M3, s.T, s.K, s.K), tensor2d(f.xs, MX_E8M0, s.T, s.K / 32, s.K / 32), tensor2d(f.w, MX_E4M3, s.N, s.K, s.K),
                   tensor2d(f.ws, MX_E8M0, s.N, s.K / 32, s.K / 32), l, layouts(true, true), f.work, f.work_bytes, st);
 }
 

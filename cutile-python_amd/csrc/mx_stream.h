@@ -19,7 +19,7 @@ bool stream_supports(int x_fmt, int w_fmt);
 // the launch refuses exactly these, so a dispatch that asks first never picks the kernel in vain
 const char* stream_issue(const StreamArgs& a);
 struct StreamPlan { int mt, m_tiles, nt, kw, units; float cost; };
-StreamPlan stream_plan(int64_t M, int64_t N, int64_t K, int w_fmt);
+StreamPlan stream_plan(int64_t M, int64_t N, int64_t K, int w_fmt, int least = 1);
 int launch_gemm_stream(const StreamArgs& a, hipStream_t stream);
 
 // the gated form of up to kStreamGatedRows rows (mx_gemm_stream_gated.hip): N = 2 F, F % 32 == 0

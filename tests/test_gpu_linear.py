@@ -112,6 +112,13 @@ CASES = [
     ("pingpong", "e4m3", "e4m3", 1531, 512, 1088, None, bf16, None),
     ("pingpong", "e4m3", "e4m3", 2305, 512, 4161, bf16, None, "gelu"),
     ("pingpong", "e4m3", "e4m3", 2305, 1024, 4160, bf16, bf16, "silu"),
+    # tiles split along K: all of them; those behind a whole round
+    ("pingpong", "e4m3", "e4m3", 500, 4096, 520, bf16, bf16, "gelu"),
+    ("pingpong", "e4m3", "e4m3", 257, 8192, 288, f32, None, "silu"),
+    ("pingpong", "e4m3", "e2m1", 1, 4096, 264, None, bf16, None),
+    ("pingpong", "e4m3", "e2m1", 600, 6144, 544, bf16, None, "gelu_tanh"),
+    ("pingpong", "e4m3", "e4m3", 4200, 4096, 4128, bf16, bf16, "gelu"),
+    ("auto", "e4m3", "e4m3", 1531, 8192, 1088, bf16, bf16, "relu"),
     ("mfma256", "e4m3", "e4m3", 300, 512, 320, bf16, bf16, "gelu"),
     ("generic", "e4m3", "e4m3", 33, 96, 64, bf16, bf16, "gelu"),
     ("generic", "e2m1", "e4m3", 5, 64, 30, f32, f32, "silu"),
@@ -137,7 +144,7 @@ def test_product_with_epilogue(ct, dev, kernel, af, wf, M, K, N, bt, rt, act):
             check(y, want, err, dtype)
         if N % 32 == 0:
             q, s = ct.block_scaled_linear(*args, out_dtype=torch.float8_e4m3fn, **kw)
-            assert q.shape == (M, N) and s.shape == (M, N // 32)
+            assert q.shape == (M, N) and s.shape == (M, N // 32) and bool(q.float().isfinite().all())
             check_codes(q, s, want, err)
 
 
