@@ -196,7 +196,7 @@ def _own(s):
     if kind == "train":
         y = ct.linear(s["x"], s["w"], s["bias"], s["res"], activation=act)
         return (y, *torch.autograd.grad(y, (s["x"], s["w"], s["bias"]), s["dy"]))
-    ct.adamw_step(s["params"], s["grads"], [ct.AdamWState(*t) for t in s["states"]], step=STEP, lr=LR, betas=(BETA1, BETA2), eps=ADAM_EPS,
+    ct.adamw_step(s["params"], s["grads"], s["states"], step=STEP, lr=LR, betas=(BETA1, BETA2), eps=ADAM_EPS,
                   weight_decay=DECAY, seed=SEED, copies=s["copies"] if case["copy"] else None)
     return _adamw_outputs(s)
 
