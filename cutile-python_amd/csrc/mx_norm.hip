@@ -44,8 +44,12 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& slot) {
   }
 }
 
-// codes and scale byte of a piece whose block's other elements are in the neighbouring lanes
-template <int T>
+// what a row's result becomes.  E4M3 under the floor rule has an instance of its own, by the hardware's conversions alone
+// (1531 x 8192 with encode_block in all of them: 23.9 us): the other formats and the ceiling rule share encode_block.
+enum { kNormFloats, kNormE4M3, kNormCodes };
+
+// codes and scale byte of a piece whose block's other elements are in the neighbouring lanes (OUT kNormE4M3: conversions saturate)
+template <int T, int OUT>
 __device__ __forceinline__ void store_codes(const NormArgs& a, int64_t row, int piece, const float (&v)[kPiece<T>]) {
   constexpr int E = kPiece<T>, LPB = 32 / E;
   uint32_t am = 0, code[E];
@@ -54,6 +58,15 @@ __device__ __forceinline__ void store_codes(const NormArgs& a, int64_t row, int 
   for (int e = 0; e < E; ++e) am = umax(am, magnitude(v[e]));
   am = max_quad(am);
   if constexpr (LPB == 8) am = umax(am, (uint32_t)__builtin_amdgcn_mov_dpp((int)am, 0x141, 0xF, 0xF, true));
+  if constexpr (OUT == kNormE4M3) {
+    const BlockScale b = block_scale<MX_E4M3, true>(am);
+    if (piece * E >= (a.H + 31) / 32 * 32) return;
+    uint8_t* const q = (uint8_t*)a.y + row * a.y_ld + piece * E;
+    if constexpr (E == 8) *(u2*)q = (u2){encode4<MX_E4M3>(v[0], v[1], v[2], v[3], b.scale), encode4<MX_E4M3>(v[4], v[5], v[6], v[7], b.scale)};
+    else *(uint32_t*)q = encode4<MX_E4M3>(v[0], v[1], v[2], v[3], b.scale);
+    if (piece % LPB == 0) a.s[row * a.s_ld + piece / LPB] = (uint8_t)b.byte;
+    return;
+  }
   encode_block<E>(v, am, a.fmt, a.scale_mode, code, byte);
   if (piece * E >= (a.H + 31) / 32 * 32) return;
   uint8_t* const q = (uint8_t*)a.y + row * a.y_ld + (a.fmt == MX_E2M1 ? piece * E / 2 : piece * E);
@@ -75,13 +88,15 @@ __device__ __forceinline__ void store_codes(const NormArgs& a, int64_t row, int 
 }
 
 // GT threads to a row, S * 8 elements to a thread
-template <int T, int S, int GT, bool CODES>
-__global__ __launch_bounds__(GT < 256 ? 256 : GT) void norm_kernel(const NormArgs a) {
-  constexpr int E = kPiece<T>, V = S * 8 / E, WG = GT < 256 ? 256 : GT, GPW = WG / GT;
+template <int T, int S, int GT, int OUT>
+__global__ __launch_bounds__(GT == 64 ? 256 : GT) void norm_kernel(const NormArgs a) {
+  constexpr bool CODES = OUT != kNormFloats;
+  constexpr int E = kPiece<T>, V = S * 8 / E, WG = GT == 64 ? 256 : GT, GPW = WG / GT;
   __shared__ float red[GT > 64 ? 2 * GT / 64 : 1];
   const int t = threadIdx.x % GT, H = a.H;
   const float count = (float)H;
   int slot = 0;
+  if constexpr (OUT == kNormE4M3) saturate_conversions();
   float w[V][E], b[V][E];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -100,7 +115,7 @@ __global__ __launch_bounds__(GT < 256 ? 256 : GT) void norm_kernel(const NormArg
   const int64_t step = (int64_t)gridDim.x * GPW;
   int64_t row = (int64_t)blockIdx.x * GPW + threadIdx.x / GT;
   load(row, raw);
-  for (; row < a.rows; row += step) {                  // (rows of more than one wave: uniform over the workgroup)
+  for (; row < a.rows; row += step) {                  // (a row of more than one wave has the workgroup to itself: uniform)
     float v[V][E], sum[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -132,7 +147,7 @@ __global__ __launch_bounds__(GT < 256 ? 256 : GT) void norm_kernel(const NormArg
       const int at = (t + i * GT) * E;
 #pragma unroll
       for (int e = 0; e < E; ++e) v[i][e] = !CODES || at + e < H ? __builtin_fmaf(v[i][e] * rstd, w[i][e], b[i][e]) : 0.f;
-      if constexpr (CODES) store_codes<T>(a, row, t + i * GT, v[i]);
+      if constexpr (CODES) store_codes<T, OUT>(a, row, t + i * GT, v[i]);
       else store_piece<T>((uint8_t*)a.y + row * a.y_ld * kSize<T>, at, H - at, pack_piece<T>(v[i]));
     }
   }
@@ -140,13 +155,15 @@ __global__ __launch_bounds__(GT < 256 ? 256 : GT) void norm_kernel(const NormArg
 
 // rows that do not fit into a workgroup's registers: read three times, from L2 after the first
 constexpr int kLongThreads = 1024;
-template <int T, bool CODES>
+template <int T, int OUT>
 __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(const NormArgs a) {
+  constexpr bool CODES = OUT != kNormFloats;
   constexpr int E = kPiece<T>;
   __shared__ float red[2 * kLongThreads / 64];
   const int H = a.H, pieces = ((H + 31) / 32 * 32) / E;
   const float count = (float)H;
   int slot = 0;
+  if constexpr (OUT == kNormE4M3) saturate_conversions();
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const uint8_t* const x = (const uint8_t*)a.x + row * a.x_ld * kSize<T>;
     float sum[1] = {0.f}, v[E];
@@ -181,7 +198,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(const NormArgs 
       load_floats<E>(a.b, a.b_dtype, (int64_t)p * E, n, 0.f, b);
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = e < n ? __builtin_fmaf((v[e] - mean) * rstd, w[e], b[e]) : 0.f;
-      if constexpr (CODES) store_codes<T>(a, row, p, v);
+      if constexpr (CODES) store_codes<T, OUT>(a, row, p, v);
       else store_piece<T>((uint8_t*)a.y + row * a.y_ld * kSize<T>, (int64_t)p * E, n, pack_piece<T>(v));
     }
   }
@@ -331,6 +348,7 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(const NormBackwardArg
   const int H = a.H, at = ((int)blockIdx.x * 256 + threadIdx.x) * E, n = H - at;
   if (n <= 0) return;
   float dw[E] = {}, db[E] = {};
+#pragma unroll 4
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const float mean = a.mean[row], rstd = a.rstd[row];
     float x[E], d[E];
@@ -376,36 +394,42 @@ bool by_length(int64_t H, F&& f) {
   if (H <= MOST) { f(std::integral_constant<int, S>{}, std::integral_constant<int, GT>{}); return true; }
   MX_CASE(512, 1, 64)
   MX_CASE(1024, 2, 64)
-  MX_CASE(2048, 4, 64)
+  MX_CASE(2048, 2, 128)
   MX_CASE(4096, 2, 256)
-  MX_CASE(8192, 4, 256)
+  MX_CASE(8192, 2, 512)
   MX_CASE(16384, 2, 1024)
-  MX_CASE(32768, 4, 1024)
 #undef MX_CASE
   return false;
 }
 
-template <int T, bool CODES>
+template <int T, int OUT>
 hipError_t run_norm(const NormArgs& a, hipStream_t stream) {
   hipError_t e = hipSuccess;
   const int64_t cus = num_cus();
   const bool held = by_length((a.H + 31ll) / 32 * 32, [&](auto s, auto gt) {
-    constexpr int S = decltype(s)::value, GT = decltype(gt)::value, WG = GT < 256 ? 256 : GT, GPW = WG / GT;
-    const int64_t blocks = std::min<int64_t>((a.rows + GPW - 1) / GPW, cus * (2048 / WG));
-    e = launch_kernel(norm_kernel<T, S, GT, CODES>, dim3((unsigned)blocks), dim3(WG), 0, stream, a);
+    constexpr int S = decltype(s)::value, GT = decltype(gt)::value, WG = GT == 64 ? 256 : GT, GPW = WG / GT;
+    const auto kern = norm_kernel<T, S, GT, OUT>;
+    static int held = 0;                               // workgroups that a CU holds at once (benign race: always the same)
+    if (!held && (hipOccupancyMaxActiveBlocksPerMultiprocessor(&held, kern, WG, 0) != hipSuccess || held < 1)) held = 1;
+    // as many rows to every workgroup: 1531 rows of 8192 in 511 workgroups of three instead of 1024 of one or two
+    const int64_t groups = (a.rows + GPW - 1) / GPW, rounds = (groups + cus * held - 1) / (cus * held);
+    e = launch_kernel(kern, dim3((unsigned)((groups + rounds - 1) / rounds)), dim3(WG), 0, stream, a);
   });
-  if (!held) e = launch_kernel(norm_long_kernel<T, CODES>, dim3((unsigned)std::min<int64_t>(a.rows, 2 * cus)), dim3(kLongThreads), 0, stream, a);
+  if (!held) e = launch_kernel(norm_long_kernel<T, OUT>, dim3((unsigned)std::min<int64_t>(a.rows, 2 * cus)), dim3(kLongThreads), 0, stream, a);
   return e;
 }
 
-constexpr int64_t kBackHeld = 16384;                   // longest row of norm_backward_kernel
+// Longest row of norm_backward_kernel.  (fp32 rows beyond 8192 do not fit into registers: 2048 x 16384 took 170 us so.)
+template <int T> constexpr int64_t kBackHeld = T == MX_F32 ? 8192 : 16384;
 int64_t back_parts(int64_t rows, int64_t H) {
-  const int64_t per = H <= 2048 ? 8 : H <= 8192 ? 2 : 1;
+  const int64_t per = H <= 1024 ? 8 : H <= 2048 ? 4 : H <= 4096 ? 2 : 1;
   return std::min<int64_t>((rows + per - 1) / per, num_cus());
 }
+// partial sums of norm_columns_kernel: a thousand workgroups or two, eight rows at least to each
+int64_t column_parts(int64_t rows, int64_t H) { return std::min<int64_t>({back_parts(rows, H), (rows + 7) / 8, std::max<int64_t>(((int64_t)2 << 20) / H, 1)}); }
 template <int T>
 hipError_t run_backward(const NormBackwardArgs& a, hipStream_t stream) {
-  const int64_t parts = back_parts(a.rows, a.H);
+  const int64_t parts = a.H <= kBackHeld<T> ? back_parts(a.rows, a.H) : column_parts(a.rows, a.H);
   hipError_t e = hipSuccess;
   auto held = [&](auto s, auto gt) {
     constexpr int S = decltype(s)::value, GT = decltype(gt)::value;
@@ -414,11 +438,12 @@ hipError_t run_backward(const NormBackwardArgs& a, hipStream_t stream) {
   using std::integral_constant;
   if (a.H <= 512) held(integral_constant<int, 1>{}, integral_constant<int, 64>{});
   else if (a.H <= 1024) held(integral_constant<int, 2>{}, integral_constant<int, 64>{});
-  else if (a.H <= 2048) held(integral_constant<int, 4>{}, integral_constant<int, 64>{});
+  else if (a.H <= 2048) held(integral_constant<int, 2>{}, integral_constant<int, 128>{});
   else if (a.H <= 4096) held(integral_constant<int, 2>{}, integral_constant<int, 256>{});
-  else if (a.H <= 8192) held(integral_constant<int, 4>{}, integral_constant<int, 256>{});
-  else if (a.H <= kBackHeld) held(integral_constant<int, 4>{}, integral_constant<int, 512>{});
-  else {
+  else if (a.H <= 8192) held(integral_constant<int, 2>{}, integral_constant<int, 512>{});
+  else if (a.H <= kBackHeld<T>) {
+    if constexpr (T != MX_F32) held(integral_constant<int, 4>{}, integral_constant<int, 512>{});
+  } else {
     if (a.dx) e = launch_kernel(norm_backward_long_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 2 * num_cus())), dim3(kLongThreads), 0, stream, a);
     if (e == hipSuccess && (a.dw || a.db)) {
       const int64_t per = 256 * kPiece<T>;
@@ -433,9 +458,10 @@ hipError_t run_backward(const NormBackwardArgs& a, hipStream_t stream) {
 
 int launch_layer_norm(const NormArgs& a, hipStream_t stream) {
   if (a.rows <= 0) return MX_OK;
+  const bool e4m3 = a.fmt == MX_E4M3 && a.scale_mode != 0;
   hipError_t e = hipSuccess;
 #define MX_CASE(T) \
-  if (a.x_dtype == T) e = a.fmt < 0 ? run_norm<T, false>(a, stream) : run_norm<T, true>(a, stream);
+  if (a.x_dtype == T) e = a.fmt < 0 ? run_norm<T, kNormFloats>(a, stream) : e4m3 ? run_norm<T, kNormE4M3>(a, stream) : run_norm<T, kNormCodes>(a, stream);
   MX_CASE(MX_F32)
   MX_CASE(MX_BF16)
   MX_CASE(MX_F16)
