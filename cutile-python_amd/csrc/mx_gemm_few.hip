@@ -123,6 +123,16 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, co
     load(s + 2, t[0]);
     multiply(t[1]);
   }
+  // (a linear layer's epilogue: a wave takes one pair of tiles, whose bias and residual are on their way meanwhile)
+  constexpr bool LINEAR = std::is_same<Out, LinearOut>::value;
+  FloatsPiece bias = {}, res = {};
+  const int row_l = m0 + 16 * (wave >> 1) + r, col_l = 64 * u + 32 * (wave & 1) + 8 * gq;
+  if constexpr (LINEAR) {
+    if (wave < 2 * MT) {
+      if (o.bias) request_floats(o.bias, o.bias_dtype, col_l, a.N - col_l, bias);
+      linear_request(o, res, row_l, col_l, a.N - col_l, row_l < a.M);
+    }
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -130,6 +140,17 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, co
     for (int j = 0; j < 4; ++j) red[((wave * MT + i) * 4 + j) * 64 + lane] = acc[i][j];
   __syncthreads();
   // ---- the ranges of K, added in their order -----------------------------------------------------------------------
+  if constexpr (LINEAR) {
+    if (wave >= 2 * MT) return;
+    v4f v[2] = {};
+    for (int k = 0; k < kFewWaves; ++k)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) v[j] += red[((k * MT + (wave >> 1)) * 4 + 2 * (wave & 1) + j) * 64 + lane];
+    float b[8] = {};
+    if (o.bias) floats_of(bias, o.bias_dtype, b);
+    linear_finish_any<true>(o, v[0], v[1], b, res, row_l, col_l, a.N - col_l, row_l < a.M, gq == 0);
+    return;
+  }
   if (wave >= MT) return;
   const int row = m0 + 16 * wave + r;
   v4f v[4] = {};
@@ -138,14 +159,6 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const FewArgs a, co
     for (int j = 0; j < 4; ++j) v[j] += red[((k * MT + wave) * 4 + j) * 64 + lane];
   if constexpr (GATED) {
     gated_store(o, v, row, 32 * u + 8 * gq, row < a.M, gq == 0);
-  } else if constexpr (std::is_same<Out, LinearOut>::value) {
-#pragma unroll 1
-    for (int p = 0; p < 2; ++p) {
-      const int n = 64 * u + 32 * p + 8 * gq;
-      float bias[8];
-      linear_bias(o, n, bias);
-      linear_finish_any<true>(o, p ? v[2] : v[0], p ? v[3] : v[1], bias, row, n, a.N - n, row < a.M, gq == 0);
-    }
   } else {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {

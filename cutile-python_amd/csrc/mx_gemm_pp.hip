@@ -695,7 +695,7 @@ __global__ __launch_bounds__(256) void pp_tail_kernel(const GemmArgs g, const Ga
         const int col = n + 32 * jp;
         float bias[8];
         linear_bias(gate, col, bias);
-        ResidualPiece res = {};
+        FloatsPiece res = {};
         linear_request(gate, res, m, col, g.N - col, m < g.M);
         linear_finish<Gate::KIND, true>(gate, v[2 * jp], v[2 * jp + 1], bias, res, m, col, g.N - col, m < g.M, gq == 0);
       }

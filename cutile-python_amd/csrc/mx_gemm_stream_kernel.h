@@ -64,6 +64,26 @@ __global__ __launch_bounds__(C::WAVES * 64) void stream_kernel(const StreamArgs 
   v4f acc[MT][NT];
   stream_products<C>(w, smem + wave * C::WAVE_BYTES, xvo, xso, wvo, wso, j0, Q0, Q1, (a.K + 127) / 128, acc);
 
+  // item = (unit, row tile, tile pair) of the workgroup; lane (c, g) of tile j holds row c, columns
+  // bperm_tile_off(j) + 8 g .. + 3 of the group, so a pair of tiles is 8 consecutive outputs of a lane
+  constexpr int JP = NT >= 2 ? 2 : 1;
+  auto item = [&](int it, int& m, int& n) {
+    const int jp = it % (NT / JP), i = it / (NT / JP) % MT, t0 = (unit0 * nwv + it / (NT / JP) / MT) * NT + jp * JP;   // t0: first tile of the item
+    n = 64 * (t0 / 4) + bperm_tile_off(t0 % 4) + 8 * gq;
+    m = m0 + 16 * i + r;
+  };
+  // a linear layer's bias and residual of the wave's first item (as a rule its only one) are on their way while the K ranges meet
+  FloatsPiece bias = {}, res = {};
+  auto request = [&](int it) {
+    if constexpr (LINEAR) {
+      int m, n;
+      item(it, m, n);
+      if (o.bias) request_floats(o.bias, o.bias_dtype, n, a.N - n, bias);
+      linear_request(o, res, m, n, a.N - n, m < a.M);
+    }
+  };
+  if (wave < nwv * MT * (NT / JP)) request(wave);
+
   // ---- the K ranges meet in LDS, added in their order ------------------------------------------------------------
   __syncthreads();
   typedef __attribute__((address_space(3))) v4f lds_v4f;
@@ -73,23 +93,21 @@ __global__ __launch_bounds__(C::WAVES * 64) void stream_kernel(const StreamArgs 
 #pragma unroll
     for (int j = 0; j < NT; ++j) red[((nw * a.kw + kq) * (MT * NT) + i * NT + j) * 64 + lane] = acc[i][j];
   __syncthreads();
-  // item = (unit, row tile, tile pair) of the workgroup; lane (c, g) of tile j holds row c, columns
-  // bperm_tile_off(j) + 8 g .. + 3 of the group, so a pair of tiles is 8 consecutive outputs of a lane
-  constexpr int JP = NT >= 2 ? 2 : 1;
   for (int it = wave; it < nwv * MT * (NT / JP); it += C::WAVES) {   // uniform per wave
     const int jp = it % (NT / JP), i = it / (NT / JP) % MT, wv = it / (NT / JP) / MT;
     v4f v[2] = {};
     for (int k = 0; k < a.kw; ++k)
 #pragma unroll
       for (int h = 0; h < JP; ++h) v[h] += red[((wv * a.kw + k) * (MT * NT) + i * NT + jp * JP + h) * 64 + lane];
-    const int t0 = (unit0 * nwv + wv) * NT + jp * JP;                     // first tile of the item
-    const int n = 64 * (t0 / 4) + bperm_tile_off(t0 % 4) + 8 * gq, m = m0 + 16 * i + r;
+    int m, n;
+    item(it, m, n);
     int cols = a.N - n;
     if (JP == 1 && cols > 4) cols = 4;
     if constexpr (LINEAR) {
-      float bias[8];
-      linear_bias(o, n, bias);
-      linear_finish_any<true>(o, v[0], v[1], bias, m, n, cols, m < a.M, gq == 0);
+      float b[8] = {};
+      if (o.bias) floats_of(bias, o.bias_dtype, b);
+      linear_finish_any<true>(o, v[0], v[1], b, res, m, n, cols, m < a.M, gq == 0);
+      if (it + C::WAVES < nwv * MT * (NT / JP)) request(it + C::WAVES);
     } else if (m < a.M && cols > 0) {
       if (a.c_dtype == MX_F32) {
         float* p = (float*)a.C + (int64_t)m * a.ldc + n;

@@ -380,11 +380,19 @@ __device__ __forceinline__ void t128_tile(const T128Args& g, lds_u8* const smem,
     float bias[NT / 2][8];
 #pragma unroll
     for (int jp = 0; jp < NT / 2; ++jp) linear_bias(out, n + 32 * jp, bias[jp]);
+    FloatsPiece res[2] = {};   // (the residual is asked for one of them ahead)
+    auto request = [&](int i, int jp) {
+      const int64_t row = m0 + wm0 + 16 * i + r;
+      linear_request(out, res[1], row, n + 32 * jp, cols - 32 * jp, i < MT && row < g.M);
+    };
+    request(0, 0);
 #pragma unroll 1
     for (int i = 0; i < MT; ++i) {
       const int64_t row = m0 + wm0 + 16 * i + r;
 #pragma unroll 1
       for (int jp = 0; jp < NT / 2; ++jp) {
+        res[0] = res[1];
+        request(jp + 1 < NT / 2 ? i : i + 1, jp + 1 < NT / 2 ? jp + 1 : 0);
         v4f lo = acc[0][0], hi = acc[0][1];
         float b[8];
 #pragma unroll
@@ -395,7 +403,7 @@ __device__ __forceinline__ void t128_tile(const T128Args& g, lds_u8* const smem,
 #pragma unroll
           for (int e = 0; e < 8; ++e) b[e] = bias[NT / 2 - 1][e];
         }
-        linear_finish_any<true>(out, lo, hi, b, row, n + 32 * jp, cols - 32 * jp, row < g.M, gq == 0);
+        linear_finish_any<true>(out, lo, hi, b, res[0], row, n + 32 * jp, cols - 32 * jp, row < g.M, gq == 0);
       }
 #pragma unroll
       for (int k = 0; k + 1 < MT; ++k)

@@ -83,34 +83,38 @@ __device__ __forceinline__ float act_slope(float x, int act) {
   return __builtin_fmaf(c * s, (1.0f - s) * slope, s);
 }
 
-// eight numbers of a row of the residual as they lie in memory (fp32: two pieces)
-struct ResidualPiece { u4 lo, hi; };
-__device__ __forceinline__ void linear_request(const LinearOut& o, ResidualPiece& r, int64_t row, int col, int cols, bool live) {
-  if (!o.res) return;
-  const int n = live ? cols : 0;
-  if (o.res_dtype == MX_F32) {
-    const float* const p = (const float*)o.res + row * o.r_ld;
-    r.lo = load_piece<MX_F32>(p, col, n);
-    r.hi = load_piece<MX_F32>(p, col + 4, n - 4);
+// eight numbers of a row as they lie in memory (fp32: two pieces), to be asked for ahead of their use
+struct FloatsPiece { u4 lo, hi; };
+__device__ __forceinline__ void request_floats(const void* p, int dtype, int64_t at, int n, FloatsPiece& r) {
+  if (dtype == MX_F32) {
+    r.lo = load_piece<MX_F32>(p, at, n);
+    r.hi = load_piece<MX_F32>(p, at + 4, n - 4);
   } else {
-    r.lo = load_piece<MX_BF16>((const uint16_t*)o.res + row * o.r_ld, col, n);
+    r.lo = load_piece<MX_BF16>(p, at, n);
   }
 }
-__device__ __forceinline__ void linear_add(const LinearOut& o, const ResidualPiece& p, float (&v)[8]) {
-  if (!o.res) return;
-  if (o.res_dtype == MX_F32) {
+__device__ __forceinline__ void floats_of(const FloatsPiece& p, int dtype, float (&v)[8]) {
+  if (dtype == MX_F32) {
     float x[4], y[4];
     unpack_piece<MX_F32>(p.lo, x);
     unpack_piece<MX_F32>(p.hi, y);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] += x[e]; v[4 + e] += y[e]; }
+    for (int e = 0; e < 4; ++e) { v[e] = x[e]; v[4 + e] = y[e]; }
+  } else if (dtype == MX_BF16) {
+    unpack_piece<MX_BF16>(p.lo, v);
   } else {
-    float r[8];
-    if (o.res_dtype == MX_BF16) unpack_piece<MX_BF16>(p.lo, r);
-    else unpack_piece<MX_F16>(p.lo, r);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += r[e];
+    unpack_piece<MX_F16>(p.lo, v);
   }
+}
+__device__ __forceinline__ void linear_request(const LinearOut& o, FloatsPiece& r, int64_t row, int col, int cols, bool live) {
+  if (o.res) request_floats((const uint8_t*)o.res + row * o.r_ld * (o.res_dtype == MX_F32 ? 4 : 2), o.res_dtype, col, live ? cols : 0, r);
+}
+__device__ __forceinline__ void linear_add(const LinearOut& o, const FloatsPiece& p, float (&v)[8]) {
+  if (!o.res) return;
+  float r[8];
+  floats_of(p, o.res_dtype, r);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += r[e];
 }
 
 // scale of the block that four lanes hold (LANES16: l ^ 16, l ^ 32, else 4 n .. 4 n + 3), and its byte
@@ -127,7 +131,7 @@ __device__ __forceinline__ float linear_scale(const float (&v)[8], uint32_t& byt
 // Columns col .. col + 7 of row `row`, of which `cols` (1 to 8; anything less: none) exist; a, b: the product.  live: the row exists.
 // With codes four lanes hold a block's 32 columns, scale_lane one of them.
 template <int KIND, bool LANES16>
-__device__ __forceinline__ void linear_finish(const LinearOut& o, const v4f& a, const v4f& b, const float (&bias)[8], const ResidualPiece& res, int64_t row, int col,
+__device__ __forceinline__ void linear_finish(const LinearOut& o, const v4f& a, const v4f& b, const float (&bias)[8], const FloatsPiece& res, int64_t row, int col,
                                               int cols, bool live, bool scale_lane) {
   const bool in = live && cols > 0;
   float v[8];
@@ -159,10 +163,8 @@ __device__ __forceinline__ void linear_finish(const LinearOut& o, const v4f& a, 
 }
 // the same with the kind chosen here, where one place finishes all that a wave has
 template <bool LANES16>
-__device__ __forceinline__ void linear_finish_any(const LinearOut& o, const v4f& a, const v4f& b, const float (&bias)[8], int64_t row, int col, int cols, bool live,
-                                                  bool scale_lane) {
-  ResidualPiece res = {};
-  linear_request(o, res, row, col, cols, live);
+__device__ __forceinline__ void linear_finish_any(const LinearOut& o, const v4f& a, const v4f& b, const float (&bias)[8], const FloatsPiece& res, int64_t row, int col,
+                                                  int cols, bool live, bool scale_lane) {
   if (o.act == MX_ACT_GELU) linear_finish<kActErf, LANES16>(o, a, b, bias, res, row, col, cols, live, scale_lane);
   else if (o.act == MX_ACT_SILU || o.act == MX_ACT_GELU_TANH) linear_finish<kActSigmoid, LANES16>(o, a, b, bias, res, row, col, cols, live, scale_lane);
   else linear_finish<kActPlain, LANES16>(o, a, b, bias, res, row, col, cols, live, scale_lane);

@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void linear_pass_kernel(const float* product, 
     }
   float bias[8];
   linear_bias(o, col, bias);
-  ResidualPiece res = {};
+  FloatsPiece res = {};
   linear_request(o, res, row, col, cols, row < M);
   linear_finish<KIND, false>(o, a, b, bias, res, row, col, cols, row < M, (threadIdx.x & 3) == 0);
 }
