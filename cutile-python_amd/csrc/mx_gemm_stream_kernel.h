@@ -8,11 +8,11 @@ namespace {
 
 // Workgroup of C::WAVES waves: kw K ranges x WAVES / kw units of NT tiles.  m_tiles row tiles of 16 MT rows are neighbours in
 // dispatch order on the same XCD (workgroup ids go round-robin over 8 XCDs), so W is read from memory once.
-// Out: Ungated (C) or LinearOut: bias, activation and residual of a linear layer (mx_linear.h; NT of 2 or 4, so that a lane has eight columns).
+// Out: Ungated (C) or LinearOut: bias, activation and residual of a linear layer (mx_linear.h; not with NT of 1 where
+// the result is quantised: a lane has four columns then, a workgroup perhaps sixteen).
 template <class C, class Out>
 __global__ __launch_bounds__(C::WAVES * 64) void stream_kernel(const StreamArgs a, const Out o) {
   constexpr bool LINEAR = std::is_same<Out, LinearOut>::value;
-  static_assert(!LINEAR || C::NT >= 2, "");
   constexpr int NT = C::NT, MT = C::MT;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem_generic[];
   lds_u8* const smem = (lds_u8*)smem_generic;
@@ -78,8 +78,9 @@ __global__ __launch_bounds__(C::WAVES * 64) void stream_kernel(const StreamArgs 
     if constexpr (LINEAR) {
       int m, n;
       item(it, m, n);
-      if (o.bias) request_floats(o.bias, o.bias_dtype, n, a.N - n, bias);
-      linear_request(o, res, m, n, a.N - n, m < a.M);
+      const int cols = JP == 1 && a.N - n > 4 ? 4 : a.N - n;
+      if (o.bias) request_floats(o.bias, o.bias_dtype, n, cols, bias);
+      linear_request(o, res, m, n, cols, m < a.M);
     }
   };
   if (wave < nwv * MT * (NT / JP)) request(wave);

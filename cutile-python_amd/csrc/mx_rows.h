@@ -18,6 +18,10 @@ __device__ __forceinline__ u4 load_piece(const void* row, int64_t at, int n) {
   if (n >= kPiece<T>) {
     const u4_any v = *(const u4_any*)p;
     r = (u4){v[0], v[1], v[2], v[3]};
+  } else if (kPiece<T> == 8 && n == 4) {
+    const u2_any v = *(const u2_any*)p;
+    r[0] = v[0];
+    r[1] = v[1];
   } else if (n > 0) {
 #pragma unroll
     for (int e = 0; e < kPiece<T>; ++e) {

@@ -91,13 +91,21 @@ CASES = [
     ("auto", "e4m3", "e2m1", 1300, 512, 1120, f32, None, "relu"),
     ("auto", "e4m3", "e4m3", 1531, 2048, 1088, bf16, bf16, "gelu"),
     ("auto", "e4m3", "e4m3", 200, 12288, 256, bf16, bf16, "silu"),
+    ("auto", "e4m3", "e2m1", 17, 8192, 24640, bf16, bf16, "gelu"),  # many weights
     ("stream", "e4m3", "e4m3", 1, 128, 32, bf16, bf16, "gelu"),
     ("stream", "e4m3", "e4m3", 17, 1152, 97, f32, bf16, "gelu_tanh"),
     ("stream", "e4m3", "e2m1", 64, 4224, 160, None, f32, "silu"),
     ("stream", "e5m2", "e5m2", 33, 640, 1000, bf16, None, "relu"),
     ("stream", "e4m3", "e4m3", 100, 2048, 2944, bf16, bf16, None),
+    ("stream", "e4m3", "e4m3", 2, 2048, 4099, f16, f32, "gelu"),   # units of sixteen columns where the result is not quantised
+    ("stream", "e4m3", "e2m1", 16, 1024, 4096, bf16, bf16, "silu"),
     ("decode", "e4m3", "e2m1", 20, 1024, 9248, bf16, bf16, "gelu"),
     ("decode", "e4m3", "e2m1", 31, 512, 224, f32, None, "silu"),
+    ("decode", "e4m3", "e2m1", 7, 8192, 96, f16, f32, "gelu"),
+    ("decode", "e4m3", "e2m1", 32, 4608, 16480, bf16, bf16, "gelu_tanh"),
+    ("decode", "e4m3", "e2m1", 16, 1536, 16416, None, f16, "relu"),
+    ("decode", "e4m3", "e2m1", 5, 512, 48, bf16, bf16, "gelu"),
+    ("decode", "e4m3", "e2m1", 40, 512, 64, bf16, bf16, None),
     ("mfma128", "e4m3", "e4m3", 1, 32, 64, bf16, None, "gelu"),
     ("mfma128", "e4m3", "e4m3", 257, 544, 192, f32, bf16, "gelu_tanh"),
     ("mfma128", "e2m1", "e2m1", 300, 1536, 450, bf16, f16, "silu"),
@@ -149,7 +157,8 @@ def test_product_with_epilogue(ct, dev, kernel, af, wf, M, K, N, bt, rt, act):
 
 
 @pytest.mark.parametrize("act", ACTS)
-@pytest.mark.parametrize("kernel,M,K,N", [("stream", 20, 256, 96), ("mfma128", 200, 288, 160), ("pingpong", 300, 544, 288), ("auto", 300, 512, 96), ("generic", 9, 64, 32)])
+@pytest.mark.parametrize("kernel,M,K,N", [("stream", 20, 256, 96), ("stream", 1, 512, 8192), ("mfma128", 200, 288, 160), ("pingpong", 300, 544, 288), ("auto", 300, 512, 96),
+                                          ("generic", 9, 64, 32)])
 def test_every_activation_everywhere(ct, dev, kernel, M, K, N, act):
     """Arguments from -40 to 40, by way of the bias; every row the same product."""
     a, w = randn_operand(1, K, O.E4M3, K, dev), randn_operand(N, K, O.E4M3, N, dev, std=K ** -0.5)
