@@ -68,11 +68,11 @@ __device__ __forceinline__ void activate(float (&v)[8], int act) {
   }
 }
 // the activation's derivative (d/dx x s(f(x)) = s + x f'(x) s (1 - s); d/dx x P = P + x exp(-x^2 / 2) / sqrt(2 pi)); NaN for NaN
+template <int KIND>
 __device__ __forceinline__ float act_slope(float x, int act) {
-  if (act == MX_ACT_NONE) return 1.0f;
-  if (act == MX_ACT_RELU) return x > 0.f ? 1.0f : x <= 0.f ? 0.f : x;
+  if constexpr (KIND == kActPlain) return x > 0.f ? 1.0f : x <= 0.f ? 0.f : x;   // (relu: with no activation nobody asks)
   const float c = __builtin_amdgcn_fmed3f(x, -126.0f, 126.0f), x2 = x * x;
-  if (act == MX_ACT_GELU) {
+  if constexpr (KIND == kActErf) {
     const float q = upper_tail(__builtin_fabsf(x), x2);
     return __builtin_fmaf(c, 0.3989422804f * __builtin_amdgcn_exp2f(x2 * (-0.5f * kLog2E)), x > 0.f ? 1.0f - q : q);
   }

@@ -362,6 +362,7 @@ int mx_linear_backward(const mx_tensor* dy, const void* saved, int64_t saved_byt
   if (dbias)
     if (int rc = check_vector(dbias, "dbias", s.N)) return rc;
   if (int rc = check_mode(scale_mode)) return rc;
+  if (s.T > 1 && dy->stride[0] > (int64_t)1 << 25) return set_error(MX_ERR_LAYOUT, "dy: rows lie more than 2^25 elements apart");
   if (s.T == 0) return set_error(MX_ERR_SHAPE, "mx_linear_backward: no tokens (the gradients of w and bias are zeros)");
   if (int rc = check_size(s)) return rc;
   if (int rc = check_room("saved", saved, saved_bytes, mx_linear_saved_bytes(s.T, s.K, s.N, activation))) return rc;

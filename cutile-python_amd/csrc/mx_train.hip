@@ -616,12 +616,19 @@ __global__ __launch_bounds__(512, 4) void silu_backward_kernel(const SiluBackwar
 // rows (the bias's gradient).  Bound: memory, 4 bytes read and 2.06 written an element.  Tiles, exchanges and layouts are those of
 // quantize_both_kernel; a column's sum is the lane's eight rows, then lanes l ^ 16, l ^ 32, the four waves, and the tiles by a second launch,
 // always in this order.
-template <int SRC, bool PRE, bool FLOOR>
-__global__ __launch_bounds__(256) void act_backward_kernel(const ActBackwardArgs a) {
+// Four workgroups to a CU: 128 registers, in which the tile as it was read and its values fit if the lanes' addresses are one offset from
+// uniform ones (4096 x 4096, silu: 47.7 us with 161 registers, 30.2 so; 100 MB).  What a NaN or, under the ceiling rule, an infinity makes of its block
+// needs no other code here: it is NaN itself, or its block's scale is.
+// KIND: of the activation (mx_linear.h), kNoAct: none.  (One instance for all of them is 64 copies of every derivative: 77 x 4096, hardly more
+// than one workgroup's latency, took 12.9 us, most of it for instructions to arrive; 8.5 so.)
+constexpr int kNoAct = -1;
+template <int SRC, int KIND, bool FLOOR>
+__global__ __launch_bounds__(256, 4) void act_backward_kernel(const ActBackwardArgs a) {
+  constexpr bool PRE = KIND != kNoAct;
   __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
   __shared__ uint32_t srow[128], scol[128];
   __shared__ float sums[4][128];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, rg = lane >> 4, cg = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), rg = lane >> 4, cg = lane & 15;
   uint32_t tr, tk;
   tile_of<2, true>(blockIdx.x, a.tiles, a.tiles_k, tr, tk);
   const int64_t r0 = (int64_t)tr * 128, k0 = (int64_t)tk * 128, rows = a.rows, N = a.N, Rpad = (rows + 31) / 32 * 32;
@@ -631,18 +638,25 @@ __global__ __launch_bounds__(256) void act_backward_kernel(const ActBackwardArgs
     for (int i = tid; i < 512; i += 256) sums[i >> 7][i & 127] = 0.f;
     __syncthreads();
   }
-  if (inside && r0 + 32 * wave < rows) {               // (waves without rows have nothing to do)
-    const int64_t row = r0 + 32 * wave + 8 * rg, col = k0 + 8 * cg;   // of the lane's first element
-    const bool col_in = col < N;
+  const int64_t w0 = r0 + 32 * wave;                   // the wave's first row
+  if (inside && w0 < rows) {                           // (waves without rows have nothing to do)
+    const bool col_in = k0 + 8 * cg < N;
+    const int left = rows - w0 < 32 ? (int)(rows - w0) - 8 * rg : 8;   // of the lane's rows
     float v[8][8];
     u4 raw[8][SRC == MX_F32 ? 2 : 1], rp[8];
+    const uint8_t *const dy = (const uint8_t*)a.dy + (w0 * a.dy_ld + k0) * kSize<SRC>, *const pre = (const uint8_t*)(a.pre + w0 * a.pre_ld + k0);
+    const uint32_t dy_at = (uint32_t)(8 * rg * (int)a.dy_ld + 8 * cg) * kSize<SRC>, pre_at = (uint32_t)(8 * rg * (int)a.pre_ld + 8 * cg) * 2;
+    auto piece = [&](const uint8_t* row, uint32_t at, bool in) -> u4 {
+      u4_any x = {0, 0, 0, 0};
+      if (in) x = *(const u4_any*)(row + at);
+      return (u4){x[0], x[1], x[2], x[3]};
+    };
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool in = col_in && row + i < rows;
-      const uint8_t* const dy = (const uint8_t*)a.dy + (row + i) * a.dy_ld * kSize<SRC>;
-      raw[i][0] = load_piece<SRC>(dy, col, in ? 8 : 0);
-      if constexpr (SRC == MX_F32) raw[i][1] = load_piece<SRC>(dy, col + 4, in ? 4 : 0);
-      if constexpr (PRE) rp[i] = load_piece<MX_BF16>(a.pre + (row + i) * a.pre_ld, col, in ? 8 : 0);
+      const bool in = col_in && i < left;
+      raw[i][0] = piece(dy + i * a.dy_ld * kSize<SRC>, dy_at, in);
+      if constexpr (SRC == MX_F32) raw[i][1] = piece(dy + i * a.dy_ld * 4 + 16, dy_at, in);
+      if constexpr (PRE) rp[i] = piece(pre + i * a.pre_ld * 2, pre_at, in);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -659,30 +673,29 @@ __global__ __launch_bounds__(256) void act_backward_kernel(const ActBackwardArgs
         float p[8];
         unpack_piece<MX_BF16>(rp[i], p);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] *= act_slope(p[e], a.act);
+        for (int e = 0; e < 8; ++e) v[i][e] *= act_slope<KIND>(p[e], a.act);
       }
     }
-    uint32_t most = 0;
+    auto scale_of = [&](uint32_t am) {
+      BlockScale b = block_scale<MX_E4M3, FLOOR>(am);
+      if constexpr (!FLOOR)
+        if (odd_block<FLOOR>(am)) b.byte = 0xFF;
+      return b;
+    };
     if (a.d) {
+      uint8_t* const d = a.d + w0 * a.d_ld + k0;
+      const uint32_t d_at = (uint32_t)(8 * rg * (int)a.d_ld + 8 * cg);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        uint32_t am = 0, c[2], byte;
+        uint32_t am = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) am = umax(am, magnitude(v[i][e]));
-        am = max_quad(am);
-        most = umax(most, am);
-        const BlockScale b = block_scale<MX_E4M3, FLOOR>(am);
-        c[0] = encode4<MX_E4M3>(v[i][0], v[i][1], v[i][2], v[i][3], b.scale);
-        c[1] = encode4<MX_E4M3>(v[i][4], v[i][5], v[i][6], v[i][7], b.scale);
-        byte = b.byte;
-        if (odd_block<FLOOR>(am)) encode_slow<8>(v[i], am, MX_E4M3, FLOOR, c, byte);
-        if (col_in && row + i < rows) *(u2*)(a.d + (row + i) * a.d_ld + col) = (u2){c[0], c[1]};
-        ((uint8_t*)srow)[(32 * wave + 8 * rg + i) * 4 + (cg >> 2)] = (uint8_t)byte;
+        const BlockScale b = scale_of(max_quad(am));
+        const u2 c = {encode4<MX_E4M3>(v[i][0], v[i][1], v[i][2], v[i][3], b.scale), encode4<MX_E4M3>(v[i][4], v[i][5], v[i][6], v[i][7], b.scale)};
+        if (col_in && i < left) *(u2*)(d + i * a.d_ld + d_at) = c;
+        ((uint8_t*)srow)[(32 * wave + 8 * rg + i) * 4 + (cg >> 2)] = (uint8_t)b.byte;
       }
     }
-    auto place = [&](int e, u2 c) {
-      *(u2*)(tile + (8 * cg + e) * 128 + (((2 * wave + (rg >> 1)) ^ (cg & 7)) << 4) + (rg & 1) * 8) = c;
-    };
     if (a.dt) {
       uint32_t m[8], own[2];
       float scale[2], s[8];
@@ -695,27 +708,15 @@ __global__ __launch_bounds__(256) void act_backward_kernel(const ActBackwardArgs
       max_columns(m, own);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        most = umax(most, own[e]);
-        const BlockScale b = block_scale<MX_E4M3, FLOOR>(own[e]);
+        const BlockScale b = scale_of(own[e]);
         scale[e] = b.scale;
         ((uint8_t*)scol)[(8 * cg + own_column(lane) + e) * 4 + wave] = (uint8_t)b.byte;
       }
       spread_columns(scale, s);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        place(e, (u2){encode4<MX_E4M3>(v[0][e], v[1][e], v[2][e], v[3][e], s[e]), encode4<MX_E4M3>(v[4][e], v[5][e], v[6][e], v[7][e], s[e])});
-      if (__builtin_amdgcn_ballot_w64(odd_block<FLOOR>(most))) {   // a wave with such a block does its columns again
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float w[8];
-          uint32_t c[2], byte;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = v[i][e];
-          encode_slow<8>(w, max_xor_16_32(m[e]), MX_E4M3, FLOOR, c, byte);
-          place(e, (u2){c[0], c[1]});
-          if (rg == 0) ((uint8_t*)scol)[(8 * cg + e) * 4 + wave] = (uint8_t)byte;
-        }
-      }
+        *(u2*)(tile + (8 * cg + e) * 128 + (((2 * wave + (rg >> 1)) ^ (cg & 7)) << 4) + (rg & 1) * 8) =
+            (u2){encode4<MX_E4M3>(v[0][e], v[1][e], v[2][e], v[3][e], s[e]), encode4<MX_E4M3>(v[4][e], v[5][e], v[6][e], v[7][e], s[e])};
     }
     if (a.partial) {
 #pragma unroll
@@ -864,21 +865,19 @@ int launch_act_backward(const ActBackwardArgs& args, hipStream_t stream) {
   if (blocks > 0x7FFFFFFF) return set_error(MX_ERR_SHAPE, "act_backward: tensor too large");
   a.tiles = (int32_t)blocks;
   hipError_t e = hipSuccess;
-#define MX_CASE(SRC, PRE, FLOOR) \
-  if (a.dy_dtype == SRC && (a.pre != nullptr) == PRE && (a.scale_mode != 0) == FLOOR) \
-    e = launch_kernel(act_backward_kernel<SRC, PRE, FLOOR>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
-  MX_CASE(MX_BF16, true, true)
-  MX_CASE(MX_BF16, true, false)
-  MX_CASE(MX_BF16, false, true)
-  MX_CASE(MX_BF16, false, false)
-  MX_CASE(MX_F32, true, true)
-  MX_CASE(MX_F32, true, false)
-  MX_CASE(MX_F32, false, true)
-  MX_CASE(MX_F32, false, false)
-  MX_CASE(MX_F16, true, true)
-  MX_CASE(MX_F16, true, false)
-  MX_CASE(MX_F16, false, true)
-  MX_CASE(MX_F16, false, false)
+  const int kind = a.pre ? act_kind(a.act) : kNoAct;
+  auto run = [&](auto src, auto k) {
+    constexpr int SRC = decltype(src)::value, KIND = decltype(k)::value;
+    e = a.scale_mode ? launch_kernel(act_backward_kernel<SRC, KIND, true>, dim3((unsigned)blocks), dim3(256), 0, stream, a)
+                     : launch_kernel(act_backward_kernel<SRC, KIND, false>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  };
+#define MX_CASE(SRC, KIND) \
+  if (a.dy_dtype == SRC && kind == KIND) run(std::integral_constant<int, SRC>{}, std::integral_constant<int, KIND>{});
+#define MX_CASES(SRC) MX_CASE(SRC, kNoAct) MX_CASE(SRC, kActPlain) MX_CASE(SRC, kActSigmoid) MX_CASE(SRC, kActErf)
+  MX_CASES(MX_BF16)
+  MX_CASES(MX_F32)
+  MX_CASES(MX_F16)
+#undef MX_CASES
 #undef MX_CASE
   if (e != hipSuccess) return set_error(MX_ERR_LAUNCH, "act_backward_kernel launch: %s", hipGetErrorString(e));
   return MX_OK;

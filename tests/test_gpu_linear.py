@@ -442,3 +442,26 @@ def test_gradient_that_is_not_finite(ct, dev):
         dx, dw, db = ct.linear_backward(dy, st)
         assert bool(dx[3].isnan().all()) and not bool(dx[[0, 1, 2, 4]].isnan().any())
         assert bool(dw[40].isnan().all()) and not bool(dw[:32].isnan().any()) and bool(db[40].isnan()) and int(db.isnan().sum()) == 1
+
+
+@pytest.mark.parametrize("mode", ["floor", "ceil"])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("T", [40, 600])
+def test_what_is_not_finite_stays_in_its_place(ct, dev, T, bad, mode):
+    """One element of dy: its row of dx, its row of dw and its column's sum are not finite (under the floor rule an infinity is the largest
+    number of its block); blocks that do not hold it give what they gave."""
+    x, w, b, dy, _ = make(dev, T, 96, 1024, f32, 15)
+    _, st = ct.linear_forward(x, w, b, activation="relu", scale_mode=mode)
+    clean = ct.linear_backward(dy, st)
+    n = int((x @ w.T + b)[5].argmax())                         # a column whose slope is one there
+    dy[5, n] = bad
+    dx, dw, db = ct.linear_backward(dy, st)
+    others = [t for t in range(T) if t != 5]
+    assert torch.equal(dx[others], clean[0][others])
+    blocks = [k for k in range(1024) if k != n]
+    assert torch.equal(dw[blocks], clean[1][blocks]) and torch.equal(db[blocks], clean[2][blocks])
+    assert not bool(db[n].isfinite())
+    if mode == "ceil" or bad != bad:
+        assert bool(dx[5].isnan().all()) and bool(dw[n].isnan().all())
+    else:
+        assert not torch.equal(dx[5], clean[0][5]) and not torch.equal(dw[n], clean[1][n])
