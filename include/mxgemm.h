@@ -438,8 +438,9 @@ MX_API int mx_ffn_backward(const mx_tensor* dy, const void* saved, int64_t saved
  * Sums as in mx_gemm (the scaled matrix instructions align an instruction's products with some 18 bits below the largest: 1.5e-5 of the
  * result's norm), everything behind them in 32 bits; the activation is within 2e-6 of its value.  act(-inf) is zero for gelu and silu;
  * a block of out with a NaN has mx_quantize's scale and zeros.
- * Operands that only the general kernel takes are refused unless opts->kernel is MX_KERNEL_GENERIC; the product then goes through the
- * workspace.  Workspace: mx_linear_gemm_workspace_bytes(); what mx_gemm_workspace_bytes calls optional is optional here.
+ * Fused into the streaming kernel, the 128 x 128 one and, for E4M3 A with E4M3 or E2M1 W and outputs in whole 16-byte pieces, the ping-pong
+ * one; with every other kernel (opts->kernel as in mx_gemm) the product goes through the workspace, some rows at a time.  residual may
+ * be out itself.  workspace: mx_linear_gemm_workspace_bytes(), all of it, aligned to 256 bytes.
  */
 MX_API int64_t mx_linear_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, const mx_gemm_opts* opts);
 MX_API int mx_linear_gemm(const mx_tensor* A, const mx_tensor* A_scale, const mx_tensor* W, const mx_tensor* W_scale, const mx_tensor* bias,
@@ -451,7 +452,8 @@ MX_API int mx_linear_gemm(const mx_tensor* A, const mx_tensor* A_scale, const mx
  *   forward   P = Q_r(x) Q_r(w)^T + bias;  y = act(P) + residual
  *   backward  d = dy act'(bf16(P));  dx = Q_r(d) Q_c(w);  dw = Q_c(d)^T Q_c(x);  dbias = sum over rows of d  (residual's gradient is dy)
  *   x [T,K], w [N,K], dy [T,N]: MX_F32, MX_BF16 or MX_F16; bias and residual as in mx_linear_gemm; y, dx, dw MX_F32 or MX_BF16; dbias
- *   [N] of any float type; rows contiguous; K and N multiples of 32; no operand (T x K, T x N, N x K) of 2^31 elements or more
+ *   [N] of any float type; rows contiguous, those of dy at most 2^25 elements apart; K and N multiples of 32; no operand (T x K, T x N, N x K) of
+ *   2^31 elements or more
  * Precision: with few tokens (up to 64, or T N up to 2^19) P is summed in 32 bits; with more, and in the other products, as in mx_linear_gemm.
  * `saved` (mx_linear_saved_bytes(), NULL where no backward pass will follow): Q_c(x), Q_c(w) and, with an activation, bf16(P).  The
  * backward pass reads it only, and neither x nor w.  Of dx, dw and dbias those that are not wanted may be NULL.  A T of zero is a valid
