@@ -172,10 +172,11 @@ __device__ __forceinline__ void linear_finish_any(const LinearOut& o, const v4f&
 
 // What a wave's row tiles of the ping-pong kernel leave by: everything through buffer descriptors, whose range takes the place of comparisons
 // with the last row; columns that are not there have an offset beyond it.  bf16 (CODES false) or E4M3 out, a bf16 residual, rows of
-// whole 16-byte pieces (codes: of 8), each tensor less than 2 GiB: linear_is_plain().
+// whole 16-byte pieces (codes: of 8), each tensor less than 2 GiB, the rows behind it that a tile reaches included (their offsets must not
+// come round): linear_is_plain().
 inline bool linear_is_plain(const LinearOut& o, int64_t M) {
   const int64_t lim = (int64_t)1 << 31;
-  auto fine = [&](const void* p, int64_t ld, int size, int align) { return !p || ((uintptr_t)p % align == 0 && ld * size % align == 0 && M * ld * size < lim); };
+  auto fine = [&](const void* p, int64_t ld, int size, int align) { return !p || ((uintptr_t)p % align == 0 && ld * size % align == 0 && (M + 256) * ld * size < lim); };
   return o.N % 8 == 0 && (o.c_fmt == MX_BF16 ? fine(o.c, o.c_ld, 2, 16) : o.c_fmt == MX_E4M3 && fine(o.c, o.c_ld, 1, 8) && fine(o.s, o.s_ld, 1, 1)) &&
          fine(o.pre, o.pre_ld, 2, 16) && (!o.res || (o.res_dtype == MX_BF16 && fine(o.res, o.r_ld, 2, 16)));
 }

@@ -292,6 +292,10 @@ int mx_linear_gemm(const mx_tensor* A, const mx_tensor* As, const mx_tensor* W, 
     l.pre = (uint16_t*)pre->ptr; l.pre_ld = pre->stride[0];
   }
   if (M == 0 || N == 0) return MX_OK;
+  if (M == 1) {   // (the pitch of one row is anything)
+    l.c_ld = l.pre_ld = l.r_ld = (N + 7) / 8 * 8;
+    l.s_ld = N / 32;
+  }
   o.accumulate = 0;
   if (int rc = check_room("workspace", workspace, workspace_bytes, linear_workspace(M, N, K, o))) return rc;
   return run_linear(*A, *As, *W, *Ws, l, o, workspace, workspace_bytes, (hipStream_t)stream);

@@ -128,6 +128,10 @@ CASES = [
     ("pingpong", "e4m3", "e4m3", 4200, 4096, 4128, bf16, bf16, "gelu"),
     ("auto", "e4m3", "e4m3", 1531, 8192, 1088, bf16, bf16, "relu"),
     ("mfma256", "e4m3", "e4m3", 300, 512, 320, bf16, bf16, "gelu"),
+    # through memory, some rows at a time
+    ("mfma256", "e2m1", "e2m1", 2305, 256, 2080, bf16, bf16, "gelu"),
+    ("pingpong32", "e4m3", "e4m3", 1500, 544, 4160, bf16, None, "silu"),
+    ("pingpong", "e5m2", "e5m2", 1100, 1024, 8200, None, bf16, "relu"),
     ("generic", "e4m3", "e4m3", 33, 96, 64, bf16, bf16, "gelu"),
     ("generic", "e2m1", "e4m3", 5, 64, 30, f32, f32, "silu"),
 ]
@@ -140,8 +144,8 @@ def test_product_with_epilogue(ct, dev, kernel, af, wf, M, K, N, bt, rt, act):
     p, want, err = definition(a, w, bias, res, act)
     kw = dict(activation=act, a_format=a.fmt_kw, w_format=w.fmt_kw, kernel=kernel)
     scales = [(a.scale_t, w.scale_t)]
-    if kernel in ("mfma128", "pingpong", "mfma256"):
-        scales.append((ct.pack_scales(a.scale_t, operand="a"), ct.pack_scales(w.scale_t, operand="b")))
+    if kernel in ("mfma128", "pingpong", "mfma256", "pingpong32"):
+        scales.append(tuple(ct.pack_scales(t.scale_t, operand=o, kernel=kernel) for t, o in ((a, "a"), (w, "b"))))
     elif kernel in ("auto", "stream") and K % 128 == 0:
         scales.append((a.scale_t, ct.pack_scales(w.scale_t, operand="b")))
     for a_s, w_s in scales:
@@ -255,6 +259,56 @@ def test_padded_outputs(ct, dev, kernel, M, K, N, out, offset):
         inner(s, 0, 0, 1)
     pre = ct.block_scaled_linear(a.storage, a.scale_t, w.storage, w.scale_t, bias, kernel=kernel)
     assert torch.equal(inner(p, M, N, 2, 1), u8(pre))
+
+
+def raw(ct, dev, kernel, a, w, bias, res, out, act=L.MX_ACT_GELU, pre=None):
+    """The C entry with views as they are."""
+    M, K, N = a.storage.shape[0], a.storage.shape[1], w.storage.shape[0]
+    o, lib = L.MxGemmOpts(struct_size=32, kernel=L.KERNELS[kernel], block_size=32), L.lib()
+    need = lib.mx_linear_gemm_workspace_bytes(M, N, K, ctypes.byref(o))
+    ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
+    ref = lambda t: None if t is None else ctypes.byref(L.desc(t, L._TORCH_TO_MX[t.dtype]))  # noqa: E731
+    rc = lib.mx_linear_gemm(ctypes.byref(L.desc(u8(a.storage), L.MX_E4M3)), ctypes.byref(L.desc(u8(a.scale_t), L.MX_E8M0)),
+                            ctypes.byref(L.desc(u8(w.storage), L.MX_E4M3)), ctypes.byref(L.desc(u8(w.scale_t), L.MX_E8M0)), ref(bias), ref(res), act, ref(out), None,
+                            ref(pre), ctypes.byref(o), ws.data_ptr(), need, L.stream_ptr(dev))
+    assert rc == L.MX_OK, L.last_error()
+
+
+@pytest.mark.parametrize("kernel", ["stream", "mfma128", "pingpong", "generic"])
+def test_one_row_of_any_pitch(ct, dev, kernel):
+    K, N = 256, 96
+    a, w = randn_operand(1, K, O.E4M3, 1, dev), randn_operand(N, K, O.E4M3, 2, dev)
+    bias, res = around(dev, 1, N, bf16, bf16, 3)
+    want = ct.block_scaled_linear(a.storage, a.scale_t, w.storage, w.scale_t, bias, res, activation="gelu", kernel=kernel)
+    pre = ct.block_scaled_linear(a.storage, a.scale_t, w.storage, w.scale_t, bias, kernel=kernel)
+    for pitch in (1, 8, 5 * N):
+        out, p = (torch.full((8 * N,), 7.0, dtype=bf16, device=dev) for _ in range(2))
+        raw(ct, dev, kernel, a, w, bias, res.as_strided((1, N), (pitch, 1)), out.as_strided((1, N), (pitch, 1)), pre=p.as_strided((1, N), (pitch, 1)))
+        assert torch.equal(out[:N], want[0]) and bool((out[N:] == 7).all())
+        assert torch.equal(p[:N], pre[0]) and bool((p[N:] == 7).all())
+
+
+@pytest.mark.parametrize("kernel", ["mfma128", "pingpong"])
+def test_rows_far_apart(ct, dev, kernel):
+    """Nine rows 2^26 numbers apart: 32 of such pitches are 2^32 bytes, where a tile's rows behind the last must not come round to."""
+    M, K, N, pitch = 9, 256, 128, (1 << 26)
+    a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(N, K, O.E4M3, 2, dev)
+    bias, res = around(dev, M, N, bf16, bf16, 3)
+    want = ct.block_scaled_linear(a.storage, a.scale_t, w.storage, w.scale_t, bias, res, activation="gelu", kernel=kernel)
+    far = torch.empty((M - 1) * pitch + N, dtype=bf16, device=dev).as_strided((M, N), (pitch, 1))
+    far.copy_(res)
+    raw(ct, dev, kernel, a, w, bias, far, far)                 # (the residual is the output itself)
+    assert torch.equal(far, want)
+
+
+@pytest.mark.parametrize("kernel,M,K,N", [("stream", 20, 256, 96), ("mfma128", 300, 288, 160), ("pingpong", 600, 544, 288), ("pingpong", 300, 4096, 320), ("generic", 9, 64, 32),
+                                          ("mfma256", 300, 256, 96)])
+def test_residual_in_place(ct, dev, kernel, M, K, N):
+    a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(N, K, O.E4M3, 2, dev)
+    bias, res = around(dev, M, N, f32, bf16, 3)
+    want = ct.block_scaled_linear(a.storage, a.scale_t, w.storage, w.scale_t, bias, res, activation="silu", kernel=kernel)
+    raw(ct, dev, kernel, a, w, bias, res, res, L.MX_ACT_SILU)
+    assert torch.equal(res, want)
 
 
 def test_empty(ct, dev):
