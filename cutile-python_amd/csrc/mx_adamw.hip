@@ -211,6 +211,25 @@ hipError_t launch(const AdamArgs& a, int64_t chunks, bool small, hipStream_t str
                : launch_kernel(adamw_kernel<P, G, false>, dim3((unsigned)chunks), dim3(kThreads), 0, stream, a);
 }
 
+typedef std::vector<std::pair<uintptr_t, uintptr_t>> Ranges;
+// (the lists are sorted and joined)
+bool overlap(Ranges (&lists)[6]) {
+  for (Ranges& l : lists)
+    if (!std::is_sorted(l.begin(), l.end())) std::sort(l.begin(), l.end());
+  std::sort(lists, lists + 6);   // by their first range, empty ones in front
+  Ranges all;
+  size_t total = 0;
+  for (const Ranges& l : lists) total += l.size();
+  all.reserve(total);
+  for (const Ranges& l : lists) {
+    const size_t mid = all.size();
+    all.insert(all.end(), l.begin(), l.end());
+    if (mid > 0 && mid < all.size() && all[mid] < all[mid - 1]) std::inplace_merge(all.begin(), all.begin() + mid, all.end());
+  }
+  for (size_t i = 1; i < all.size(); ++i)
+    if (all[i].first < all[i - 1].second) return true;
+  return false;
+}
 int check_adamw(int32_t count, const mx_adamw_tensor* list, const mx_adamw_opts& o) {
   if (o.state_bits != 8 && o.state_bits != 32) return set_error(MX_ERR_INVALID, "states have 8 or 32 bits (got %d)", o.state_bits);
   auto within = [](double x, double lo, double hi) { return x >= lo && x <= hi; };   // (not NaN)
@@ -221,7 +240,10 @@ int check_adamw(int32_t count, const mx_adamw_tensor* list, const mx_adamw_opts&
   if (!within(o.weight_decay, 0.0, 3e38)) return set_error(MX_ERR_INVALID, "the weight decay must be a number of at least zero (got %g)", o.weight_decay);
   if (!o.step_at && o.step < 1) return set_error(MX_ERR_INVALID, "steps are counted from 1 (got %lld)", (long long)o.step);
   if (!o.scale_at && !within(o.grad_scale, -3e38, 3e38)) return set_error(MX_ERR_INVALID, "the gradients' scale must be a number");
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  // What is written, a list for each kind: as a rule ascending, as its tensors were allocated.  (200 tensors: a step takes 28 us of host time, with
+  // all of it sorted at once 40.)
+  Ranges written[6];
+  for (int k = 0; k < (o.state_bits == 8 ? 6 : 4); ++k) written[k].reserve(count);
   for (int32_t i = 0; i < count; ++i) {
     const mx_adamw_tensor& t = list[i];
     if (t.n < 0) return set_error(MX_ERR_SHAPE, "tensor %d: negative extent", i);
@@ -236,22 +258,19 @@ int check_adamw(int32_t count, const mx_adamw_tensor* list, const mx_adamw_opts&
         ((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) % (small ? 8 : 4) || (uintptr_t)t.copy % 2)
       return set_error(MX_ERR_LAYOUT, "tensor %d: misaligned", i);
     const int64_t state = small ? round32(t.n) : t.n * 4;
-    auto writes = [&](const void* p, int64_t bytes) {
-      if (p) written.emplace_back((uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes);
+    auto writes = [&](int k, const void* p, int64_t bytes) {
+      if (p) written[k].emplace_back((uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes);
     };
-    writes(t.param, t.n * (t.param_dtype == MX_F32 ? 4 : 2));
-    writes(t.exp_avg, state);
-    writes(t.exp_avg_sq, state);
-    writes(t.copy, t.n * 2);
+    writes(0, t.param, t.n * (t.param_dtype == MX_F32 ? 4 : 2));
+    writes(1, t.exp_avg, state);
+    writes(2, t.exp_avg_sq, state);
+    writes(3, t.copy, t.n * 2);
     if (small) {
-      writes(t.exp_avg_scale, state / 32);
-      writes(t.exp_avg_sq_scale, state / 32);
+      writes(4, t.exp_avg_scale, state / 32);
+      writes(5, t.exp_avg_sq_scale, state / 32);
     }
   }
-  std::sort(written.begin(), written.end());
-  for (size_t i = 1; i < written.size(); ++i)
-    if (written[i].first < written[i - 1].second) return set_error(MX_ERR_INVALID, "parameters, states and copies must not overlap (is a tensor listed twice?)");
-  return MX_OK;
+  return overlap(written) ? set_error(MX_ERR_INVALID, "parameters, states and copies must not overlap (is a tensor listed twice?)") : MX_OK;
 }
 
 }  // namespace

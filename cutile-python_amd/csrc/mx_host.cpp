@@ -1161,8 +1161,14 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   for (int i = 1; i < 4; ++i)
     if (a[i] != Py_None && PySequence_Fast_GET_SIZE(a[i]) != cnt) Py_RETURN_NONE;
   std::vector<mx_adamw_tensor> list(cnt);
-  std::vector<at::Tensor> keep;   // written to; the lists may change while the GIL is released
-  keep.reserve(6 * cnt);
+  // what is written to (parameters, copies, states in tuples, which hold their tensors), and the gradients: the lists may change while the
+  // GIL is released
+  struct Kept : std::vector<PyObject*> {
+    void hold(PyObject* o) { Py_INCREF(o); push_back(o); }
+    ~Kept() { for (PyObject* o : *this) Py_DECREF(o); }
+  } kept, grads;
+  kept.reserve(3 * cnt);
+  grads.reserve(cnt);
   at::Device dev(at::kCUDA);
   int bits = 0;
   for (Py_ssize_t i = 0; i < cnt; ++i) {
@@ -1200,18 +1206,19 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const auto type = b == 32 ? at::kFloat : k < 2 ? at::kFloat8_e4m3fn : at::kFloat8_e8m0fnu;
       if (x.scalar_type() != type || x.numel() != want || x.device() != dev || !x.is_contiguous()) Py_RETURN_NONE;
       at[k] = x.data_ptr();
-      keep.push_back(x);
     }
     if (b == 32 && (s[2] != Py_None || s[3] != Py_None)) Py_RETURN_NONE;
     t.param = p.data_ptr(); t.grad = g.data_ptr();
+    grads.hold(item(1));
     t.exp_avg = at[0]; t.exp_avg_sq = at[1]; t.exp_avg_scale = at[2]; t.exp_avg_sq_scale = at[3];
-    keep.push_back(p);
+    kept.hold(item(0));
+    kept.hold(state);
     if (a[3] != Py_None && item(3) != Py_None) {
       if (!THPVariable_Check(item(3))) Py_RETURN_NONE;
       const at::Tensor& c = THPVariable_Unpack(item(3));
       if (c.scalar_type() != at::kBFloat16 || c.sizes() != p.sizes() || c.device() != dev || !c.is_contiguous()) Py_RETURN_NONE;
       t.copy = c.data_ptr();
-      keep.push_back(c);
+      kept.hold(item(3));
     }
   }
   mx_adamw_opts o = {};
@@ -1233,10 +1240,13 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {
     NoGil nogil;
     rc = lib.p_mx_adamw_step((int32_t)cnt, list.data(), &o, stream_of(dev));
-    if (rc == MX_OK)
-      for (const at::Tensor& t : keep) written(t);
   }
   if (rc != MX_OK) return PyLong_FromLong(rc);
+  for (PyObject* k : kept) {
+    if (!PyTuple_Check(k)) written(THPVariable_Unpack(k));
+    else
+      for (int i = 0; i < (bits == 8 ? 4 : 2); ++i) written(THPVariable_Unpack(PyTuple_GET_ITEM(k, i)));
+  }
   Py_RETURN_TRUE;
 }
 
