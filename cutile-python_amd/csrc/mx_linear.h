@@ -48,6 +48,8 @@ __device__ __forceinline__ void sigmoid_constants(int act, float& k1, float& k3)
   k1 = act == MX_ACT_SILU ? kLog2E : 1.5957691216f * kLog2E;
   k3 = act == MX_ACT_SILU ? 0.f : 1.5957691216f * 0.044715f * kLog2E;
 }
+// (maximum, which keeps NaN, and the median in the place of fmax and fmin: for those what comes from another block of code is made canonical
+// first, an instruction each)
 template <int KIND>
 __device__ __forceinline__ void activate(float (&v)[8], int act) {
   if constexpr (KIND == kActPlain) {
@@ -58,12 +60,12 @@ __device__ __forceinline__ void activate(float (&v)[8], int act) {
     float k1, k3;
     sigmoid_constants(act, k1, k3);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = fmaxf(v[e], -126.0f) * sigmoid_of(v[e] * __builtin_fmaf(fminf(v[e] * v[e], 1e30f), k3, k1));
+    for (int e = 0; e < 8; ++e) v[e] = __builtin_elementwise_maximum(v[e], -126.0f) * sigmoid_of(v[e] * __builtin_fmaf(fminf(v[e] * v[e], 1e30f), k3, k1));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float a = __builtin_fabsf(v[e]);
-      v[e] = __builtin_fmaf(-fminf(a, 126.0f), upper_tail(a, v[e] * v[e]), fmaxf(v[e], 0.f));
+      v[e] = __builtin_fmaf(-__builtin_amdgcn_fmed3f(a, 0.f, 126.0f), upper_tail(a, v[e] * v[e]), __builtin_elementwise_maximum(v[e], 0.f));
     }
   }
 }
