@@ -808,7 +808,8 @@ int launch_pp_pair(const GemmArgs& g, hipStream_t stream) {
   return g.tail ? run(std::true_type{}) : run(std::false_type{});
 }
 #if MX_PP_PAIR >= 8
-template int launch_pp_linear_pair<MX_E4M3, MX_PP_PAIR < 11 ? MX_E4M3 : MX_E2M1, (MX_PP_PAIR - 8) % 3>(const GemmArgs&, const LinearOut&, hipStream_t);
+template int launch_pp_linear_pair<MX_PP_PAIR < 14 ? MX_E4M3 : MX_E2M1, MX_PP_PAIR < 11 ? MX_E4M3 : MX_E2M1, (MX_PP_PAIR - 8) % 3>(const GemmArgs&, const LinearOut&,
+                                                                                                                  hipStream_t);
 #elif MX_PP_PAIR >= 4
 template int launch_pp_gated_pair<MX_PP_PAIR == 4 || MX_PP_PAIR == 7 ? MX_E4M3 : MX_PP_PAIR == 5 ? MX_E5M2 : MX_E2M1,
                                   MX_PP_PAIR == 4 ? MX_E4M3 : MX_PP_PAIR == 5 ? MX_E5M2 : MX_E2M1>(const GemmArgs&, const GateOut&, hipStream_t);
@@ -829,24 +830,28 @@ int launch_gemm_pingpong_gated(const GemmArgs& g, const GateOut& o, hipStream_t 
 #undef MX_CASE
   return set_error(MX_ERR_DTYPE, "MFMA kernel: unsupported element format pair (%d, %d)", g.a_fmt, g.b_fmt);
 }
-#define MX_EXTERN(BF, KIND) extern template int launch_pp_linear_pair<MX_E4M3, BF, KIND>(const GemmArgs&, const LinearOut&, hipStream_t);
-MX_EXTERN(MX_E4M3, kActPlain)
-MX_EXTERN(MX_E4M3, kActSigmoid)
-MX_EXTERN(MX_E4M3, kActErf)
-MX_EXTERN(MX_E2M1, kActPlain)
-MX_EXTERN(MX_E2M1, kActSigmoid)
-MX_EXTERN(MX_E2M1, kActErf)
+#define MX_EXTERN(AF, BF, KIND) extern template int launch_pp_linear_pair<AF, BF, KIND>(const GemmArgs&, const LinearOut&, hipStream_t);
+MX_EXTERN(MX_E4M3, MX_E4M3, kActPlain)
+MX_EXTERN(MX_E4M3, MX_E4M3, kActSigmoid)
+MX_EXTERN(MX_E4M3, MX_E4M3, kActErf)
+MX_EXTERN(MX_E4M3, MX_E2M1, kActPlain)
+MX_EXTERN(MX_E2M1, MX_E2M1, kActPlain)
+MX_EXTERN(MX_E4M3, MX_E2M1, kActSigmoid)
+MX_EXTERN(MX_E2M1, MX_E2M1, kActSigmoid)
+MX_EXTERN(MX_E4M3, MX_E2M1, kActErf)
+MX_EXTERN(MX_E2M1, MX_E2M1, kActErf)
 #undef MX_EXTERN
 
-// (E4M3 activations, linear_is_plain())
+// (linear_is_plain())
 int launch_gemm_pingpong_linear(const GemmArgs& g, const LinearOut& o, hipStream_t stream) {
   const int kind = act_kind(o.act);
-#define MX_CASE(BF) \
-  if (g.a_fmt == MX_E4M3 && g.b_fmt == BF) \
-    return kind == kActErf ? launch_pp_linear_pair<MX_E4M3, BF, kActErf>(g, o, stream) \
-           : kind == kActSigmoid ? launch_pp_linear_pair<MX_E4M3, BF, kActSigmoid>(g, o, stream) : launch_pp_linear_pair<MX_E4M3, BF, kActPlain>(g, o, stream);
-  MX_CASE(MX_E4M3)
-  MX_CASE(MX_E2M1)
+#define MX_CASE(AF, BF) \
+  if (g.a_fmt == AF && g.b_fmt == BF) \
+    return kind == kActErf ? launch_pp_linear_pair<AF, BF, kActErf>(g, o, stream) \
+           : kind == kActSigmoid ? launch_pp_linear_pair<AF, BF, kActSigmoid>(g, o, stream) : launch_pp_linear_pair<AF, BF, kActPlain>(g, o, stream);
+  MX_CASE(MX_E4M3, MX_E4M3)
+  MX_CASE(MX_E4M3, MX_E2M1)
+  MX_CASE(MX_E2M1, MX_E2M1)
 #undef MX_CASE
   return set_error(MX_ERR_DTYPE, "linear ping-pong kernel: unsupported element format pair (%d, %d)", g.a_fmt, g.b_fmt);
 }

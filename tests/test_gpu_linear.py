@@ -127,6 +127,14 @@ CASES = [
     ("pingpong", "e4m3", "e2m1", 600, 6144, 544, bf16, None, "gelu_tanh"),
     ("pingpong", "e4m3", "e4m3", 4200, 4096, 4128, bf16, bf16, "gelu"),
     ("auto", "e4m3", "e4m3", 1531, 8192, 1088, bf16, bf16, "relu"),
+    ("pingpong", "e2m1", "e2m1", 500, 8192, 520, bf16, bf16, "gelu"),
+    ("pingpong", "e2m1", "e2m1", 300, 1536, 448, f32, None, "gelu_tanh"),
+    ("pingpong", "e2m1", "e2m1", 1531, 1056, 1088, None, bf16, None),
+    ("auto", "e2m1", "e2m1", 2048, 2048, 4096, bf16, bf16, "silu"),
+    # at the ping-pong kernel's sizes what it does not finish
+    ("auto", "e5m2", "e5m2", 2048, 1024, 4096, bf16, bf16, "gelu"),
+    ("auto", "e4m3", "e4m3", 2048, 1024, 4097, bf16, f32, "silu"),
+    ("auto", "e4m3", "e2m1", 2048, 1024, 4096, f16, f16, "relu"),
     ("mfma256", "e4m3", "e4m3", 300, 512, 320, bf16, bf16, "gelu"),
     # through memory, some rows at a time
     ("mfma256", "e2m1", "e2m1", 2305, 256, 2080, bf16, bf16, "gelu"),
@@ -231,7 +239,7 @@ def inner(buf, rows, cols, size, offset=0):
 
 
 @pytest.mark.parametrize("kernel,M,K,N", [("stream", 3, 640, 96), ("stream", 50, 256, 67), ("mfma128", 77, 288, 160), ("mfma128", 130, 4096, 100), ("pingpong", 300, 512, 320),
-                                          ("pingpong", 500, 512, 333), ("generic", 5, 64, 32)])
+                                          ("pingpong", 500, 512, 333), ("pingpong", 300, 4096, 320), ("stream", 2, 1024, 4096), ("generic", 5, 64, 32)])
 @pytest.mark.parametrize("out,offset", [("bf16", 0), ("bf16", 1), ("f32", 0), ("f32", 3), ("e4m3", 0)])
 def test_padded_outputs(ct, dev, kernel, M, K, N, out, offset):
     if out == "e4m3" and N % 32:
@@ -427,6 +435,28 @@ def test_gradients_against_differences(ct, dev):
         step[i] = 1e-5
         diff = (f(*at[:k], at[k] + step.view(g.shape), *at[k + 1:]) - f(*at[:k], at[k] - step.view(g.shape), *at[k + 1:])) / 2e-5
         assert abs(float(diff - g.flatten()[i])) <= 1e-6 * float(g.abs().max())
+
+
+@pytest.mark.parametrize("T", [33, 600])
+def test_any_strides(ct, dev, T):
+    """Transposed, broadcast and strided inputs and gradients give what their copies give."""
+    K, N = 128, 1024
+    x, w, b, dy, res = make(dev, T, K, N, f32, 16, f32)
+    views = [x.T.contiguous().T, torch.stack([w, w], 2)[:, :, 0], torch.stack([b, b], 1)[:, 0], res.T.contiguous().T]
+    plain = [t.clone().requires_grad_() for t in (x, w, b, res)]
+    odd = [t.detach().requires_grad_() for t in views]
+    assert not any(t.is_contiguous() for t in odd)
+    y, z = ct.linear(*plain, activation="silu"), ct.linear(*odd, activation="silu")
+    assert torch.equal(y, z)
+    y.backward(dy)
+    z.backward(dy.T.contiguous().T)
+    assert all(torch.equal(p.grad, o.grad) for p, o in zip(plain, odd))
+    one, x1 = torch.ones((), device=dev), x[:1].expand(T, K)
+    g = [torch.autograd.grad(ct.linear(t, plain[1], plain[2], activation="gelu"), plain[1:3], d) for t, d in ((x1, one.expand(T, N)), (x1.clone(), torch.ones((T, N), device=dev)))]
+    assert all(torch.equal(a, c) for a, c in zip(*g))
+    _, st = ct.linear_forward(views[0], views[1], views[2], views[3], activation="relu")
+    _, st2 = ct.linear_forward(x, w, b, res, activation="relu")
+    assert all(torch.equal(a, c) for a, c in zip(ct.linear_backward(dy.T.contiguous().T, st), ct.linear_backward(dy, st2)))
 
 
 def test_residual_alone_and_no_tokens(ct, dev):
