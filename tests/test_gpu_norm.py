@@ -164,6 +164,24 @@ def test_quantized_from_16_bits(ct, dev, rows, H, dtype):
     assert q3.shape == (1, rows, y.shape[1]) and torch.equal(q3[0].view(torch.uint8), q.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", [f32, bf16], ids=str)
+@pytest.mark.parametrize("rows,H", [(33000, 40), (9001, 600), (5003, 1500), (3001, 4096), (1531, 8192), (1100, 16000), (1030, 17000)])
+def test_more_rows_than_fit_at_once(ct, dev, rows, H, dtype):
+    """Workgroups that take several rows, the last of them fewer: every row is what it is by itself, and the definition's."""
+    x = make(dev, rows, H, dtype, 20, 2.0, 0.5)
+    w, b = vectors(dev, H, dtype)
+    y, mean, rstd = ct.layer_norm_forward(x, w, b)
+    q, s = ct.layer_norm_quantize(x, w, b)
+    for at in (slice(0, 5), slice(rows // 2, rows // 2 + 3), slice(rows - 2, rows)):
+        part = ct.layer_norm_forward(x[at], w, b)
+        assert torch.equal(part[0], y[at]) and torch.equal(part[1], mean[at]) and torch.equal(part[2], rstd[at])
+        pq, ps = ct.layer_norm_quantize(x[at], w, b)
+        assert torch.equal(pq.view(torch.uint8), q[at].view(torch.uint8)) and torch.equal(ps.view(torch.uint8), s[at].view(torch.uint8))
+    some = torch.randperm(rows, generator=torch.Generator().manual_seed(1))[:1000]
+    want, off = forward(x[some.to(dev)], w, b, 1e-5)
+    near(y[some.to(dev)], want, off, dtype)
+
+
 # ---- backward ---------------------------------------------------------------------------------------------------------------
 def backward(dy, x, w, eps):
     dy, x, w = d64(dy), d64(x), d64(w)
