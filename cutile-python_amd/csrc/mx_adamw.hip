@@ -2,7 +2,8 @@
 //
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// Bound: memory, 28 bytes an element (fp32 parameters, gradients and states) down to 10.1 (bf16, 8-bit states).  A workgroup takes
+// Bound: memory, 28 bytes an element (fp32 parameters, gradients and states) down to 10.1 (bf16, 8-bit states); 117 M elements of 16.1
+// bytes (fp32 parameters with bf16 copies and gradients, 8-bit states) 370 us, 5.1 TB/s.  A workgroup takes
 // kChunk elements of one tensor; which tensor, it finds in a table in the kernel's arguments, so that nothing is copied to the
 // device and a launch serves kTensors of them.
 //

@@ -9,7 +9,7 @@
 namespace mx {
 namespace {
 
-// One pass over fp32 products (of a sum that was split along K, one each): a lane has 8 columns of a row.  Bound: memory.
+// One pass over fp32 products (of a sum that was split along K, one each): a lane has 8 columns of a row.  Bound: memory (32 x 28672: 3 us, a launch).
 template <int KIND>
 __global__ __launch_bounds__(256) void linear_pass_kernel(const float* product, const int splits, const int64_t M, const LinearOut o) {
   const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (o.N + 7) / 8;   // (N % 32 == 0 with codes: four lanes of a wave are a block)

@@ -436,7 +436,7 @@ MX_API int mx_ffn_backward(const mx_tensor* dy, const void* saved, int64_t saved
  *   at multiples of 8 bytes: quantised by the floor rule from the unrounded result, the left operand of the next product
  *   pre [M,N] MX_BF16 or NULL: product + bias, for a backward pass
  * Sums as in mx_gemm (the scaled matrix instructions align an instruction's products with some 18 bits below the largest: 1.5e-5 of the
- * result's norm), everything behind them in 32 bits; the activation is within 2e-6 of its value.  act(-inf) is zero for gelu and silu;
+ * result's norm), everything behind them in 32 bits; the activation is within 2e-6 of its value (gelu below -7: 4e-5).  act(-inf) is zero for gelu and silu;
  * a block of out with a NaN has mx_quantize's scale and zeros.
  * Fused into the streaming kernel, the 128 x 128 one and, for operands of E4M3, E4M3 by E2M1 or E2M1 with a bf16 or E4M3 result and a bf16
  * residual in whole 16-byte pieces, the ping-pong one; with other kernels (opts->kernel as in mx_gemm) the product goes through the
