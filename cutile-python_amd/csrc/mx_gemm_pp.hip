@@ -57,10 +57,11 @@ namespace {
 // Gate: Ungated, GateOut or LinearGate: bias, activation and residual of a linear layer (mx_linear.h).  The activation's kind and the output's
 // are instances of their own: a wave has 16 groups of eight columns, each with its own copy of all this, and with the choices made there the
 // 270 KiB of a kernel were more than the instruction cache for either team.
-template <int KIND_, bool CODES_>
+enum { kLinear16, kLinearCodes, kLinear32 };   // result and residual of 16 bits; E4M3; of 16 or 32, as the arguments say
+template <int KIND_, int OUT_>
 struct LinearGate : LinearOut {
-  static constexpr int KIND = KIND_;
-  static constexpr bool CODES = CODES_;
+  static constexpr int KIND = KIND_, OUT = OUT_;
+  static constexpr bool CODES = OUT_ == kLinearCodes;
 };
 template <class C, typename OutT, bool GROUPED, bool SPLIT, int TEAM, bool KTAIL, class Gate>
 __device__ __forceinline__ void pp_body(const GemmArgs& g, const Gate& gate, lds_u8* const smem, const int wn,
@@ -302,27 +303,38 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, const Gate& gate, lds
       const uint32_t row = m0 + wm0 + r;
       float bias[2][8];
       uint32_t vc[2], vs[2], vp[2], vr[2];             // offsets of the lane's columns in its first row
-      const uint32_t c_ld = (uint32_t)gate.c_ld * (CODES ? 1 : 2), s_ld = (uint32_t)gate.s_ld, p_ld = (uint32_t)gate.pre_ld * 2, r_ld = (uint32_t)gate.r_ld * 2;
+      const bool c32 = Gate::OUT == kLinear32 && gate.c_fmt == MX_F32, r32 = Gate::OUT == kLinear32 && gate.res_dtype == MX_F32;   // uniform
+      const uint32_t c_size = CODES ? 1 : c32 ? 4 : 2, r_size = r32 ? 4 : 2;
+      const uint32_t c_ld = (uint32_t)gate.c_ld * c_size, s_ld = (uint32_t)gate.s_ld, p_ld = (uint32_t)gate.pre_ld * 2, r_ld = (uint32_t)gate.r_ld * r_size;
       const __amdgpu_buffer_rsrc_t rc = make_rsrc(gate.c, g.M * c_ld), rsc = make_rsrc(gate.s, CODES ? g.M * s_ld : 0u), rp = make_rsrc(gate.pre, gate.pre ? g.M * p_ld : 0u),
-                                   rr = make_rsrc(gate.res, gate.res ? (g.M - 1) * r_ld + gate.N * 2 : 0u);   // (its rows may overlap)
+                                   rr = make_rsrc(gate.res, gate.res ? (g.M - 1) * r_ld + gate.N * r_size : 0u);   // (its rows may overlap)
 #pragma unroll
       for (int jp = 0; jp < 2; ++jp) {
         const uint32_t n = col + 32 * jp, out = (int)n < gate.N ? 0u : kOobOffset;
         linear_bias(gate, n, bias[jp]);
-        vc[jp] = out | (row * c_ld + n * (CODES ? 1 : 2));
+        vc[jp] = out | (row * c_ld + n * c_size);
         vs[jp] = out | (gq == 0 ? row * s_ld + n / 32 : kOobOffset);
         vp[jp] = out | (row * p_ld + n * 2);
-        vr[jp] = out | (row * r_ld + n * 2);
+        vr[jp] = out | (row * r_ld + n * r_size);
       }
+      // the residual: of 16 bits a row tile ahead; of 32, which take the registers of both, when their row tile's turn comes
       u4 res[2][2];
-      auto request = [&](int i) {                      // (a row tile ahead)
+      auto piece = [&](int i, int jp, int at) { return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rr, vr[jp] + 16 * i * r_ld, at, 0)); };
+      auto request = [&](int i) {
 #pragma unroll
-        for (int jp = 0; jp < 2; ++jp) res[i & 1][jp] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rr, vr[jp] + 16 * i * r_ld, 0, 0));
+        for (int jp = 0; jp < 2; ++jp) res[i & 1][jp] = piece(i, jp, 0);
       };
-      if (gate.res) request(0);
+      if (gate.res && !r32) request(0);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        if (gate.res && i + 1 < MT) request(i + 1);
+        if (gate.res) {
+          if (!r32) {
+            if (i + 1 < MT) request(i + 1);
+          } else {
+#pragma unroll
+            for (int jp = 0; jp < 2; ++jp) { res[0][jp] = piece(i, jp, 0); res[1][jp] = piece(i, jp, 16); }
+          }
+        }
 #pragma unroll
         for (int jp = 0; jp < 2; ++jp) {
           float v[8];
@@ -334,10 +346,18 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, const Gate& gate, lds
           if (gate.pre) __builtin_amdgcn_raw_buffer_store_b128(pack_piece<MX_BF16>(v), rp, vp[jp] + 16 * i * p_ld, 0, 0);
           activate<Gate::KIND>(v, gate.act);
           if (gate.res) {
-            float x[8];
-            unpack_piece<MX_BF16>(res[i & 1][jp], x);
+            if (!r32) {
+              float x[8];
+              unpack_piece<MX_BF16>(res[i & 1][jp], x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += x[e];
+              for (int e = 0; e < 8; ++e) v[e] += x[e];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[e] += __builtin_bit_cast(float, (uint32_t)res[0][jp][e]);
+                v[4 + e] += __builtin_bit_cast(float, (uint32_t)res[1][jp][e]);
+              }
+            }
           }
           if constexpr (CODES) {
             uint32_t byte;
@@ -347,6 +367,9 @@ __device__ __forceinline__ void pp_body(const GemmArgs& g, const Gate& gate, lds
             __builtin_amdgcn_raw_buffer_store_b64(c, rc, vc[jp] + 16 * i * c_ld, 0, 0);
             saturate_conversions(false);
             __builtin_amdgcn_raw_buffer_store_b8((uint8_t)byte, rsc, vs[jp] + 16 * i * s_ld, 0, 0);
+          } else if (c32) {
+            __builtin_amdgcn_raw_buffer_store_b128(pack_piece<MX_F32>({v[0], v[1], v[2], v[3]}), rc, vc[jp] + 16 * i * c_ld, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b128(pack_piece<MX_F32>({v[4], v[5], v[6], v[7]}), rc, vc[jp] + 16 * i * c_ld, 16, 0);
           } else {
             __builtin_amdgcn_raw_buffer_store_b128(pack_piece<MX_BF16>(v), rc, vc[jp] + 16 * i * c_ld, 0, 0);
           }
@@ -779,14 +802,17 @@ int launch_pp_gated_pair(const GemmArgs& g, const GateOut& o, hipStream_t stream
 // A linear layer's, one kind of activation.
 template <int AF, int BF, int KIND>
 int launch_pp_linear_pair(const GemmArgs& g, const LinearOut& o, hipStream_t stream) {
-  auto run = [&](auto codes) {
-    LinearGate<KIND, decltype(codes)::value> gate = {};
+  auto run = [&](auto out) {
+    LinearGate<KIND, decltype(out)::value> gate = {};
     static_cast<LinearOut&>(gate) = o;
     if (g.tile_rows == 192) return launch_pp_gated<Cfg<AF, BF, 192, 256, 2, 4>>(g, gate, stream);
     using C = Cfg<AF, BF, 256, 256, 2, 4>;
     return g.tail ? launch_pp_gated<C, true>(g, gate, stream) : launch_pp_gated<C>(g, gate, stream);
   };
-  return o.c_fmt == MX_E4M3 ? run(std::true_type{}) : run(std::false_type{});
+  // (one instance for both sizes of numbers: 8192 x 14336 x 4096 with a residual 443 us instead of 399 in bf16)
+  return o.c_fmt == MX_E4M3                                              ? run(std::integral_constant<int, kLinearCodes>{})
+         : o.c_fmt == MX_F32 || (o.res && o.res_dtype == MX_F32) ? run(std::integral_constant<int, kLinear32>{})
+                                                                         : run(std::integral_constant<int, kLinear16>{});
 }
 
 // One element-format pair (grouped and plain, fp32 and bf16 output) per compilation of this file, so that the pairs

@@ -175,14 +175,15 @@ __device__ __forceinline__ void linear_finish_any(const LinearOut& o, const v4f&
 }
 
 // What a wave's row tiles of the ping-pong kernel leave by: everything through buffer descriptors, whose range takes the place of comparisons
-// with the last row; columns that are not there have an offset beyond it.  bf16 (CODES false) or E4M3 out, a bf16 residual, rows of
-// whole 16-byte pieces (codes: of 8), each tensor less than 2 GiB, the rows behind it that a tile reaches included (their offsets must not
+// with the last row; columns that are not there have an offset beyond it.  bf16 or fp32 (CODES false) or E4M3 out, a bf16 residual or, CODES false, an fp32
+// one, rows of whole 16-byte pieces (codes: of 8), each tensor less than 2 GiB, the rows behind it that a tile reaches included (their offsets must not
 // come round): linear_is_plain().
 inline bool linear_is_plain(const LinearOut& o, int64_t M) {
   const int64_t lim = (int64_t)1 << 31;
   auto fine = [&](const void* p, int64_t ld, int size, int align) { return !p || ((uintptr_t)p % align == 0 && ld * size % align == 0 && (M + 256) * ld * size < lim); };
-  return o.N % 8 == 0 && (o.c_fmt == MX_BF16 ? fine(o.c, o.c_ld, 2, 16) : o.c_fmt == MX_E4M3 && fine(o.c, o.c_ld, 1, 8) && fine(o.s, o.s_ld, 1, 1)) &&
-         fine(o.pre, o.pre_ld, 2, 16) && (!o.res || (o.res_dtype == MX_BF16 && fine(o.res, o.r_ld, 2, 16)));
+  const bool codes = o.c_fmt == MX_E4M3, r32 = o.res_dtype == MX_F32;
+  const bool out = codes ? fine(o.c, o.c_ld, 1, 8) && fine(o.s, o.s_ld, 1, 1) : fine(o.c, o.c_ld, o.c_fmt == MX_F32 ? 4 : 2, 16);
+  return o.N % 8 == 0 && out && fine(o.pre, o.pre_ld, 2, 16) && (!o.res || ((o.res_dtype == MX_BF16 || (r32 && !codes)) && fine(o.res, o.r_ld, r32 ? 4 : 2, 16)));
 }
 __device__ __forceinline__ void linear_bias(const LinearOut& o, int col, float (&bias)[8]) { load_floats<8>(o.bias, o.bias_dtype, col, o.N - col, 0.f, bias); }
 
