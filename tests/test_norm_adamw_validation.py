@@ -188,7 +188,7 @@ def adam(tensors, **over):
 
 def one(at=0, n=64, p=F, g=F, small=False, **over):
     q = P + at
-    t = L.MxAdamwTensor(param=q, grad=q + 1024, exp_avg=q + 2048, exp_avg_sq=q + 3072, n=n, param_dtype=p, grad_dtype=g)
+    t = L.MxAdamwTensor(param=q, grad=q + 1024, exp_avg=q + 2048, exp_avg_sq=q + 3008, n=n, param_dtype=p, grad_dtype=g)
     if small:
         t.exp_avg_scale, t.exp_avg_sq_scale = q + 3500, q + 3600
     for k, v in over.items():
