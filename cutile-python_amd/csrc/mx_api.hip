@@ -672,7 +672,8 @@ int gemm_impl(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const
     // the decode kernel has no such epilogue.  A pass behind it costs 3 us, which it makes up for with many weights alone (32 rows, 28672 x 8192:
     // 26 us against 31 streamed; 16384 x 8192: 19.7 against 17.6, 14336 x 4096: 11.5 against 10.3; 1 row, 28672 x 8192: 23.5 both)
     if (kernel == MX_KERNEL_DECODE && o.kernel == MX_KERNEL_AUTO && !why_stream && !(M > 8 && N * K >= (int64_t)192 << 20)) kernel = MX_KERNEL_STREAM;
-    const bool pp = ((A->dtype == MX_E4M3 && (B->dtype == MX_E4M3 || B->dtype == MX_E2M1)) || (A->dtype == MX_E2M1 && B->dtype == MX_E2M1)) && linear_is_plain(*lin, M);
+    const bool whole = K % 128 == 0 && K >= 256;
+    const bool pp = ((A->dtype == MX_E4M3 && (B->dtype == MX_E4M3 || B->dtype == MX_E2M1) && whole) || (A->dtype == MX_E2M1 && B->dtype == MX_E2M1)) && linear_is_plain(*lin, M);
     // (8192 x 14336 x 4096 with an fp32 result, which once was such a case: 568 us so, 1119 through memory, some rows at a time)
     if (kernel == MX_KERNEL_MFMA_PINGPONG && o.kernel == MX_KERNEL_AUTO && !pp) kernel = MX_KERNEL_MFMA_128x128;
     const bool fused = kernel == MX_KERNEL_STREAM || kernel == MX_KERNEL_MFMA_128x128 || (kernel == MX_KERNEL_MFMA_PINGPONG && pp);

@@ -659,12 +659,16 @@ __device__ __forceinline__ void pp_kernel(const GemmArgs& g, const Gate& gate) {
   if (walk.head() == kNoTile) return;   // uniform: nothing left for this workgroup
   // (uniform.  The MXFP4 instance keeps the one masked body: a second, unmasked one measured no faster on it.)
   // (a split K is a whole number of K-quads)
+  // (a linear layer of 8-bit operands comes with whole stages only: an epilogue is too much code to have it in four bodies)
+  constexpr bool WHOLE = std::is_base_of<LinearOut, Gate>::value && C::KSUB == 1;
   const bool ktail = C::KSUB != 1 || (!SPLIT && (g.K % 128 != 0 || ksteps < 2));
-  if (ktail) {
-    if (wave < 4)
-      pp_body<C, OutT, GROUPED, SPLIT, 0, true>(g, gate, smem, wave, lane, walk);
-    else
-      pp_body<C, OutT, GROUPED, SPLIT, 1, true>(g, gate, smem, wave - 4, lane, walk);
+  if (!WHOLE && ktail) {
+    if constexpr (!WHOLE) {
+      if (wave < 4)
+        pp_body<C, OutT, GROUPED, SPLIT, 0, true>(g, gate, smem, wave, lane, walk);
+      else
+        pp_body<C, OutT, GROUPED, SPLIT, 1, true>(g, gate, smem, wave - 4, lane, walk);
+    }
   } else if constexpr (C::KSUB == 1) {
     if (wave < 4)
       pp_body<C, OutT, GROUPED, SPLIT, 0, false>(g, gate, smem, wave, lane, walk);

@@ -438,7 +438,7 @@ MX_API int mx_ffn_backward(const mx_tensor* dy, const void* saved, int64_t saved
  * Sums as in mx_gemm (the scaled matrix instructions align an instruction's products with some 18 bits below the largest: 1.5e-5 of the
  * result's norm), everything behind them in 32 bits; the activation is within 2e-6 of its value (gelu below -7: 4e-5).  act(-inf) is zero for gelu and silu;
  * a block of out with a NaN has mx_quantize's scale and zeros.
- * Fused into the streaming kernel, the 128 x 128 one and, for operands of E4M3, E4M3 by E2M1 or E2M1, rows in whole 16-byte pieces and
+ * Fused into the streaming kernel, the 128 x 128 one and, for operands of E4M3, E4M3 by E2M1 (K % 128 == 0) or E2M1, rows in whole 16-byte pieces and
  * residuals that are not fp16 (bf16 beside an E4M3 result), the ping-pong one; with other kernels (opts->kernel as in mx_gemm) the product goes
  * through the workspace, some rows at a time.  residual may
  * be out itself.  workspace: mx_linear_gemm_workspace_bytes(), all of it, aligned to 256 bytes.

@@ -131,6 +131,9 @@ CASES = [
     ("pingpong", "e2m1", "e2m1", 300, 1536, 448, f32, None, "gelu_tanh"),
     ("pingpong", "e2m1", "e2m1", 1531, 1056, 1088, None, bf16, None),
     ("auto", "e2m1", "e2m1", 2048, 2048, 4096, bf16, bf16, "silu"),
+    ("pingpong", "e4m3", "e4m3", 700, 640, 1088, bf16, f32, "gelu"),
+    ("pingpong", "e4m3", "e4m3", 257, 640, 192, f32, bf16, "gelu_tanh"),
+    ("pingpong", "e4m3", "e4m3", 300, 256, 320, bf16, None, "silu"),
     ("pingpong", "e4m3", "e4m3", 700, 544, 1088, bf16, f32, "gelu"),   # (results of both types: fp32 with fp32 residuals)
     ("pingpong", "e4m3", "e2m1", 500, 4096, 520, None, f32, "silu"),
     ("pingpong", "e2m1", "e2m1", 300, 1056, 448, f32, f32, None),
@@ -172,7 +175,7 @@ def test_product_with_epilogue(ct, dev, kernel, af, wf, M, K, N, bt, rt, act):
 
 
 @pytest.mark.parametrize("act", ACTS)
-@pytest.mark.parametrize("kernel,M,K,N", [("stream", 20, 256, 96), ("stream", 1, 512, 8192), ("mfma128", 200, 288, 160), ("pingpong", 300, 544, 288), ("auto", 300, 512, 96),
+@pytest.mark.parametrize("kernel,M,K,N", [("stream", 20, 256, 96), ("stream", 1, 512, 8192), ("mfma128", 200, 288, 160), ("pingpong", 300, 544, 288), ("pingpong", 300, 640, 288), ("auto", 300, 512, 96),
                                           ("generic", 9, 64, 32)])
 def test_every_activation_everywhere(ct, dev, kernel, M, K, N, act):
     """Arguments from -40 to 40, by way of the bias; every row the same product."""
@@ -186,7 +189,7 @@ def test_every_activation_everywhere(ct, dev, kernel, M, K, N, act):
         check(y, want, err, dtype)
 
 
-@pytest.mark.parametrize("kernel,M,K,N", [("stream", 20, 256, 96), ("mfma128", 200, 288, 160), ("pingpong", 300, 544, 288), ("pingpong", 1100, 1024, 1056), ("auto", 70, 512, 96)])
+@pytest.mark.parametrize("kernel,M,K,N", [("stream", 20, 256, 96), ("mfma128", 200, 288, 160), ("pingpong", 300, 544, 288), ("pingpong", 300, 640, 288), ("pingpong", 1100, 1024, 1056), ("auto", 70, 512, 96)])
 def test_not_finite(ct, dev, kernel, M, K, N):
     a, w = randn_operand(M, K, O.E4M3, M, dev), randn_operand(N, K, O.E4M3, N, dev, std=K ** -0.5)
     args, inf = (a.storage, a.scale_t, w.storage, w.scale_t), float("inf")
@@ -326,7 +329,7 @@ def test_rows_far_apart(ct, dev, kernel, dtype):
     assert torch.equal(far, want)
 
 
-@pytest.mark.parametrize("kernel,M,K,N", [("stream", 20, 256, 96), ("mfma128", 300, 288, 160), ("pingpong", 600, 544, 288), ("pingpong", 300, 4096, 320), ("generic", 9, 64, 32),
+@pytest.mark.parametrize("kernel,M,K,N", [("stream", 20, 256, 96), ("mfma128", 300, 288, 160), ("pingpong", 600, 640, 288), ("pingpong", 300, 4096, 320), ("generic", 9, 64, 32),
                                           ("mfma256", 300, 256, 96)])
 def test_residual_in_place(ct, dev, kernel, M, K, N):
     a, w = randn_operand(M, K, O.E4M3, 1, dev), randn_operand(N, K, O.E4M3, 2, dev)
