@@ -123,7 +123,7 @@ int run_linear(const mx_tensor& A, const mx_tensor& As, const mx_tensor& W, cons
     Deal ws = {(uint8_t*)workspace};
     mx_tensor a = A, as = As, c = tensor2d(ws.take(rows * N * 4), MX_F32, m, N, N);
     a.shape[0] = m;
-    a.ptr = (uint8_t*)A.ptr + m0 * A.stride[0];
+    a.ptr = (uint8_t*)A.ptr + (A.dtype == MX_E2M1 && A.packed_dim == 0 ? m0 / 2 : m0) * A.stride[0];   // (two rows to a byte, packed along M)
     if (o.a_scale_layout == MX_SCALE_2D || o.a_scale_layout == MX_SCALE_SWIZZLE_32_4_4) {
       as.shape[0] = o.a_scale_layout == MX_SCALE_2D ? m : m / 128;
       as.ptr = (uint8_t*)As.ptr + (o.a_scale_layout == MX_SCALE_2D ? m0 : m0 / 128) * As.stride[0];
