@@ -246,12 +246,13 @@ __global__ __launch_bounds__(kBackThreads) void norm_backward_kernel(const NormB
     float h[V][E], xh[V][E], sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+      const int n = H - (t + i * GT) * E;
       float d[E];
       unpack_piece<T>(rx[i], xh[i]);
       unpack_piece<T>(rd[i], d);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        xh[i][e] = (xh[i][e] - mean) * rstd;
+        xh[i][e] = e < n ? (xh[i][e] - mean) * rstd : 0.f;   // (the mean of a row far from zero times rstd may be infinite)
         db[i][e] += d[e];
         dw[i][e] = __builtin_fmaf(d[e], xh[i][e], dw[i][e]);
         h[i][e] = d[e] * w[i][e];
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_backward_long_kernel(const 
       load_floats<E>(a.w, a.w_dtype, (int64_t)p * E, n, 1.f, w);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        xh[e] = (xh[e] - mean) * rstd;
+        xh[e] = e < n ? (xh[e] - mean) * rstd : 0.f;   // (as above)
         h[e] *= w[e];
       }
     };
