@@ -76,6 +76,10 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
         return r
     if r is not None:
         _raise_code(r)
+    return _backward(dy, x, mean, rstd, weight, need_dx, need_dweight, need_dbias, torch.float32 if weight is None else weight.dtype)
+
+
+def _backward(dy, x, mean, rstd, weight, need_dx, need_dweight, need_dbias, bias_dtype):
     _check(x, weight, None, 0.0)
     dev = _same_device(x, dy, mean, rstd)
     if dy.dtype != x.dtype:
@@ -87,11 +91,10 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or tuple(t.shape) != (T,):
             raise ValueError(f"{name} must be ({T},) float32 as the forward pass leaves it, got {tuple(t.shape)} {_dtype_name(t.dtype)}")
-    vec = torch.float32 if weight is None else weight.dtype
     make = torch.empty if T else torch.zeros    # no rows: the sums over them are zeros
     dx = torch.empty((T, H), dtype=x.dtype, device=dev) if need_dx else None
-    dw = make(H, dtype=vec, device=dev) if need_dweight else None
-    db = make(H, dtype=vec, device=dev) if need_dbias else None
+    dw = make(H, dtype=torch.float32 if weight is None else weight.dtype, device=dev) if need_dweight else None
+    db = make(H, dtype=bias_dtype, device=dev) if need_dbias else None
     if T and (need_dx or need_dweight or need_dbias):
         lib = L.lib()
         need = lib.mx_layer_norm_backward_workspace_bytes(T, H)
@@ -114,8 +117,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dw, db = layer_norm_backward(dy.to(x.dtype), x, mean, rstd, weight, need_dx=need[0], need_dweight=need[1], need_dbias=need[2])
-        return dx, dw, None if db is None else db.to(ctx.bias_dtype), None
+        return (*_backward(dy.to(x.dtype), x, mean, rstd, weight, need[0], need[1], need[2], ctx.bias_dtype), None)   # (sums are rounded once)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *, eps: float = 1e-5) -> torch.Tensor:

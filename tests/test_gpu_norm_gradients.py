@@ -1,12 +1,13 @@
-"""Gradients of layer norm where its backward pass can go wrong: rows whose mean times rstd is beyond the largest float."""
+"""Gradients of layer norm where its backward pass can go wrong: rows whose mean times rstd is beyond the largest float in rows that do not
+fill their threads, and gradients of weight and bias that are of different types."""
 import pytest
 import torch
 
-from test_gpu_norm import SUM, d64, make, near, vectors
+from test_gpu_norm import SUM, backward, d64, make, near, vectors
 
 pytestmark = pytest.mark.gpu
 
-bf16, f32 = torch.bfloat16, torch.float32
+bf16, f16, f32 = torch.bfloat16, torch.float16, torch.float32
 
 
 @pytest.mark.parametrize("dtype", [f32, bf16], ids=str)
@@ -29,3 +30,40 @@ def test_mean_times_rstd_beyond_the_largest_float(ct, dev, H, dtype):
     assert bool((dw == 0).all())
     near(db, d64(dy).sum(0), SUM * d64(dy).abs().sum(0), f32)
     assert torch.equal(ct.layer_norm_backward(dy, x, mean, rstd, w, need_dweight=False, need_dbias=False)[0], dx)
+
+
+@pytest.mark.parametrize("how", ["x", "weight", "bias"])
+@pytest.mark.parametrize("wt,bt", [(bf16, f32), (f16, f32), (f16, bf16), (f32, bf16), (None, f16), (f32, f32)])
+def test_each_gradient_in_its_own_type(ct, dev, wt, bt, how):
+    """Rows, weight or bias that lie apart take another way to the same kernels than contiguous ones: gradients are the same bits, and a bias's
+    sum is rounded once, to the bias's type, whatever the weight's (sums here go to 1e5, beyond fp16's largest number)."""
+    if how == "weight" and wt is None:
+        pytest.skip("no weight")
+    B, S, H = 10, 100, 300
+    big = 100.0 if bt != f16 else 1.0
+    dy = make(dev, B * S, H, f32, 31, 1.0, big).view(B, S, H)
+    base = make(dev, S * B, H, f32, 32, 2.0, 0.5).view(S, B, H)
+    w0, b0 = vectors(dev, H, f32)
+    w0, b0 = None if wt is None else w0.to(wt), b0.to(bt)
+    apart = lambda t: torch.stack((t, t), -1)[..., 0]  # noqa: E731
+
+    def grads(strided):
+        x = base.transpose(0, 1) if strided and how == "x" else base.transpose(0, 1).contiguous()
+        w, b = w0, b0
+        if strided and how == "weight":
+            w = apart(w)
+        if strided and how == "bias":
+            b = apart(b)
+        leaves = [t.detach().requires_grad_() if t is not None else None for t in (x, w, b)]
+        assert not strided or not leaves[["x", "weight", "bias"].index(how)].is_contiguous()
+        ct.layer_norm(*leaves).backward(dy)
+        return [None if t is None else t.grad for t in leaves]
+
+    want, off = backward(dy.reshape(-1, H), base.transpose(0, 1).reshape(-1, H), w0, 1e-5)
+    plain, strided = grads(False), grads(True)
+    for g, p, t, o, typ in zip(strided, plain, want, off, (f32, wt, bt)):
+        if g is not None:
+            assert g.dtype == typ and torch.equal(g, p)
+            if typ != f16 or float(t.abs().max()) < 65000:
+                near(g.reshape(t.shape), t, o, typ)
+    assert bool(torch.isfinite(strided[2]).all())
