@@ -86,7 +86,7 @@ def _backward(dy, x, mean, rstd, weight, need_dx, need_dweight, need_dbias, bias
         raise TileTypeError(f"dy must have the dtype of x ({_dtype_name(x.dtype)}), got {_dtype_name(dy.dtype)}")
     if dy.shape != x.shape:
         raise ValueError(f"dy must have the shape of x {tuple(x.shape)}, got {tuple(dy.shape)}")
-    x2, dy2, w = _rows(x.detach()), _rows(dy.detach()), _vector(weight)
+    x2, dy2, w, m2, r2 = _rows(x.detach()), _rows(dy.detach()), _vector(weight), _vector(mean), _vector(rstd)
     T, H = x2.shape
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or tuple(t.shape) != (T,):
@@ -99,7 +99,7 @@ def _backward(dy, x, mean, rstd, weight, need_dx, need_dweight, need_dbias, bias
         lib = L.lib()
         need = lib.mx_layer_norm_backward_workspace_bytes(T, H)
         ws = _workspace(dev, need)
-        _call(dev, lib.mx_layer_norm_backward, _ref(dy2), _ref(x2), _ref(mean.contiguous()), _ref(rstd.contiguous()), _opt(w), _opt(dx), _opt(dw), _opt(db),
+        _call(dev, lib.mx_layer_norm_backward, _ref(dy2), _ref(x2), _ref(m2), _ref(r2), _opt(w), _opt(dx), _opt(dw), _opt(db),
               ws.data_ptr(), need)
     return (dx.reshape(x.shape) if need_dx else None), dw, db
 

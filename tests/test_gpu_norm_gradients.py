@@ -3,6 +3,7 @@ fill their threads, and gradients of weight and bias that are of different types
 import pytest
 import torch
 
+from cutile_amd import norm
 from test_gpu_norm import SUM, backward, d64, make, near, vectors
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +68,24 @@ def test_each_gradient_in_its_own_type(ct, dev, wt, bt, how):
             if typ != f16 or float(t.abs().max()) < 65000:
                 near(g.reshape(t.shape), t, o, typ)
     assert bool(torch.isfinite(strided[2]).all())
+
+
+def test_statistics_that_lie_apart(ct, dev, monkeypatch):
+    """mean and rstd as columns of one tensor: the copies that are made of them are held until the kernel has been enqueued, so that nobody else on
+    the stream gets their memory before."""
+    x, dy = make(dev, 300, 700, bf16, 41, 2.0, 0.5), make(dev, 300, 700, bf16, 42)
+    w, b = vectors(dev, 700, f32)
+    _, mean, rstd = ct.layer_norm_forward(x, w, b)
+    want = ct.layer_norm_backward(dy, x, mean, rstd, w)
+    both = torch.stack((mean, rstd), -1)
+    assert not both[:, 0].is_contiguous()
+    real = norm._call
+
+    def call(dev, f, *args):
+        others = [torch.full((300,), float("nan"), device=dev) for _ in range(64)]
+        real(dev, f, *args)
+        del others
+
+    monkeypatch.setattr(norm, "_call", call)
+    got = ct.layer_norm_backward(dy, x, both[:, 0], both[:, 1], w)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
