@@ -578,6 +578,12 @@ PyObject* py_silu_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 struct Refused { int rc; };   // by the library, before anything was enqueued
+// an input of forward-mode differentiation, which no operator here has: the Python side refuses it
+bool has_tangent(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
+  return false;
+}
 struct FfnSizes { int64_t T, H, F, Ho; };
 // the block's operands as matrices; false: not for the native path
 bool ffn_operands(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, mx_tensor* dx, mx_tensor* d1, mx_tensor* d2, FfnSizes* s) {
@@ -674,6 +680,7 @@ PyObject* py_feed_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   FfnSizes s;
   if (!ffn_operands(x, w1, w2, &dx, &d1, &d2, &s)) Py_RETURN_NONE;
   const int mode = (int)PyLong_AsLong(a[3]), form = (int)PyLong_AsLong(a[4]);
+  if (form != 1 && has_tangent({&x, &w1, &w2})) Py_RETURN_NONE;
   if (form == 2 && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) Py_RETURN_NONE;
   at::Tensor y, saved;
   int rc = MX_OK;
@@ -851,6 +858,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
   mx_tensor dx, dw, db;
   if (!norm_operands(x, w, b, &dx, &dw, &db)) Py_RETURN_NONE;
+  if (form != 1 && has_tangent({&x, &w, &b})) Py_RETURN_NONE;
   if (form == 2 && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) Py_RETURN_NONE;
   at::Tensor y, mean, rstd;
   int rc = MX_OK;
@@ -1078,6 +1086,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   LinearSizes s;
   if (!linear_operands(x, w, bias, res, &dx, &dw, &db, &dr, &s)) Py_RETURN_NONE;
   const int act = (int)PyLong_AsLong(a[4]), mode = (int)PyLong_AsLong(a[5]), form = (int)PyLong_AsLong(a[6]);
+  if (form != 1 && has_tangent({&x, &w, &bias, &res})) Py_RETURN_NONE;
   if (form == 2 && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) Py_RETURN_NONE;
   at::Tensor y, saved;
   int rc = MX_OK;

@@ -40,6 +40,13 @@ def _same_device(*tensors):
     return dev
 
 
+def _no_tangents(what, *tensors):
+    """Refuses inputs of forward-mode differentiation: a result without its tangent would be taken for a constant."""
+    for t in tensors:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
 def _call(dev, fn, *args):
     """fn(*args, stream) with `dev` as the current device, on its current stream."""
     if torch.cuda.current_device() == dev.index:
@@ -272,6 +279,8 @@ def _forward(x, w1, w2, mode: int, train: bool):
         _raise_code(r)
     if r is not None:
         return r if train else (r, None)
+    if not train:
+        _no_tangents("gated_feed_forward", x, w1, w2)
     dev, H, F, H_out = _check_block(x, w1, w2)
     x2, w1, w2 = _rows(x.detach()), _rows(w1.detach()), _rows(w2.detach())
     T = x2.shape[0]
@@ -360,7 +369,7 @@ def gated_feed_forward(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, *, s
 
     With gradients enabled the call refuses to be captured into a HIP graph (autograd accumulates a leaf's gradient on the
     stream that first used it, which a capture must not touch): capture :func:`gated_feed_forward_forward` and
-    :func:`gated_feed_forward_backward`."""
+    :func:`gated_feed_forward_backward`.  Inputs of forward-mode differentiation are refused."""
     mode = _mode(scale_mode)
     if not (torch.is_grad_enabled() and (x.requires_grad or w1.requires_grad or w2.requires_grad)):
         return _forward(x, w1, w2, mode, False)[0]
@@ -369,6 +378,7 @@ def gated_feed_forward(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, *, s
         _raise_code(r)
     if r is not None:
         return r
+    _no_tangents("gated_feed_forward", x, w1, w2)
     if x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("gated_feed_forward with gradients cannot be captured into a graph: capture "
                            "gated_feed_forward_forward and gated_feed_forward_backward")

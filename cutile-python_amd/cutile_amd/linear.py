@@ -17,7 +17,7 @@ import torch
 
 from . import _lib as L
 from .errors import TileTypeError, TileValueError
-from .ffn import _FLOATS, _call, _codes, _mode, _ref, _rows, _same_device
+from .ffn import _FLOATS, _call, _codes, _mode, _no_tangents, _ref, _rows, _same_device
 from .ops import _DTYPE_FMT, _FMT_CODE, PackedScales, _as_u8, _dtype_name, _elem_format, _opts, _raise_code, _scale_code, _scale_desc, _workspace
 
 _ACTS = {None: L.MX_ACT_NONE, "relu": L.MX_ACT_RELU, "gelu": L.MX_ACT_GELU, "gelu_tanh": L.MX_ACT_GELU_TANH, "silu": L.MX_ACT_SILU}
@@ -139,6 +139,8 @@ def _forward(x, w, bias, residual, act: int, mode: int, train: bool):
         _raise_code(r)
     if r is not None:
         return r if train else (r, None)
+    if not train:
+        _no_tangents("linear", x, w, bias, residual)
     dev, K, N = _check(x, w, bias, residual)
     x2, w2, b2 = _rows(x.detach()), _rows(w.detach()), None if bias is None else bias.detach().contiguous()
     r2 = None if residual is None else _rows(residual.detach())
@@ -228,7 +230,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     the largest number of its block, so gradients made of it may be finite; ``scale_mode="ceil"`` makes its block NaN.
 
     With gradients enabled the call refuses to be captured into a HIP graph (autograd accumulates a leaf's gradient on the stream that
-    first used it, which a capture must not touch): capture :func:`linear_forward` and :func:`linear_backward`."""
+    first used it, which a capture must not touch): capture :func:`linear_forward` and :func:`linear_backward`.  Inputs of forward-mode
+    differentiation are refused."""
     act, mode = _act(activation), _mode(scale_mode)
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual))):
         return _forward(x, w, bias, residual, act, mode, False)[0]
@@ -237,6 +240,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
         _raise_code(r)
     if r is not None:
         return r
+    _no_tangents("linear", x, w, bias, residual)
     if x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("linear with gradients cannot be captured into a graph: capture linear_forward and linear_backward")
     return _Linear.apply(x, w, bias, residual, activation, scale_mode)

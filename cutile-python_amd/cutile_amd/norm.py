@@ -17,7 +17,7 @@ import torch
 
 from . import _lib as L
 from .errors import TileTypeError, TileValueError
-from .ffn import _ELEM8, _FLOATS, _call, _mode, _ref, _rows, _same_device, _up32
+from .ffn import _ELEM8, _FLOATS, _call, _mode, _no_tangents, _ref, _rows, _same_device, _up32
 from .ops import _DTYPE_FMT, _FMT_CODE, _dtype_name, _raise_code, _workspace
 
 
@@ -51,6 +51,8 @@ def _forward(x, weight, bias, eps, stats):
         _raise_code(r)
     if r is not None:
         return r if stats else (r, None, None)
+    if not stats:
+        _no_tangents("layer_norm", x, weight, bias)
     dev, H = _check(x, weight, bias, eps)
     x2, w, b = _rows(x.detach()), _vector(weight), _vector(bias)
     T = x2.shape[0]
@@ -128,7 +130,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     the differences from the mean.  A row with a NaN or an infinity is NaN.
 
     With gradients enabled the call refuses to be captured into a HIP graph (autograd accumulates a leaf's gradient on the stream that
-    first used it, which a capture must not touch): capture :func:`layer_norm_forward` and :func:`layer_norm_backward`."""
+    first used it, which a capture must not touch): capture :func:`layer_norm_forward` and :func:`layer_norm_backward`.  Inputs of
+    forward-mode differentiation are refused."""
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))):
         return _forward(x, weight, bias, eps, False)[0]
     r = L.host().layer_norm(x, weight, bias, eps, 2)
@@ -136,6 +139,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         _raise_code(r)
     if r is not None:
         return r
+    _no_tangents("layer_norm", x, weight, bias)
     if x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("layer_norm with gradients cannot be captured into a graph: capture layer_norm_forward and layer_norm_backward")
     return _LayerNorm.apply(x, weight, bias, eps)
