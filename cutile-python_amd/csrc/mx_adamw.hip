@@ -213,8 +213,9 @@ hipError_t launch(const AdamArgs& a, int64_t chunks, bool small, hipStream_t str
 }
 
 typedef std::vector<std::pair<uintptr_t, uintptr_t>> Ranges;
-// (the lists are sorted and joined)
-bool overlap(Ranges (&lists)[6]) {
+// Of the ranges in the lists, two with one another (1), or one with one of `read` (2), which may overlap among themselves.  (The lists are sorted and
+// joined.)
+int overlap(Ranges (&lists)[6], Ranges& read) {
   for (Ranges& l : lists)
     if (!std::is_sorted(l.begin(), l.end())) std::sort(l.begin(), l.end());
   std::sort(lists, lists + 6);   // by their first range, empty ones in front
@@ -228,8 +229,14 @@ bool overlap(Ranges (&lists)[6]) {
     if (mid > 0 && mid < all.size() && all[mid] < all[mid - 1]) std::inplace_merge(all.begin(), all.begin() + mid, all.end());
   }
   for (size_t i = 1; i < all.size(); ++i)
-    if (all[i].first < all[i - 1].second) return true;
-  return false;
+    if (all[i].first < all[i - 1].second) return 1;
+  if (!std::is_sorted(read.begin(), read.end())) std::sort(read.begin(), read.end());
+  size_t k = 0;
+  for (const auto& r : read) {
+    while (k < all.size() && all[k].second <= r.first) ++k;
+    if (k < all.size() && all[k].first < r.second) return 2;
+  }
+  return 0;
 }
 int check_adamw(int32_t count, const mx_adamw_tensor* list, const mx_adamw_opts& o) {
   if (o.state_bits != 8 && o.state_bits != 32) return set_error(MX_ERR_INVALID, "states have 8 or 32 bits (got %d)", o.state_bits);
@@ -243,7 +250,14 @@ int check_adamw(int32_t count, const mx_adamw_tensor* list, const mx_adamw_opts&
   if (!o.scale_at && !within(o.grad_scale, -3e38, 3e38)) return set_error(MX_ERR_INVALID, "the gradients' scale must be a number");
   // What is written, a list for each kind: as a rule ascending, as its tensors were allocated.  (200 tensors: a step takes 28 us of host time, with
   // all of it sorted at once 40.)
-  Ranges written[6];
+  Ranges written[6], read;
+  read.reserve((size_t)count + 3);
+  auto reads = [&](const void* p, int64_t bytes) {
+    if (p) read.emplace_back((uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes);
+  };
+  reads(o.lr_at, 4);
+  reads(o.step_at, 8);
+  reads(o.scale_at, 4);
   for (int k = 0; k < (o.state_bits == 8 ? 6 : 4); ++k) written[k].reserve(count);
   for (int32_t i = 0; i < count; ++i) {
     const mx_adamw_tensor& t = list[i];
@@ -262,6 +276,7 @@ int check_adamw(int32_t count, const mx_adamw_tensor* list, const mx_adamw_opts&
     auto writes = [&](int k, const void* p, int64_t bytes) {
       if (p) written[k].emplace_back((uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes);
     };
+    reads(t.grad, t.n * (t.grad_dtype == MX_F32 ? 4 : 2));
     writes(0, t.param, t.n * (t.param_dtype == MX_F32 ? 4 : 2));
     writes(1, t.exp_avg, state);
     writes(2, t.exp_avg_sq, state);
@@ -271,7 +286,9 @@ int check_adamw(int32_t count, const mx_adamw_tensor* list, const mx_adamw_opts&
       writes(5, t.exp_avg_sq_scale, state / 32);
     }
   }
-  return overlap(written) ? set_error(MX_ERR_INVALID, "parameters, states and copies must not overlap (is a tensor listed twice?)") : MX_OK;
+  const int bad = overlap(written, read);
+  if (bad == 1) return set_error(MX_ERR_INVALID, "parameters, states and copies must not overlap (is a tensor listed twice?)");
+  return bad ? set_error(MX_ERR_INVALID, "parameters, states and copies must not overlap a gradient, nor a step, rate or scale that the kernel reads") : MX_OK;
 }
 
 }  // namespace

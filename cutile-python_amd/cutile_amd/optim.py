@@ -67,7 +67,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     With 8-bit states (:func:`adamw_state`) elements are rounded up or down at random, since a step of ``b2`` = 0.999 is far
     smaller than the distance of two E4M3 numbers; the random bits are a hash of ``seed``, ``step``, the place in the list and
     the element, the same for the same arguments.  All states of a call have the same number of bits.  Parameters, states and copies must
-    not overlap: a parameter listed twice is refused.  A NaN or an infinity of a gradient reaches its parameter, and with 8-bit states the 31
+    not overlap one another (a parameter listed twice is refused) nor what the kernel reads beside them: a gradient, or a ``step``, ``lr`` or
+    ``grad_scale`` on the device; gradients may be the same.  A NaN or an infinity of a gradient reaches its parameter, and with 8-bit states the 31
     states that share its scale."""
     beta1, beta2 = betas
     r = L.host().adamw(params, grads, states, copies, step, lr, beta1, beta2, eps, weight_decay, grad_scale, seed)

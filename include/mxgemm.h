@@ -509,7 +509,8 @@ MX_API int mx_layer_norm_backward(const mx_tensor* dy, const mx_tensor* x, const
  *     the two neighbours gives: the random bits are a hash of seed, step, place in the list and element, so that a call can be
  *     repeated.  A root above zero is never stored as zero.  Zeros (elements and scales) are the state to begin with.
  * lr_at, step_at, scale_at: device addresses of lr, step and grad_scale, or NULL; what is given there is read by the kernel, so that a
- * captured graph can go on counting.  Parameters, states and copies must not overlap one another, nor a gradient.
+ * captured graph can go on counting.  Parameters, states and copies that overlap one another, a gradient or what is at these
+ * addresses are refused (the tensors' workgroups run in any order); gradients may overlap.
  */
 typedef struct mx_adamw_tensor {
   void* param;                 /* MX_F32 | MX_BF16 */
