@@ -1016,11 +1016,15 @@ at::Tensor linear_forward(const at::Tensor& x, const at::Tensor& w, const at::Te
   return y;
 }
 // dx, dw, dbias (undefined where not asked for) from dy [T, N]
-std::vector<at::Tensor> linear_backward(const at::Tensor& dy, const at::Tensor& saved, const LinearSizes& s, const at::ScalarType (&types)[3],
+std::vector<at::Tensor> linear_backward(at::Tensor dy, const at::Tensor& saved, const LinearSizes& s, const at::ScalarType (&types)[3],
                                         const bool (&want)[3], int act, int mode) {
   const at::Device dev = dy.device();
   mx_tensor d{};
   if (!matrix(dy, float_code(dy.scalar_type()), &d)) throw Refused{0};
+  if (s.T > 1 && d.stride[0] > (int64_t)1 << 25) {   // rows farther apart than the library takes them
+    dy = dy.contiguous();
+    matrix(dy, d.dtype, &d);
+  }
   std::vector<at::Tensor> out(3);
   mx_tensor od[3];
   for (int i = 0; i < 3; ++i)

@@ -189,6 +189,8 @@ def linear_backward(dy: torch.Tensor, state: LinearState, *, need_dx: bool = Tru
     if s.T and (need_dx or need_dw or need_dbias):
         lib = L.lib()
         dy2 = _rows(dy.detach())
+        if s.T > 1 and dy2.stride(0) > 1 << 25:    # rows farther apart than the library takes them
+            dy2 = dy2.contiguous()
         need = lib.mx_linear_backward_workspace_bytes(s.T, s.K, s.N)
         ws = _workspace(dev, need)
         _call(dev, lib.mx_linear_backward, _ref(dy2), s.saved.data_ptr(), s.saved.numel(), s.K, act, _opt(dx), _opt(dw), _opt(db), _mode(s.scale_mode),

@@ -45,3 +45,23 @@ def test_fp4_packed_along_the_rows(dev, M, columns):
     exact = A @ W.T
     # 64 products and the sum's roundings in 32 bits
     assert bool(((want.cpu().double() - exact).abs() <= 66 * 2.0 ** -24 * (A.abs() @ W.abs().T)).all())
+
+
+# ---- gradients ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T", [2, 3])
+@pytest.mark.parametrize("pitch", [1 << 25, (1 << 25) + 1, (1 << 25) + 64])
+def test_gradient_whose_rows_lie_far_apart(ct, dev, pitch, T):
+    K, N = 96, 64
+    g = torch.Generator().manual_seed(T)
+    x, w, b = ((torch.randn(s, generator=g)).to(bf16).to(dev) for s in ((T, K), (N, K), (N,)))
+    room = torch.zeros((T - 1) * pitch + N, dtype=bf16, device=dev)
+    far = room.as_strided((T, N), (pitch, 1))
+    near = torch.randn((T, N), generator=g).to(bf16).to(dev)
+    far.copy_(near)
+    _, state = ct.linear_forward(x, w, b, activation="gelu")
+    want = ct.linear_backward(near, state)
+    for got in (ct.linear_backward(far, state), ct.linear_backward(far.unsqueeze(0), state)):
+        assert all(torch.equal(p.reshape(q.shape), q) for p, q in zip(got, want))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    got = torch.autograd.grad(ct.linear(*leaves, activation="gelu"), leaves, far)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
