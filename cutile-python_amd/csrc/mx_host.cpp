@@ -1052,13 +1052,15 @@ struct Linear : torch::autograd::Function<Linear> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const bool again = at::GradMode::is_enabled();
-    at::AutoDispatchBelowADInplaceOrView below;
     const auto v = ctx->saved_data["sizes"].toIntVector();
     const bool has_b = v[7] >= 0, has_r = v[8] >= 0;
+    const bool want_r = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
+    at::Tensor dr;
+    if (want_r) dr = grads[0].to((at::ScalarType)v[8]);   // (recorded, if a graph of the gradients is asked for: this one has one)
+    at::AutoDispatchBelowADInplaceOrView below;
     const at::ScalarType types[3] = {(at::ScalarType)v[5], (at::ScalarType)v[6], has_b ? (at::ScalarType)v[7] : at::kFloat};
     // (edges are counted over the tensors that there are)
     const bool want[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), has_b && ctx->needs_input_grad(2)};
-    const bool want_r = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
     at::Tensor dy = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({v[0], v[2]});
     if (dy.stride(1) != 1 || dy.stride(0) < 0) dy = dy.contiguous();
     std::vector<at::Tensor> r(3);
@@ -1072,7 +1074,7 @@ struct Linear : torch::autograd::Function<Linear> {
     const auto shape = ctx->saved_data["x"].toIntVector();
     if (want[0] && shape.size() != 2) r[0] = r[0].view(shape);
     if (again) r = without_graph(std::move(r), "linear: its gradients cannot be differentiated");
-    r.push_back(want_r ? grads[0].to((at::ScalarType)v[8]) : at::Tensor());
+    r.push_back(dr);
     r.emplace_back();
     r.emplace_back();
     return r;

@@ -65,3 +65,22 @@ def test_gradient_whose_rows_lie_far_apart(ct, dev, pitch, T):
     leaves = [t.requires_grad_() for t in (x, w, b)]
     got = torch.autograd.grad(ct.linear(*leaves, activation="gelu"), leaves, far)
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("T", [40, 600])
+@pytest.mark.parametrize("xt,rt", [(bf16, f32), (bf16, f16), (f32, bf16), (bf16, bf16)], ids=str)
+def test_graph_of_the_residuals_gradient(ct, dev, T, xt, rt):
+    """The residual's gradient is dy, in the residual's type: its graph is that of dy.  The others have none and say so."""
+    K, N = 64, 96
+    g = torch.Generator().manual_seed(7)
+    x, w, b = ((torch.randn(s, generator=g)).to(xt).to(dev).requires_grad_() for s in ((T, K), (N, K), (N,)))
+    r = torch.randn((T, N), generator=g).to(rt).to(dev).requires_grad_()
+    dy = torch.randn((T, N), generator=g).to(xt).to(dev).requires_grad_()
+    weight = torch.randn((T, N), generator=g).to(rt).to(dev)
+    dx, dw, db, dr = torch.autograd.grad(ct.linear(x, w, b, r, activation="silu"), (x, w, b, r), dy, create_graph=True)
+    assert dr.dtype == rt and torch.equal(dr.detach(), dy.detach().to(rt))
+    (back,) = torch.autograd.grad((dr * weight).sum(), dy)
+    assert torch.equal(back, weight.to(xt))
+    for t in (dx, dw, db):
+        with pytest.raises(RuntimeError, match="cannot be differentiated"):
+            t.sum().backward(retain_graph=True)
