@@ -5,7 +5,10 @@
 //   silu       x s(x),  s(z) = 1 / (1 + exp(-z))
 //   gelu_tanh  x s(2 c (x + 0.044715 x^3)),  c = sqrt(2 / pi): the same form, its argument x (k1 + k3 x^2)
 //   gelu       x P(X < x) = max(x, 0) - |x| q(|x|),  q(a) = erfc(a / sqrt 2) / 2 = exp(-a^2 / 2) t (c1 + c2 t + .. + c7 t^6) with t = 1 / (1 + 0.35 a):
-//              fitted to 2.6e-7 of the value up to a = 7 (4e-5 up to 14, where q is 1e-44); exp's argument rounds to 1e-6 there
+//              fitted to 2.6e-7 of the value up to a = 7 (3.5e-5 up to 12.75, where x q is 2e-36, 4.4e-5 up to 14)
+// Each is within 2e-6 + 2.5e-7 |z| of its value (gelu beyond 7: the fit's error more), exp(-|z|) the exponential in it: z is off by its roundings and
+// those of its constants, by 2.3e-7 of it at most (gelu_tanh), and so is the exponential, relatively, by that much.  Where 1 / (1 + exp(-z)) or q is below
+// 2^-126 it is zero: so may be numbers below 2e-36.
 // Bound, in a large product: this arithmetic, which little of the product runs beside (8192 x 14336 x 4096 on the ping-pong kernel, to bf16: plain
 // product 338 us, bias 348, silu 368, gelu 390); in a small one the launch (1 x 8192 x 2048: 4.8 and 5.1 to 5.5).
 // Far out a factor is 0 or 1, and x ends at -126 in front of it: -inf makes -0 of silu and gelu (inf times 0 is NaN; x^2 ends at 1e30 for

@@ -8,6 +8,7 @@ import torch
 from cutile_amd import _lib as L
 from mxutil import randn_operand
 from oracle import mx_oracle as O
+from test_gpu_linear import d64
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +85,39 @@ def test_graph_of_the_residuals_gradient(ct, dev, T, xt, rt):
     for t in (dx, dw, db):
         with pytest.raises(RuntimeError, match="cannot be differentiated"):
             t.sum().backward(retain_graph=True)
+
+
+# ---- the activations alone ----------------------------------------------------------------------------------------------------
+def exponent(p, act):
+    """|z| of the exponential exp(-|z|) that an activation has in it."""
+    return {"silu": p.abs(), "gelu": p * p / 2, "gelu_tanh": (2 * (2 / torch.pi) ** 0.5 * (p + 0.044715 * p ** 3)).abs()}[act]
+
+
+def act_exact(p, act):
+    """The activation where tanh(z / 2) + 1 and the like have lost their bits: x s(z) through exp."""
+    if act == "gelu":
+        return p * 0.5 * torch.special.erfc(-p * 0.5 ** 0.5)
+    z = p if act == "silu" else 2 * (2 / torch.pi) ** 0.5 * (p + 0.044715 * p ** 3)
+    return p * torch.sigmoid(z)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("kernel,M", [("stream", 1), ("stream", 40), ("mfma128", 200), ("pingpong", 300), ("generic", 2), ("auto", 70)])
+def test_activation_to_its_stated_precision(ct, dev, kernel, M, act):
+    """A product of zero and an fp32 result leave act(bias): within 2e-6 + 2.5e-7 |z| of its value, gelu below -7 within 4e-5 more; numbers below
+    2e-36 may be zero.  (z: roundings of x^2, of its product and sum, of the last product, 2^-24 each, and constants off by 5e-8, are
+    2.3e-7 of it at most, and so much of the exponential.  The rest: 2^x and reciprocals 2^-23 each, some 2^-24, gelu's fit 2.6e-7 up to 7 and
+    3.5e-5 up to 12.75, from where on numbers are below 2e-36.)"""
+    K, N = 256, 4096
+    for lo, hi in ((-100.0, 100.0), (-14.0, 4.0), (-2.0, 2.0), (-1e-3, 1e-3)):
+        bias = torch.linspace(lo, hi, N, dtype=f32, device=dev)
+        a, w = torch.zeros((M, K), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn), torch.zeros((N, K), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+        one = lambda rows: torch.full((rows, K // 32), 127, dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu)  # noqa: E731
+        y = d64(ct.block_scaled_linear(a, one(M), w, one(N), bias, activation=act, out_dtype=f32, kernel=kernel))
+        p = d64(bias)
+        want = act_exact(p, act)
+        err = (2e-6 + 2.5e-7 * exponent(p, act)) * want.abs()
+        if act == "gelu":
+            err = err + torch.where(p < -7, 4e-5, 0.0) * want.abs()
+        bad = ~((y - want).abs() <= err + 2e-36)
+        assert not bool(bad.any()), (p[bad[0]][:4].tolist(), y[0][bad[0]][:4].tolist(), want[bad[0]][:4].tolist())
