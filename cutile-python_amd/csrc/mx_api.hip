@@ -669,12 +669,14 @@ int gemm_impl(const mx_tensor* A, const mx_tensor* As, const mx_tensor* B, const
     return set_error(MX_ERR_LAYOUT, "split_k = %d is only available on the one-tile MFMA kernels (kernel %d chosen)",
                      o.split_k, kernel);
   if (lin) {
-    // the decode kernel has no such epilogue.  A pass behind it costs 3 us, which it makes up for with many weights alone (32 rows, 28672 x 8192:
-    // 26 us against 31 streamed; 16384 x 8192: 19.7 against 17.6, 14336 x 4096: 11.5 against 10.3; 1 row, 28672 x 8192: 23.5 both)
+    // the decode kernel has no such epilogue.  A pass behind it costs 3 us, which it makes up for with more than 8 rows of many weights (streamed | product and
+    // pass, us: 28672 x 8192, 1, 8, 16, 32 rows 24.8 | 26.7, 26.0 | 26.8, 27.6 | 27.1, 32.6 | 28.3; 24576 x 8192 23.6 | 23.9, 24.9 | 24.4, 26.8 | 24.5, 32.0 | 25.5;
+    // 16384 x 8192 19.9 | 19.7, 20.0 | 20.0, 19.9 | 20.0, 22.7 | 20.8; 14336 x 4096 10.6 | 13.0, 10.7 | 13.1, 11.1 | 13.4, 12.9 | 14.0)
     if (kernel == MX_KERNEL_DECODE && o.kernel == MX_KERNEL_AUTO && !why_stream && !(M > 8 && N * K >= (int64_t)192 << 20)) kernel = MX_KERNEL_STREAM;
     const bool whole = K % 128 == 0 && K >= 256;
     const bool pp = ((A->dtype == MX_E4M3 && (B->dtype == MX_E4M3 || B->dtype == MX_E2M1) && whole) || (A->dtype == MX_E2M1 && B->dtype == MX_E2M1)) && linear_is_plain(*lin, M);
-    // (8192 x 14336 x 4096 with an fp32 result, which once was such a case: 568 us so, 1119 through memory, some rows at a time)
+    // (gelu to bf16, 8192 x 14336 x 4096: here 393 us, in the 128 x 128 kernel 521, through memory, some rows at a time, 1824 of E5M2; K = 4128, which leaves a
+    // step of it unfinished and would take the masked body, half of a kernel's code again: 632 in the 128 x 128 kernel, 2330 through memory, the plain product 404)
     if (kernel == MX_KERNEL_MFMA_PINGPONG && o.kernel == MX_KERNEL_AUTO && !pp) kernel = MX_KERNEL_MFMA_128x128;
     const bool fused = kernel == MX_KERNEL_STREAM || kernel == MX_KERNEL_MFMA_128x128 || (kernel == MX_KERNEL_MFMA_PINGPONG && pp);
     if (!fused) return kLinearNotFused;

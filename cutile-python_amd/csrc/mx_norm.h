@@ -20,7 +20,7 @@ struct NormBackwardArgs {
   const void *dy, *x, *w;            // w may be null
   const float *mean, *rstd;
   void *dx, *dw, *db;                // each may be null
-  float* partial;                    // norm_backward_partials() rows of dw and db
+  float* partial;                    // rows of dw and db, one for each workgroup: norm_backward_bytes()
   int64_t dy_ld, x_ld, dx_ld;
   int32_t rows, H, x_dtype, w_dtype, dw_dtype, db_dtype;
 };

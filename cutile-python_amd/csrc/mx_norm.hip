@@ -3,7 +3,7 @@
 //   mean = sum x / H,  rstd = 1 / sqrt(sum (x - mean)^2 / H + eps),  y = (x - mean) rstd w + b
 //   h = dy w,  xhat = (x - mean) rstd:  dx = rstd (h - mean(h) - xhat mean(h xhat)),  dw = sum_rows dy xhat,  db = sum_rows dy
 //
-// Bound: memory.  A row stays in the registers of its threads, a wave up to 2048 elements, a workgroup beyond, so that it is read once
+// Bound: memory.  A row stays in the registers of its threads, a wave's up to 1024 elements, those of two to sixteen waves beyond, so that it is read once
 // and the second moment is that of the differences from the mean (of x^2 - mean^2 nothing is left where the mean is large).  Threads
 // keep their columns for all of their rows: weight and bias are loaded once, and the gradients of both are summed in
 // registers; each workgroup leaves one row of partial sums, which a second launch adds up in their order.
@@ -45,7 +45,8 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* red, int& slot) {
 }
 
 // what a row's result becomes.  E4M3 under the floor rule has an instance of its own, by the hardware's conversions alone
-// (1531 x 8192 with encode_block in all of them: 23.9 us): the other formats and the ceiling rule share encode_block.
+// (1531 x 8192, calls one after another on inputs that are in no cache: 13.9 us; by the ceiling rule, with encode_block, 17.2, E5M2 17.7): the
+// other formats and the ceiling rule share encode_block.
 enum { kNormFloats, kNormE4M3, kNormCodes };
 
 // codes and scale byte of a piece whose block's other elements are in the neighbouring lanes (OUT kNormE4M3: conversions saturate)
@@ -153,7 +154,7 @@ __global__ __launch_bounds__(GT == 64 ? 256 : GT) void norm_kernel(const NormArg
   }
 }
 
-// rows that do not fit into a workgroup's registers: read three times, from L2 after the first (1024 x 32768 bf16 41 us; with 32 elements to a
+// rows that do not fit into a workgroup's registers: read three times, from L2 after the first (1024 x 32768 bf16 43 us; with 32 elements to a
 // thread, which spill, 49)
 constexpr int kLongThreads = 1024;
 template <int T, int OUT>
@@ -390,8 +391,8 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const NormBackwardArg
   store_float(out, which ? a.db_dtype : a.dw_dtype, col, s);
 }
 
-// S and the threads of a row by its length: 16 elements to a thread.  (With 32, fewer threads and fewer barriers, 1531 x 8192 takes 15.4 us
-// where this takes 13.6, fp32 8192 x 2048 35 and 24; with 8 up to 8192 elements the same as this.)
+// S and the threads of a row by its length: 16 elements to a thread.  (With 32, fewer threads and fewer barriers, or 8 up to 8192, full occupancy:
+// 1531 x 8192 to E4M3 13.9 us, 16.2 and 14.2; fp32 8192 x 2048 25.5, 30.0 and 23.9; bf16 16384 x 4096 46.0, 47.7 and 47.4; inputs that are in no cache.)
 template <typename F>
 bool by_length(int64_t H, F&& f) {
 #define MX_CASE(MOST, S, GT) \

@@ -18,7 +18,7 @@ import torch
 from . import _lib as L
 from .errors import TileTypeError, TileValueError
 from .ffn import _FLOATS, _call, _codes, _mode, _no_tangents, _ref, _rows, _same_device
-from .ops import _DTYPE_FMT, _FMT_CODE, PackedScales, _as_u8, _dtype_name, _elem_format, _opts, _raise_code, _scale_code, _scale_desc, _workspace
+from .ops import _FMT_CODE, PackedScales, _as_u8, _dtype_name, _elem_format, _opts, _raise_code, _scale_code, _scale_desc, _workspace
 
 _ACTS = {None: L.MX_ACT_NONE, "relu": L.MX_ACT_RELU, "gelu": L.MX_ACT_GELU, "gelu_tanh": L.MX_ACT_GELU_TANH, "silu": L.MX_ACT_SILU}
 
@@ -55,7 +55,8 @@ def block_scaled_linear(A: torch.Tensor, A_scale, W: torch.Tensor, W_scale, bias
 
     Returns (M, N) in ``torch.bfloat16`` or ``torch.float32``, or with ``out_dtype`` ``torch.float8_e4m3fn`` ``(q, scale)``, quantised from
     the unrounded result by the floor rule (N a multiple of 32): the left operand of the next product.  Sums are the scaled matrix
-    instructions' (1.5e-5 of the result's norm), what is behind them is in 32 bits.  A NaN is NaN; gelu and silu of -inf are zero."""
+    instructions' (1.5e-5 of the result's norm; ``kernel="generic"`` sums in 32 bits, far slower), what is behind them is in 32 bits.  A NaN
+    is NaN; gelu and silu of -inf are zero."""
     act = _act(activation)
     if kernel in L.KERNELS:
         r = L.host().linear_gemm(A, A_scale, W, W_scale, bias, residual, a_format, w_format, out_dtype, act, L.KERNELS[kernel])

@@ -436,7 +436,7 @@ MX_API int mx_ffn_backward(const mx_tensor* dy, const void* saved, int64_t saved
  *   at multiples of 8 bytes: quantised by the floor rule from the unrounded result, the left operand of the next product
  *   pre [M,N] MX_BF16 or NULL: product + bias, for a backward pass
  * Sums as in mx_gemm (the scaled matrix instructions align an instruction's products with some 18 bits below the largest: 1.5e-5 of the
- * result's norm), everything behind them in 32 bits.  With exp(-|z|) the exponential in it (z = x of silu, 2 sqrt(2 / pi) (x + 0.044715 x^3) of
+ * result's norm; MX_KERNEL_GENERIC sums in 32 bits), everything behind them in 32 bits.  With exp(-|z|) the exponential in it (z = x of silu, 2 sqrt(2 / pi) (x + 0.044715 x^3) of
  * gelu_tanh, x^2 / 2 of gelu), the activation is within 2e-6 + 2.5e-7 |z| of its value, gelu below -7 within 4e-5 more; numbers below 2e-36 may be
  * zero.  act(-inf) is zero for gelu and silu; a block of out with a NaN has mx_quantize's scale and zeros.
  * Fused into the streaming kernel, the 128 x 128 one and, for operands of E4M3, E4M3 by E2M1 (K % 128 == 0) or E2M1, rows in whole 16-byte pieces and
