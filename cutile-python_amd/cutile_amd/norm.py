@@ -127,7 +127,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x (..., H), weight and bias (H,) or None (ones, zeros) are float32, bfloat16 or float16, of the same dtype or not; the result has
     that of x, every gradient that of what it is the gradient of.  In 32 bits with one rounding at the end; the variance is that of
-    the differences from the mean.  A row with a NaN or an infinity is NaN.
+    the differences from the mean.  A row with a NaN or an infinity is NaN, and one whose sum passes 3.4e38; where the sum of the squared differences
+    does (differences around 1e19), 1 / sqrt of it is zero.
 
     With gradients enabled the call refuses to be captured into a HIP graph (autograd accumulates a leaf's gradient on the stream that
     first used it, which a capture must not touch): capture :func:`layer_norm_forward` and :func:`layer_norm_backward`.  Inputs of

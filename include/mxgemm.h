@@ -475,7 +475,8 @@ MX_API int mx_linear_backward(const mx_tensor* dy, const void* saved, int64_t sa
  *   x [rows,H] MX_F32 | MX_BF16 | MX_F16, rows contiguous, of any alignment and pitch; H at least 1
  *   weight, bias [H] of any of these types, each may be NULL (ones, zeros)
  *   y [rows,H] of x's type; mean, rstd [rows] MX_F32, each may be NULL
- * In 32 bits, one rounding at the end; a row with a NaN or an infinity is NaN.
+ * In 32 bits, one rounding at the end; a row with a NaN or an infinity is NaN.  So is one whose sum passes 3.4e38; where the squared differences from the
+ * mean do, rstd is zero.
  */
 MX_API int mx_layer_norm(const mx_tensor* x, const mx_tensor* weight, const mx_tensor* bias, double eps, mx_tensor* y, mx_tensor* mean,
                   mx_tensor* rstd, void* stream);
